@@ -534,6 +534,47 @@ int melgpt_conv1d_out1_fused(const void* h, const float* w, const float* bias, f
 int melgpt_resblock_narrow(const void* x, void* y, const void* wfrag, const float* b3, const float* b1s, int B, int L,
                            int C, int dilation, float slope, int dtype, void* stream);
 
+/* ===================================================================== packed and cached sequences
+ * Attention at lengths, head layouts and batches the fixed-size kernels above are not built for (they hold one whole
+ * sequence of at most 288 positions in LDS, head size 64, as many key heads as query heads, one length per batch).
+ * Rows of q, k, v are (row, head, value) tensors: row and head strides in elements, unit inner stride, 16-byte aligned;
+ * outputs are contiguous unless a stride is given.  Hk key heads serve Hq = G * Hk query heads, query head h reading key
+ * head h / G.
+ *
+ * Per-head RMS norm and position rotation of queries and keys in one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * weight      (skipped when both weights are NULL; weights (D,) f32)
+ *   pair i < rot / 2, t = positions[row] * freqs[i]:  y_lo = amplitude (n_lo cos t - n_hi sin t),
+ *   y_hi = amplitude (n_hi cos t + n_lo sin t); pairs (i, i + rot/2), or (2i, 2i+1) when interleaved; values beyond rot
+ *   are only normed.  positions (M,) int32, freqs (rot/2,) f64 radians per position (rot == 0: NULL allowed).
+ *   D and rot multiples of 16, D <= 256.
+ * The backward takes the gradients of both outputs and the forward's inputs; dw_partials (melgpt_qk_norm_rotary_bwd_blocks(M),
+ * 2, D) f32 receives partial sums of the weights' gradients (queries, keys) to be added up in row order by
+ * melgpt_reduce_rows; NULL without weights. */
+int melgpt_qk_norm_rotary_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                              long long k_head, const int* positions, const double* freqs, int rot, int interleaved,
+                              float amplitude, const float* q_weight, const float* k_weight, float eps, void* q_out,
+                              void* k_out, long long M, int Hq, int Hk, int D, int dtype, void* stream);
+int melgpt_qk_norm_rotary_bwd_blocks(long long M);
+int melgpt_qk_norm_rotary_bwd(const void* dq_out, long long dq_row, long long dq_head, const void* dk_out, long long dk_row,
+                              long long dk_head, const void* q, long long q_row, long long q_head, const void* k,
+                              long long k_row, long long k_head, const int* positions, const double* freqs, int rot,
+                              int interleaved, float amplitude, const float* q_weight, const float* k_weight, float eps,
+                              void* dq, void* dk, float* dw_partials, long long M, int Hq, int Hk, int D, int dtype,
+                              void* stream);
+
+/* Keys and values of new tokens into a paged cache, the keys normed and rotated on the way (as above), and the queries
+ * normed and rotated into q_out (q == NULL: none).  k_pages, v_pages (n_pages, Hk, page_size, D), page_size a power of two.
+ * Row r belongs to sequence sequences[r] and is stored at positions[r]: page page_table[seq * table_ld + pos / page_size],
+ * slot pos % page_size.  A row of negative position or sequence is padding: nothing is stored and its q_out row is left as
+ * it was (zero_pad: zeroed).  A row whose sequence, table column or page lies outside S, width or n_pages is not stored
+ * (the kernel checks every index); two rows of one slot leave one of them. */
+int melgpt_kv_append(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
+                     const void* v, long long v_row, long long v_head, const int* sequences, const int* positions,
+                     const int* page_table, long long table_ld, int S, int width, const double* freqs, int rot,
+                     int interleaved, float amplitude, const float* q_weight, const float* k_weight, float eps, void* q_out,
+                     int zero_pad, void* k_pages, void* v_pages, long long n_pages, int page_size, long long M, int Hq,
+                     int Hk, int D, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

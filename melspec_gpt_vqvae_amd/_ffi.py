@@ -129,6 +129,12 @@ _PROTOS = {
     "melgpt_softmax_bwd_rows": [_p, _l, _p, _l, _i, _l, _f, _p, _l, _i, _p],
     "melgpt_im2col_c1": [_p, _p, _i, _i, _i, _i, _p],
     "melgpt_groupnorm_swish_bwd_workspace": [_i, _i, _i],
+    "melgpt_qk_norm_rotary_fwd": [_p, _l, _l, _p, _l, _l, _p, _p, _i, _i, _f, _p, _p, _f, _p, _p, _l, _i, _i, _i, _i, _p],
+    "melgpt_qk_norm_rotary_bwd_blocks": [_l],
+    "melgpt_qk_norm_rotary_bwd": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _i, _i, _f, _p, _p, _f, _p, _p, _p, _l,
+                                  _i, _i, _i, _i, _p],
+    "melgpt_kv_append": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _p, _l, _i, _i, _p, _i, _i, _f, _p, _p, _f, _p, _i, _p, _p,
+                         _l, _i, _l, _i, _i, _i, _i, _p],
     "melgpt_groupnorm_swish_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p],
 }
 _RESTYPE = {"melgpt_strerror": C.c_char_p, "melgpt_vq_image_bytes": C.c_int64, "melgpt_linear_lds_workspace": C.c_int64,

@@ -964,3 +964,153 @@ def conv1d_out1(xp, w, bias, L, K, tanh=True):
     y = torch.empty(B, L, dtype=torch.float32, device=xp.device)
     call("melgpt_conv1d_out1", ptr(xp), ptr(w), ptr(bias), ptr(y), B, L, C, K, int(tanh), dtype_code(xp.dtype), stream())
     return y
+
+
+# --------------------------------------------------------------------------------- packed and cached sequences
+class _NoGuard:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _on(device):
+    """context in which the tensors' own device is the current one (its current stream is the one launched on)"""
+    if device.type != "cuda":
+        raise _ffi.MelgptError("melgpt kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _heads(x, what):
+    """(rows, heads, D) tensor -> the same or a copy with unit inner stride and 16-byte aligned rows and heads"""
+    assert x.dim() == 3, f"{what}: expected (rows, heads, head size), got {tuple(x.shape)}"
+    vec = 16 // x.element_size()
+    st = x.stride()
+    if st[2] != 1 or st[0] % vec or st[1] % vec or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _same_device(device, **tensors):
+    for name, t_ in tensors.items():
+        assert t_ is None or t_.device == device, f"{name} is on {t_.device}, expected {device}"
+
+
+def _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, device):
+    assert D % 16 == 0 and 16 <= D <= 256, f"head size {D}: a multiple of 16 up to 256"
+    rot = 2 * freqs.numel() if freqs is not None else 0
+    assert rot % 16 == 0 and rot <= D, f"{rot} rotated values of {D}: a multiple of 16 within the head"
+    assert positions.dtype == torch.int32 and positions.shape == (M,) and positions.is_contiguous()
+    assert freqs is None or (freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous())
+    assert (q_weight is None) == (k_weight is None), "the norm takes both weights or none"
+    for w in (q_weight, k_weight):
+        assert w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous())
+    _same_device(device, positions=positions, freqs=freqs, q_weight=q_weight, k_weight=k_weight)
+    return rot
+
+
+def qk_norm_rotary_fwd(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
+    """RMS norm of every query and key head (skipped without weights) and the rotation of its first 2 * freqs.numel() values
+    by positions * freqs (freqs None: no rotation), one launch.  q (M, Hq, D), k (M, Hk, D), any row and head strides;
+    positions (M,) int32; freqs f64 radians per position; weights (D,) f32 -> (q', k') contiguous."""
+    M, Hq, D = q.shape
+    Hk = k.shape[1]
+    assert k.shape == (M, Hk, D) and k.dtype == q.dtype and Hq > 0 and Hk > 0, (q.shape, k.shape, q.dtype, k.dtype)
+    dt = dtype_code(q.dtype)
+    with _on(q.device):
+        _same_device(q.device, k=k)
+        rot = _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, q.device)
+        q, k = _heads(q, "q"), _heads(k, "k")
+        qo = torch.empty(M, Hq, D, dtype=q.dtype, device=q.device)
+        ko = torch.empty(M, Hk, D, dtype=q.dtype, device=q.device)
+        call("melgpt_qk_norm_rotary_fwd", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(positions),
+             ptr(freqs), rot, int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(qo), ptr(ko), M,
+             Hq, Hk, D, dt, stream())
+    return qo, ko
+
+
+def qk_norm_rotary_bwd(dq_out, dk_out, q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                       amplitude=1.0):
+    """gradients of qk_norm_rotary_fwd: dq_out, dk_out like its outputs (any row and head strides), the other arguments its
+    inputs -> (dq, dk, d q_weight, d k_weight), the last two f32 (D,) or None without weights."""
+    M, Hq, D = q.shape
+    Hk = k.shape[1]
+    assert dq_out.shape == q.shape and dk_out.shape == k.shape == (M, Hk, D) and dq_out.dtype == dk_out.dtype == q.dtype == k.dtype
+    dt = dtype_code(q.dtype)
+    with _on(q.device):
+        _same_device(q.device, k=k, dq_out=dq_out, dk_out=dk_out)
+        rot = _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, q.device)
+        q, k, dq_out, dk_out = _heads(q, "q"), _heads(k, "k"), _heads(dq_out, "dq_out"), _heads(dk_out, "dk_out")
+        dq = torch.empty(M, Hq, D, dtype=q.dtype, device=q.device)
+        dk = torch.empty(M, Hk, D, dtype=q.dtype, device=q.device)
+        part = dw = None
+        if q_weight is not None:
+            dw = torch.empty(2, D, dtype=torch.float32, device=q.device)
+            if M == 0:
+                zero_(dw)
+            n = _ffi.lib().melgpt_qk_norm_rotary_bwd_blocks(M)
+            part = torch.empty(n, 2, D, dtype=torch.float32, device=q.device)
+        call("melgpt_qk_norm_rotary_bwd", ptr(dq_out), dq_out.stride(0), dq_out.stride(1), ptr(dk_out), dk_out.stride(0),
+             dk_out.stride(1), ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(positions), ptr(freqs), rot,
+             int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(dq), ptr(dk), ptr(part), M, Hq, Hk,
+             D, dt, stream())
+        if dw is not None and M > 0:
+            call("melgpt_reduce_rows", ptr(part), n, 2 * D, 2 * D, ptr(dw), 0, 1.0, stream())
+    return dq, dk, (dw[0] if dw is not None else None), (dw[1] if dw is not None else None)
+
+
+def _pages_of(k_pages, v_pages, page_table, dtype, device):
+    P, Hk, page, D = k_pages.shape
+    assert v_pages.shape == k_pages.shape and k_pages.is_contiguous() and v_pages.is_contiguous()
+    assert k_pages.dtype == v_pages.dtype == dtype, (k_pages.dtype, v_pages.dtype, dtype)
+    assert page > 0 and page & (page - 1) == 0, f"page size {page}: a power of two"
+    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and (page_table.stride(1) == 1 or page_table.shape[1] == 1)
+    _same_device(device, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    return P, Hk, page, D
+
+
+def kv_append(k, v, k_pages, v_pages, page_table, sequences, positions, *, q=None, freqs=None, q_weight=None, k_weight=None,
+              eps=1e-6, interleaved=False, amplitude=1.0, q_out=None):
+    """Stores the keys and values of M new tokens in a paged cache, the keys normed and rotated on the way exactly as
+    qk_norm_rotary_fwd does, and returns the queries treated likewise (None without q): a layer's whole step in front of its
+    attention in one launch.  k, v (M, Hk, D), q (M, Hq, D) with any row and head strides; k_pages, v_pages (pages, Hk, page
+    size, D); page_table (S, width) int32; row r goes to sequence sequences[r], position positions[r] (both (M,) int32).
+    A row of negative sequence or position is padding: nothing is stored, its row of a given q_out stays as it was (of a
+    returned new one: zero).  A row that points outside the table or the pages is not stored.  Slots must be distinct."""
+    M, Hk, D = k.shape
+    assert v.shape == k.shape and v.dtype == k.dtype
+    dt = dtype_code(k.dtype)
+    with _on(k.device):
+        P, Hkp, page, Dp = _pages_of(k_pages, v_pages, page_table, k.dtype, k.device)
+        assert (Hkp, Dp) == (Hk, D), (k_pages.shape, k.shape)
+        _same_device(k.device, v=v, q=q, q_out=q_out, sequences=sequences)
+        assert sequences.dtype == torch.int32 and sequences.shape == (M,) and sequences.is_contiguous()
+        if q is None:
+            assert q_weight is None and q_out is None
+            rot = _norm_rotary_args(M, D, positions, freqs, k_weight, k_weight, k.device)
+            Hq = 0
+        else:
+            rot = _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, k.device)
+            Hq = q.shape[1]
+            assert q.shape == (M, Hq, D) and q.dtype == k.dtype and Hq > 0
+            q = _heads(q, "q")
+        zero_pad = q is not None and q_out is None
+        if zero_pad:
+            q_out = torch.empty(M, Hq, D, dtype=k.dtype, device=k.device)
+        elif q is not None:
+            assert q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous()
+            assert q_out.data_ptr() != q.data_ptr(), "q_out is a buffer of its own"
+        k, v = _heads(k, "k"), _heads(v, "v")
+        if M == 0 or page_table.numel() == 0 or P == 0:
+            assert M == 0, "a cache without pages takes no rows"
+            return q_out
+        qs = q.stride() if q is not None else (0, 0)
+        call("melgpt_kv_append", ptr(q), qs[0], qs[1], ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1),
+             ptr(sequences), ptr(positions), ptr(page_table), page_table.stride(0), page_table.shape[0], page_table.shape[1],
+             ptr(freqs), rot, int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(q_out),
+             int(zero_pad), ptr(k_pages), ptr(v_pages), P, page, M, Hq, Hk, D, dt, stream())
+    return q_out
