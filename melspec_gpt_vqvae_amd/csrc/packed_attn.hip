@@ -1,0 +1,544 @@
+// Causal attention with grouped heads over packed sequences of different lengths, forward and backward.
+//
+//   sequence s: queries rows cu_q[s] .. cu_q[s+1], keys rows cu_k[s] .. cu_k[s+1] (nq, nk of them); query i sees the keys
+//   j <= i + nk - nq (the last query sees every key; with nq > nk the first nq - nk queries see none: output 0, lse -inf);
+//   query head h reads key head h / G.
+//   forward   s_ij = scale q_i . k_j,  lse_i = log sum_j e^s_ij,  o_i = sum_j e^(s_ij - lse_i) v_j
+//   backward  p_ij = e^(s_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//             dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i,h ds_ij q_i,  dv_j = sum_i,h p_ij do_i  (h over the G heads)
+//
+// One pass over the keys with a running maximum and sum; scores, probabilities and their gradients live in registers only.
+// The backward is two kernels - queries (dq, delta), then keys (dk, dv) - that each own their rows: no atomics, the same
+// bits every time, at the price of forming the scores and do . v twice (7 products instead of 5).
+//
+// Row tiles of a sequence: nobody knows the lengths on the host, so sequence s is allotted tiles floor(cu[s] / B) + s up to
+// floor(cu[s+1] / B) + s + 1 - never fewer than it needs, one too many at most - and a workgroup finds its sequence by a
+// 64-way search over the offsets.  The rows in front of the first and behind the last sequence are two sequences without keys.
+#include "mma.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+struct PackedParams {
+  const void *q, *k, *v;
+  long long q_row, q_head, k_row, k_head, v_row, v_head;
+  void* o;                       // forward out / backward in
+  long long o_row, o_head;
+  const void* dout;
+  long long do_row, do_head;
+  void *dq, *dk, *dv;
+  long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  float *lse, *delta;            // (Hq, Mq)
+  const int *cu_q, *cu_k;        // (S + 1)
+  int S, Hq, Hk, G, write_gaps;  // write_gaps: zero the rows no sequence owns
+  long long Mq, Mk;
+  float scale;
+};
+
+// ---------------------------------------------------------------------------------------------- which rows are mine
+// Boundaries of the S + 2 row ranges over M rows: [0, cu[0]), the sequences, [cu[S], M).  Out-of-range offsets are clamped.
+__device__ __forceinline__ int bound_at(const int* cu, int S, long long M, int i) {
+  if (i <= 0) return 0;
+  if (i > S + 1) return (int)M;
+  const int b = cu[i - 1];
+  return b < 0 ? 0 : b > (int)M ? (int)M : b;
+}
+struct Rows {
+  int seq;       // -1 or S: a gap, no keys
+  int lo, n;     // its first row and their number
+  int tile, tiles;
+  bool any;
+};
+// tile number t (of rows of `B`) -> its range and the tile within it, the last tile of a range first (the causal tiles
+// with the most keys start first)
+template <int B>
+__device__ __forceinline__ Rows find_rows(const int* cu, int S, long long M, int t, int lane) {
+  // the largest range i of 0 .. S + 1 with bound(i) / B + i <= t, 64 candidates at a time (the lanes of every wave)
+  int lo = 0, n = S + 2;
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int i = lo + lane * step;
+    const bool yes = lane * step < n && bound_at(cu, S, M, i) / B + i <= t;
+    const unsigned long long m = __ballot(yes);
+    const int c = m ? 63 - __builtin_clzll(m) : 0;   // (offsets that do not rise leave holes; any candidate stays in range)
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  Rows r;
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int a = bound_at(cu, S, M, lo), b = max(bound_at(cu, S, M, lo + 1), a);
+  r.seq = lo - 1;
+  r.lo = a;
+  r.n = b - a;
+  r.tiles = (r.n + B - 1) / B;
+  const int at = t - (a / B + lo);
+  r.any = at >= 0 && at < r.tiles;
+  r.tile = r.tiles - 1 - at;
+  return r;
+}
+// rows of the other side of sequence seq
+__device__ __forceinline__ void other_rows(const int* cu, int S, long long M, int seq, int& lo, int& n) {
+  if (seq < 0 || seq >= S) {
+    lo = 0;
+    n = 0;
+    return;
+  }
+  lo = bound_at(cu, S, M, seq + 1);
+  n = max(bound_at(cu, S, M, seq + 2) - lo, 0);
+}
+long long tiles_for(long long M, int S, int B) { return M / B + S + 2; }
+
+// workgroup -> (tile, query head): consecutive workgroups go to consecutive XCDs, so with the key head fastest the
+// workgroups that read one key head's rows share an XCD's L2 when the key heads are a multiple of 8
+__device__ __forceinline__ void head_of(int w, const PackedParams& p, int& h) {
+  const int kv = w % p.Hk, g = w / p.Hk;
+  h = kv * p.G + g;
+}
+
+// ------------------------------------------------------------------------------------------------- tiles in LDS
+// R rows of D values, 16-byte chunks xor-swizzled by the row so that neither row reads (16 rows, one chunk) nor transposed
+// reads pile up on banks.
+template <typename T, int D>
+struct Tile {
+  static constexpr int ES = Tr<T>::ES, RB = D * ES, CP = RB / 16, VEC = 16 / ES;
+  static constexpr int NKS = CP / 4;           // fragments along D
+  static constexpr int DT = D / 16;            // 16-column tiles
+  static constexpr int STEPS = ES == 2 ? 1 : 2;   // contraction steps along 32 rows
+  static __device__ __forceinline__ int off(int row, int c) {
+    if constexpr (RB == 128) return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
+    else return row * RB + ((c ^ (row & 15)) << 4);
+  }
+  // fragment of 16 rows (16 tile16 + (lane & 15)), contraction along D
+  static __device__ __forceinline__ u32x4 rows(const char* t, int tile16, int ks, int lane) {
+    return *(const u32x4*)(t + off(16 * tile16 + (lane & 15), 4 * ks + (lane >> 4)));
+  }
+  // fragment of 16 columns (16 dt + (lane & 15)), contraction along rows, step st: 32 rows for 16-bit types (slot j < 4: row
+  // 32 st + 4 g + j, else 32 st + 16 + 4 g + j - 4), 16 for f32 (slot e: row 16 st + 4 g + e) - the order in which the
+  // accumulators of the score products hold them, so those are the other operand as they stand
+  static __device__ __forceinline__ u32x4 cols(const char* t, int st, int dt, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    if constexpr (ES == 2) {
+      const int r0 = 32 * st + 4 * g + (i >> 2), c = 2 * dt + ((i & 3) >> 1);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off(r0, c) + 8 * (i & 1)));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off(r0 + 16, c) + 8 * (i & 1)));
+      const s16x8 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(u32x4, f);
+    } else {
+      const int col = 16 * dt + i;
+      u32x4 f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = *(const unsigned*)(t + off(16 * st + 4 * g + e, col >> 2) + (col & 3) * 4);
+      return f;
+    }
+  }
+};
+
+// accumulators of 32 rows as operands that contract over them: one for 16-bit types, two for f32
+template <typename T>
+__device__ __forceinline__ u32x4 operand(const f32x4& lo, const f32x4& hi, int step) {
+  if constexpr (Tr<T>::ES == 2)
+    return u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
+  else
+    return __builtin_bit_cast(u32x4, step ? hi : lo);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4 v) {
+  if constexpr (Tr<T>::ES == 2) *(u32x2*)p = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  else *(f32x4*)p = v;
+}
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// 32 rows of two tensors on their way into LDS: the loads of the next pair are in flight under the current pair's products.
+// Rows at and beyond n are zero (their products are masked, but 0 * NaN is not 0).
+template <typename T, int D>
+struct Stage {
+  using L = Tile<T, D>;
+  static constexpr int PER = 32 * L::CP / 256;   // chunks per thread
+  u32x4 a[PER], b[PER];
+  __device__ __forceinline__ void load(const T* pa, long long ra, const T* pb, long long rb, int row0, int n, int t) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int q = t + 256 * i, row = min(row0 + q / L::CP, n - 1), c = q % L::CP;
+      a[i] = *(const u32x4*)(pa + row * ra + c * L::VEC);
+      b[i] = *(const u32x4*)(pb + row * rb + c * L::VEC);
+    }
+  }
+  __device__ __forceinline__ void store(char* ta, char* tb, int row0, int n, int t) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int q = t + 256 * i, row = q / L::CP, c = q % L::CP;
+      const bool in = row0 + row < n;
+      const u32x4 z = {0u, 0u, 0u, 0u};
+      *(u32x4*)(ta + L::off(row, c)) = in ? a[i] : z;
+      *(u32x4*)(tb + L::off(row, c)) = in ? b[i] : z;
+    }
+  }
+};
+
+// -------------------------------------------------------------------------------------------------------- forward
+// 256 threads, 64 queries of one head: a wave owns 16 queries and walks the keys 32 at a time.  S^T = K Q^T puts the query
+// on the lane: its maximum and sum are in registers and two exchanges away, and the probabilities are the operand of
+// O^T = V^T P^T as they stand.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
+  using L = Tile<T, D>;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
+  int h;
+  head_of(blockIdx.x, p, h);
+  const Rows R = find_rows<64>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  if (!R.any) return;
+  int k_lo, nk;
+  other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
+  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
+  const int q_in = 64 * R.tile + 16 * wave + (lane & 15);          // this lane's query within its sequence
+  const bool mine = q_in < R.n;
+  const long long row = R.lo + min(q_in, R.n - 1);
+  const int sees = min(max(q_in + nk - R.n + 1, 0), nk);           // keys 0 .. sees - 1
+  const int last = min(64 * R.tile + 63, R.n - 1);
+  const int most = min(max(last + nk - R.n + 1, 0), nk);           // of any query of the workgroup
+  const T* qp = (const T*)p.q + row * p.q_row + h * p.q_head;
+  u32x4 qf[L::NKS];
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * L::VEC);
+  const T* kp = (const T*)p.k + (long long)k_lo * p.k_row + (h / p.G) * p.k_head;
+  const T* vp = (const T*)p.v + (long long)k_lo * p.v_row + (h / p.G) * p.v_head;
+  const float c2 = p.scale * LOG2E;
+  f32x4 o[L::DT];
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), l = 0.f;
+  if (most > 0) {
+    Stage<T, D> st;
+    st.load(kp, p.k_row, vp, p.v_row, 0, nk, t);
+    st.store(lds[0][0], lds[0][1], 0, nk, t);
+    __syncthreads();
+    for (int k0 = 0, buf = 0; k0 < most; k0 += 32, buf ^= 1) {
+      const bool more = k0 + 32 < most;
+      if (more) st.load(kp, p.k_row, vp, p.v_row, k0 + 32, nk, t);
+      const char *kt = lds[buf][0], *vt = lds[buf][1];
+      f32x4 s[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < L::NKS; ++ks) mma<T>(s[i], L::rows(kt, i, ks, lane), qf[ks]);
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[i][r] = k0 + 16 * i + 4 * g + r < sees ? s[i][r] * c2 : -__builtin_inff();
+          top = fmaxf(top, s[i][r]);
+        }
+      top = fmaxf(across_groups_max(top), m);
+      const float base = top == -__builtin_inff() ? 0.f : top;     // (no key seen yet: every term stays e^-inf = 0)
+      const float keep = __builtin_amdgcn_exp2f(m - base);
+      m = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - base);
+          sum += s[i][r];
+        }
+      l = l * keep + sum;
+#pragma unroll
+      for (int d = 0; d < L::DT; ++d) o[d] *= keep;
+#pragma unroll
+      for (int e = 0; e < L::STEPS; ++e) {
+        const u32x4 pf = operand<T>(s[0], s[1], e);
+#pragma unroll
+        for (int d = 0; d < L::DT; ++d) mma<T>(o[d], L::cols(vt, e, d, lane), pf);
+      }
+      if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 32, nk, t);
+      __syncthreads();
+    }
+    l = across_groups_sum(l);
+  }
+  if (!mine) return;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;        // (NaN stays NaN)
+  T* op = (T*)p.o + row * p.o_row + h * p.o_head;
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) store4<T>(op + 16 * d + 4 * g, o[d] * inv);
+  if (g == 0) p.lse[h * p.Mq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// -------------------------------------------------------------------------------------------------------- backward
+// dq and delta: the forward's walk with a second score product, do . v, on the same tiles
+template <typename T, int D>
+__global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
+  using L = Tile<T, D>;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
+  int h;
+  head_of(blockIdx.x, p, h);
+  const Rows R = find_rows<64>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  if (!R.any) return;
+  int k_lo, nk;
+  other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
+  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
+  const int q_in = 64 * R.tile + 16 * wave + (lane & 15);
+  const bool mine = q_in < R.n;
+  const long long row = R.lo + min(q_in, R.n - 1);
+  const int sees = min(max(q_in + nk - R.n + 1, 0), nk);
+  const int last = min(64 * R.tile + 63, R.n - 1);
+  const int most = min(max(last + nk - R.n + 1, 0), nk);
+  const T* qp = (const T*)p.q + row * p.q_row + h * p.q_head;
+  const T* gp = (const T*)p.dout + row * p.do_row + h * p.do_head;
+  const T* op = (const T*)p.o + row * p.o_row + h * p.o_head;
+  u32x4 qf[L::NKS], gf[L::NKS];
+  float dl = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) {
+    qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * L::VEC);
+    gf[ks] = *(const u32x4*)(gp + (4 * ks + g) * L::VEC);
+    const u32x4 of = *(const u32x4*)(op + (4 * ks + g) * L::VEC);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (L::ES == 2) {
+        dl = fmaf(half_lo(gf[ks][e]), half_lo(of[e]), dl);
+        dl = fmaf(half_hi(gf[ks][e]), half_hi(of[e]), dl);
+      } else {
+        dl = fmaf(__uint_as_float(gf[ks][e]), __uint_as_float(of[e]), dl);
+      }
+    }
+  }
+  dl = across_groups_sum(dl);
+  if (mine && g == 0) p.delta[h * p.Mq + row] = dl;
+  const float lse2 = p.lse[h * p.Mq + row] * LOG2E;
+  const T* kp = (const T*)p.k + (long long)k_lo * p.k_row + (h / p.G) * p.k_head;
+  const T* vp = (const T*)p.v + (long long)k_lo * p.v_row + (h / p.G) * p.v_head;
+  const float c2 = p.scale * LOG2E;
+  f32x4 dq[L::DT];
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) dq[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (most > 0) {
+    Stage<T, D> st;
+    st.load(kp, p.k_row, vp, p.v_row, 0, nk, t);
+    st.store(lds[0][0], lds[0][1], 0, nk, t);
+    __syncthreads();
+    for (int k0 = 0, buf = 0; k0 < most; k0 += 32, buf ^= 1) {
+      const bool more = k0 + 32 < most;
+      if (more) st.load(kp, p.k_row, vp, p.v_row, k0 + 32, nk, t);
+      const char *kt = lds[buf][0], *vt = lds[buf][1];
+      f32x4 s[2], dp[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i] = dp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < L::NKS; ++ks) {
+          mma<T>(s[i], L::rows(kt, i, ks, lane), qf[ks]);
+          mma<T>(dp[i], L::rows(vt, i, ks, lane), gf[ks]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[i][r] = k0 + 16 * i + 4 * g + r < sees ? __builtin_amdgcn_exp2f(s[i][r] * c2 - lse2) * (dp[i][r] - dl) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < L::STEPS; ++e) {
+        const u32x4 sf = operand<T>(s[0], s[1], e);
+#pragma unroll
+        for (int d = 0; d < L::DT; ++d) mma<T>(dq[d], L::cols(kt, e, d, lane), sf);
+      }
+      if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 32, nk, t);
+      __syncthreads();
+    }
+  }
+  if (!mine) return;
+  T* out = (T*)p.dq + row * p.dq_row + h * p.dq_head;
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) store4<T>(out + 16 * d + 4 * g, dq[d] * p.scale);
+}
+
+// dk and dv: 64 keys of one key head, a wave owns 16 keys (in registers) and walks the queries of its G heads that see
+// them, 32 at a time.  S = Q K^T puts the key on the lane; P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
+  using L = Tile<T, D>;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
+  __shared__ float stat[2][2][32];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
+  const int hk = blockIdx.x;
+  const Rows R = find_rows<64>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
+  if (!R.any) return;
+  int q_lo, nq;
+  other_rows(p.cu_q, p.S, p.Mq, R.seq, q_lo, nq);
+  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
+  const int nk = R.n;
+  const int k_in = 64 * R.tile + 16 * wave + (lane & 15);
+  const bool mine = k_in < nk;
+  const long long row = R.lo + min(k_in, nk - 1);
+  // query i sees key j <= i + nk - nq: the queries from j - (nk - nq) on
+  const int from = max(k_in - (nk - nq), 0);
+  const int first = max(64 * R.tile - (nk - nq), 0) & ~31;
+  const T* kp = (const T*)p.k + row * p.k_row + hk * p.k_head;
+  const T* vp = (const T*)p.v + row * p.v_row + hk * p.v_head;
+  u32x4 kf[L::NKS], vf[L::NKS];
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) {
+    kf[ks] = *(const u32x4*)(kp + (4 * ks + g) * L::VEC);
+    vf[ks] = *(const u32x4*)(vp + (4 * ks + g) * L::VEC);
+  }
+  const float c2 = p.scale * LOG2E;
+  f32x4 dk[L::DT], dv[L::DT];
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int blocks = first < nq ? (nq - first + 31) / 32 : 0, total = blocks * p.G;
+  if (total > 0) {
+    Stage<T, D> st;
+    float sv = 0.f;
+    auto load = [&](int n) {
+      const int h = hk * p.G + n / blocks, q0 = first + 32 * (n % blocks);
+      st.load((const T*)p.q + (long long)q_lo * p.q_row + h * p.q_head, p.q_row,
+              (const T*)p.dout + (long long)q_lo * p.do_row + h * p.do_head, p.do_row, q0, nq, t);
+      if (t < 64) {
+        const long long r = h * p.Mq + q_lo + min(q0 + (t & 31), nq - 1);
+        sv = t < 32 ? p.lse[r] * LOG2E : p.delta[r];
+      }
+    };
+    auto store = [&](int n, int buf) {
+      st.store(lds[buf][0], lds[buf][1], first + 32 * (n % blocks), nq, t);
+      if (t < 64) stat[buf][t >> 5][t & 31] = sv;
+    };
+    load(0);
+    store(0, 0);
+    __syncthreads();
+    for (int n = 0, buf = 0; n < total; ++n, buf ^= 1) {
+      if (n + 1 < total) load(n + 1);
+      const int q0 = first + 32 * (n % blocks);
+      const char *qt = lds[buf][0], *gt = lds[buf][1];
+      f32x4 s[2], dp[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i] = dp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < L::NKS; ++ks) {
+          mma<T>(s[i], L::rows(qt, i, ks, lane), kf[ks]);
+          mma<T>(dp[i], L::rows(gt, i, ks, lane), vf[ks]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = 16 * i + 4 * g + r, q = q0 + at;
+          const bool in = q >= from && q < nq;
+          const float pr = in ? __builtin_amdgcn_exp2f(s[i][r] * c2 - stat[buf][0][at]) : 0.f;
+          s[i][r] = pr;
+          dp[i][r] = in ? pr * (dp[i][r] - stat[buf][1][at]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < L::STEPS; ++e) {
+        const u32x4 pf = operand<T>(s[0], s[1], e), sf = operand<T>(dp[0], dp[1], e);
+#pragma unroll
+        for (int d = 0; d < L::DT; ++d) {
+          mma<T>(dv[d], L::cols(gt, e, d, lane), pf);
+          mma<T>(dk[d], L::cols(qt, e, d, lane), sf);
+        }
+      }
+      if (n + 1 < total) store(n + 1, buf ^ 1);
+      __syncthreads();
+    }
+  }
+  if (!mine) return;
+  T* ok = (T*)p.dk + row * p.dk_row + hk * p.dk_head;
+  T* ov = (T*)p.dv + row * p.dv_row + hk * p.dv_head;
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) {
+    store4<T>(ok + 16 * d + 4 * g, dk[d] * p.scale);
+    store4<T>(ov + 16 * d + 4 * g, dv[d]);
+  }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check(const PackedParams& p, int D, int dtype) {
+  if (p.S < 0 || p.Hq <= 0 || p.Hk <= 0 || p.Mq < 0 || p.Mk < 0 || !p.cu_q || !p.cu_k) return MELGPT_ERR_BAD_ARG;
+  if (dtype != MELGPT_F32 && dtype != MELGPT_BF16) return MELGPT_ERR_UNSUPPORTED;
+  if ((D != 64 && D != 128) || p.Hq % p.Hk) return MELGPT_ERR_UNSUPPORTED;
+  // tile numbers and row numbers are 32-bit, a grid's second dimension ends at 65535
+  if (p.Mq > (1 << 30) || p.Mk > (1 << 30) || p.S > (1 << 24)) return MELGPT_ERR_UNSUPPORTED;
+  const int vec = dtype == MELGPT_F32 ? 4 : 8;
+  if (p.Mq > 0 && (!p.q || !p.o || !p.lse)) return MELGPT_ERR_BAD_ARG;
+  if (p.Mk > 0 && (!p.k || !p.v)) return MELGPT_ERR_BAD_ARG;
+  if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.o)) return MELGPT_ERR_ALIGN;
+  if (p.q_row % vec || p.q_head % vec || p.k_row % vec || p.k_head % vec || p.v_row % vec || p.v_head % vec || p.o_row % vec ||
+      p.o_head % vec)
+    return MELGPT_ERR_ALIGN;
+  return MELGPT_OK;
+}
+
+template <typename T, int D>
+int launch_fwd(const PackedParams& p, hipStream_t s) {
+  const long long tiles = tiles_for(p.Mq, p.S, 64);
+  if (tiles > 65535) return MELGPT_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((packed_fwd_kernel<T, D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
+  return melgpt_launch_status();
+}
+
+template <typename T, int D>
+int launch_bwd(const PackedParams& p, hipStream_t s) {
+  const long long tq = tiles_for(p.Mq, p.S, 64), tk = tiles_for(p.Mk, p.S, 64);
+  if (tq > 65535 || tk > 65535) return MELGPT_ERR_UNSUPPORTED;
+  if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_kernel<T, D>), dim3(p.Hq, (unsigned)tq), dim3(256), 0, s, p);
+  if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_kernel<T, D>), dim3(p.Hk, (unsigned)tk), dim3(256), 0, s, p);
+  return melgpt_launch_status();
+}
+
+}  // namespace
+
+extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                                      long long k_head, const void* v, long long v_row, long long v_head, const int* cu_q,
+                                      const int* cu_k, int S, void* out, long long o_row, long long o_head, float* lse,
+                                      int write_gaps, long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype,
+                                      void* stream) {
+  PackedParams p = {};
+  p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head;
+  p.v = v; p.v_row = v_row; p.v_head = v_head; p.o = out; p.o_row = o_row; p.o_head = o_head; p.lse = lse;
+  p.cu_q = cu_q; p.cu_k = cu_k; p.S = S; p.Hq = Hq; p.Hk = Hk; p.write_gaps = write_gaps; p.Mq = Mq; p.Mk = Mk; p.scale = scale;
+  const int e = check(p, D, dtype);
+  if (e) return e;
+  if (Mq == 0) return MELGPT_OK;
+  p.G = Hq / Hk;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MELGPT_F32) return D == 64 ? launch_fwd<float, 64>(p, s) : launch_fwd<float, 128>(p, s);
+  return D == 64 ? launch_fwd<bf16_t, 64>(p, s) : launch_fwd<bf16_t, 128>(p, s);
+}
+
+extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
+                                      long long k_head, const void* v, long long v_row, long long v_head, const int* cu_q,
+                                      const int* cu_k, int S, const void* out, long long o_row, long long o_head,
+                                      const void* dout, long long do_row, long long do_head, const float* lse, float* delta,
+                                      void* dq, long long dq_row, long long dq_head, void* dk, long long dk_row,
+                                      long long dk_head, void* dv, long long dv_row, long long dv_head, int write_gaps,
+                                      long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype, void* stream) {
+  PackedParams p = {};
+  p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head;
+  p.v = v; p.v_row = v_row; p.v_head = v_head; p.o = const_cast<void*>(out); p.o_row = o_row; p.o_head = o_head;
+  p.lse = const_cast<float*>(lse); p.delta = delta; p.dout = dout; p.do_row = do_row; p.do_head = do_head;
+  p.dq = dq; p.dq_row = dq_row; p.dq_head = dq_head; p.dk = dk; p.dk_row = dk_row; p.dk_head = dk_head;
+  p.dv = dv; p.dv_row = dv_row; p.dv_head = dv_head;
+  p.cu_q = cu_q; p.cu_k = cu_k; p.S = S; p.Hq = Hq; p.Hk = Hk; p.write_gaps = write_gaps; p.Mq = Mq; p.Mk = Mk; p.scale = scale;
+  const int e = check(p, D, dtype);
+  if (e) return e;
+  if (Mq > 0 && (!dout || !delta || !dq)) return MELGPT_ERR_BAD_ARG;
+  if (Mk > 0 && (!dk || !dv)) return MELGPT_ERR_BAD_ARG;
+  const int vec = dtype == MELGPT_F32 ? 4 : 8;
+  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_row % vec || do_head % vec || dq_row % vec ||
+      dq_head % vec || dk_row % vec || dk_head % vec || dv_row % vec || dv_head % vec)
+    return MELGPT_ERR_ALIGN;
+  p.G = Hq / Hk;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MELGPT_F32) return D == 64 ? launch_bwd<float, 64>(p, s) : launch_bwd<float, 128>(p, s);
+  return D == 64 ? launch_bwd<bf16_t, 64>(p, s) : launch_bwd<bf16_t, 128>(p, s);
+}

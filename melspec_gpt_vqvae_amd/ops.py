@@ -1114,3 +1114,74 @@ def kv_append(k, v, k_pages, v_pages, page_table, sequences, positions, *, q=Non
              ptr(freqs), rot, int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(q_out),
              int(zero_pad), ptr(k_pages), ptr(v_pages), P, page, M, Hq, Hk, D, dt, stream())
     return q_out
+
+
+def _offsets(cu, what, device):
+    assert cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 1 and cu.is_contiguous(), f"{what}: (sequences + 1,) int32"
+    _same_device(device, **{what: cu})
+    return cu.numel() - 1
+
+
+def _packed_args(q, k, v, cu_q, cu_k):
+    Mq, Hq, D = q.shape
+    Mk, Hk, _ = k.shape
+    assert k.shape == v.shape == (Mk, Hk, D) and q.dtype == k.dtype == v.dtype, (q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype)
+    assert D in (64, 128), f"head size {D}: 64 or 128"
+    assert Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads over {Hk} key heads"
+    assert max(Mq, Mk) // 64 + cu_q.numel() + 1 <= 65535, "too many rows"
+    S = _offsets(cu_q, "cu_q", q.device)
+    if cu_k is None:
+        assert Mq == Mk, "queries and keys of different lengths need cu_k"
+        cu_k = cu_q
+    assert _offsets(cu_k, "cu_k", q.device) == S, "cu_q and cu_k: one offset per sequence and the end"
+    _same_device(q.device, k=k, v=v)
+    return Mq, Mk, Hq, Hk, D, S, cu_k
+
+
+def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None):
+    """Causal attention of packed sequences: q (Mq, Hq, D), k, v (Mk, Hk, D), any row and head strides, Hq a multiple of Hk;
+    sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
+    cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
+    -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  Rows behind the last sequence: left as they were in a given `out`, zero in a
+    new one.  scale: 1 / sqrt(D) unless given."""
+    dt = dtype_code(q.dtype)
+    with _on(q.device):
+        Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(q, k, v, cu_q, cu_k)
+        q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+        gaps = out is None
+        if gaps:
+            out = torch.empty(Mq, Hq, D, dtype=q.dtype, device=q.device)
+        else:
+            assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+            _same_device(q.device, out=out)
+        lse = torch.empty(Hq, Mq, dtype=torch.float32, device=q.device)
+        call("melgpt_packed_attn_fwd", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
+             v.stride(1), ptr(cu_q), ptr(cu_k), S, ptr(out), out.stride(0), out.stride(1), ptr(lse), int(gaps), Mq, Mk, Hq, Hk, D,
+             float(scale if scale is not None else D ** -0.5), dt, stream())
+    return out, lse
+
+
+def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, grads=None):
+    """gradients of packed_attn_fwd from its inputs, both its results and dout (any row and head strides) -> (dq, dk, dv),
+    contiguous and zero in rows that no sequence owns, unless `grads` gives the three tensors (any row and head strides,
+    such rows left as they were)."""
+    dt = dtype_code(q.dtype)
+    with _on(q.device):
+        Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(q, k, v, cu_q, cu_k)
+        assert out.shape == q.shape == dout.shape and out.dtype == dout.dtype == q.dtype and out.stride(2) == 1
+        assert lse.shape == (Hq, Mq) and lse.dtype == torch.float32 and lse.is_contiguous()
+        _same_device(q.device, out=out, dout=dout, lse=lse)
+        q, k, v, dout = _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(dout, "dout")
+        gaps = grads is None
+        if gaps:
+            grads = (torch.empty(Mq, Hq, D, dtype=q.dtype, device=q.device), torch.empty(Mk, Hk, D, dtype=q.dtype, device=q.device),
+                     torch.empty(Mk, Hk, D, dtype=q.dtype, device=q.device))
+        dq, dk, dv = grads
+        for g, x in ((dq, q), (dk, k), (dv, v)):
+            assert g.shape == x.shape and g.dtype == x.dtype and g.stride(2) == 1 and g.device == x.device
+        delta = torch.empty(Hq, Mq, dtype=torch.float32, device=q.device)
+        call("melgpt_packed_attn_bwd", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
+             v.stride(1), ptr(cu_q), ptr(cu_k), S, ptr(out), out.stride(0), out.stride(1), ptr(dout), dout.stride(0), dout.stride(1),
+             ptr(lse), ptr(delta), ptr(dq), dq.stride(0), dq.stride(1), ptr(dk), dk.stride(0), dk.stride(1), ptr(dv), dv.stride(0),
+             dv.stride(1), int(gaps), Mq, Mk, Hq, Hk, D, float(scale if scale is not None else D ** -0.5), dt, stream())
+    return dq, dk, dv

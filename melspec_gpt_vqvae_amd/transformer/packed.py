@@ -57,3 +57,23 @@ class _QkNormRotaryFn(torch.autograd.Function):
 def qk_norm_rotary(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
     """ops.qk_norm_rotary_fwd with gradients for q, k and both weights."""
     return _QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, freqs, float(eps), bool(interleaved), float(amplitude))
+
+
+class _PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, scale):
+        out, lse = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        return ops.packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k, scale=ctx.scale) + (None, None, None)
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, *, scale=None):
+    """ops.packed_attn_fwd's output with gradients for q, k and v (those of a key head summed over its query heads)."""
+    return _PackedAttentionFn.apply(q, k, v, cu_q, cu_k, scale)

@@ -73,3 +73,50 @@ def pair_size(x, freqs, interleaved, amplitude):
 # two products and a sum 3 u.  Together < 32 u of the pair's size.
 def rotary_bound(n, want, dtype, freqs, interleaved, amplitude):
     return half_step(dtype) * want.abs() + 32 * U * pair_size(n, freqs, interleaved, abs(amplitude))
+
+
+# ---------------------------------------------------------------------------------------------------------- attention
+def attention(q, k, v, scale, dout=None, sees=None):
+    """one head of one sequence in 64 bits: q (nq, D), k, v (nk, D) -> dict of o, lse and, with dout, dq, dk, dv, and for each
+    the size its f32 errors scale with (s_*)"""
+    nq, nk = q.shape[0], k.shape[0]
+    q, k, v = q.double(), k.double(), v.double()
+    if sees is None:
+        sees = torch.arange(nk)[None] <= torch.arange(nq)[:, None] + (nk - nq)
+    s = scale * q @ k.t()
+    s = s.masked_fill(~sees, -math.inf)
+    lse = torch.logsumexp(s, -1) if nk else torch.full((nq,), -math.inf, dtype=torch.float64)
+    some = lse > -math.inf
+    p = torch.where(some[:, None], torch.exp(s - torch.where(some, lse, 0.0)[:, None]), 0.0)
+    r = dict(o=p @ v, lse=lse, p=p, s_o=p @ v.abs(), s_score=(abs(scale) * q.abs() @ k.abs().t()).masked_fill(~sees, 0).amax(-1) if nk else torch.zeros(nq).double())
+    if dout is not None:
+        g = dout.double()
+        dp = g @ v.t()
+        delta = (g * r["o"]).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        r.update(dq=scale * ds @ k, dk=scale * ds.t() @ q, dv=p.t() @ g)
+        sds = p * (g.abs() @ v.abs().t() + (g.abs() * r["s_o"]).sum(-1, keepdim=True))
+        r.update(s_ds=sds, s_dq=abs(scale) * sds @ k.abs(), s_dk=abs(scale) * sds.t() @ q.abs(), s_dv=p.t() @ g.abs())
+        one = sees.double()
+        sdp = one * (1 + g.abs() @ v.abs().t() + (g.abs() * r["s_o"]).sum(-1, keepdim=True))
+        r.update(a_dq=abs(scale) * sdp @ k.abs(), a_dk=abs(scale) * sdp.t() @ q.abs(), a_dv=one.t() @ g.abs())
+    r["a_o"] = sees.double() @ v.abs()
+    return r
+
+
+def smallest(dtype):
+    """absolute error of a probability, of ds or of a result below the normal range: the exponential's subnormal results are
+    flushed (2^-126, f32 and bf16); IEEE half rounds there by half its smallest step, 2^-25.  The a_* sums carry it through
+    the second product."""
+    return 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+
+
+# Attention.  A score is a product of D <= 128 terms summed in f32 by matrix instructions: |error| <= D u times the sum of
+# sizes (s_score), so an exponential carries e = D u s_score + 4 u relative, and so does the sum of exponentials.
+# Probabilities (and ds) are rounded to the tensors' type before the second product: h each relative; its sum over n keys
+# is n u at worst.  The output is rounded once.  A relative error common to numerator and denominator only cancels in part:
+# both are counted.
+def attention_relative(D, s_score, n, dtype):
+    """of a probability-weighted sum of n terms against its sum of sizes, in front of the last rounding"""
+    h = half_step(dtype) if dtype != torch.float32 else 0.0
+    return h + 2 * (D * U * s_score + 4 * U) + n * U

@@ -1,0 +1,263 @@
+"""Causal attention over packed sequences (melgpt_packed_attn_*) against its definition in 64 bits."""
+import pytest
+import torch
+
+import packed_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _half():
+    from melspec_gpt_vqvae_amd import _ffi
+
+    return _ffi.HALF_DTYPE
+
+
+def _dt(name):
+    return torch.float32 if name == "f32" else _half()
+
+
+def _cu(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32)
+
+
+def make(lens_q, lens_k, Hq, Hk, D, dtype, seed, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn(sum(lens_q), Hq, D, generator=g) * std).to(dtype)
+    kv = torch.randn(sum(lens_k), 2, Hk, D, generator=g).to(dtype)
+    do = torch.randn(sum(lens_q), Hq, D, generator=g).to(dtype)
+    return q, kv[:, 0], kv[:, 1], do
+
+
+def reference(q, k, v, lens_q, lens_k, scale, do=None):
+    """per (sequence, query head) results of packed_ref.attention"""
+    Hq, Hk = q.shape[1], k.shape[1]
+    cq, ck = _cu(lens_q).tolist(), _cu(lens_k).tolist()
+    for s in range(len(lens_q)):
+        a, b = slice(cq[s], cq[s + 1]), slice(ck[s], ck[s + 1])
+        for h in range(Hq):
+            yield a, b, h, h // (Hq // Hk), R.attention(q[a, h], k[b, h // (Hq // Hk)], v[b, h // (Hq // Hk)], scale,
+                                                        None if do is None else do[a, h])
+
+
+def check(lens_q, lens_k, Hq, Hk, D, dtype, backward=True, seed=0, scale=None, std=1.0):
+    from melspec_gpt_vqvae_amd import ops
+    from melspec_gpt_vqvae_amd.transformer.packed import packed_attention
+
+    q, k, v, do = make(lens_q, lens_k, Hq, Hk, D, dtype, seed, std)
+    sc = D ** -0.5 if scale is None else scale
+    leaves = [x.to(DEV).requires_grad_(backward) for x in (q, k, v)]
+    cu_q = _cu(lens_q).to(DEV)
+    cu_k = None if lens_k == lens_q else _cu(lens_k).to(DEV)
+    out = packed_attention(*leaves, cu_q, cu_k, scale=scale)
+    _, lse = ops.packed_attn_fwd(*[x.detach() for x in leaves], cu_q, cu_k, scale=scale)
+    assert out.dtype == dtype and out.shape == q.shape
+    if backward:
+        dq, dk, dv = torch.autograd.grad(out, leaves, do.to(DEV))
+        want_dk, want_dv = torch.zeros(k.shape).double(), torch.zeros(v.shape).double()
+        tol_dk, tol_dv = torch.zeros(k.shape).double(), torch.zeros(v.shape).double()
+    h2, tiny = R.half_step(dtype), R.smallest(dtype)
+    for a, b, h, hk, r in reference(q, k, v, lens_q, lens_k, sc, do if backward else None):
+        n = b.stop - b.start
+        rel = R.attention_relative(D, r["s_score"], n, dtype)[:, None]
+        what = f"rows {a.start}.. head {h}"
+        R.assert_within(out[a, h], r["o"], h2 * r["o"].abs() + rel * r["s_o"] + tiny * (1 + r["a_o"]), "out " + what)
+        R.assert_within(lse[h, a], r["lse"], (D + 4) * R.U * r["s_score"] + (n + 4) * R.U + 4 * R.U * r["lse"].abs().nan_to_num(posinf=0), "lse " + what)
+        if backward:
+            # delta is formed with the stored output (h |o| more), the scores against the stored log-sum (its error, as above):
+            # twice the forward's relative error, and once more h for ds and p
+            rel = 3 * rel + 8 * R.U + 2 * R.U * r["lse"].abs().nan_to_num(posinf=0)[:, None]
+            R.assert_within(dq[a, h], r["dq"], h2 * r["dq"].abs() + _max(rel) * r["s_dq"] + tiny * (1 + r["a_dq"]), "dq " + what)
+            want_dk[b, hk] += r["dk"]
+            want_dv[b, hk] += r["dv"]
+            m = _max(rel) + (a.stop - a.start) * (Hq // Hk) * R.U
+            tol_dk[b, hk] += m * r["s_dk"] + tiny * (1 + r["a_dk"])
+            tol_dv[b, hk] += m * r["s_dv"] + tiny * (1 + r["a_dv"])
+    if backward:
+        R.assert_within(dk, want_dk, h2 * want_dk.abs() + tol_dk, "dk")
+        R.assert_within(dv, want_dv, h2 * want_dv.abs() + tol_dv, "dv")
+
+
+def _max(x):
+    return float(x.max()) if x.numel() else 0.0
+
+
+LENS = [([1], [1]), ([266], [266]), ([64, 1, 63, 65, 31, 32, 33, 128], None), ([5, 300, 129], [40, 301, 129]), ([1, 1, 1], [513, 7, 64]),
+        ([70, 33, 3], [10, 0, 3]), ([0, 40, 0, 0, 17], [5, 40, 0, 3, 17]), ([129], [1000])]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", range(len(LENS)))
+def test_lengths(lens, D, dtype):
+    lq, lk = LENS[lens]
+    check(lq, lk or lq, 4, 2, D, _dt(dtype), seed=lens)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (16, 16), (7, 1), (24, 8), (32, 2)])
+def test_heads(Hq, Hk, dtype):
+    check([100, 37], [100, 37], Hq, Hk, 64, _dt(dtype), seed=5)
+
+
+def test_scale_and_large_scores():
+    check([130], [130], 2, 1, 64, _half(), scale=0.5, std=4.0)
+    check([130], [130], 2, 1, 128, torch.float32, scale=1.0, std=3.0)
+    check([50], [50], 2, 2, 64, torch.float32, scale=-0.125)
+
+
+def test_many_short_sequences():
+    lens = [(7 * i) % 5 for i in range(5000)]                     # more sequences than one 64-way step of the search covers
+    check(lens[:300], lens[:300], 2, 1, 64, _half(), seed=2)
+    from melspec_gpt_vqvae_amd import ops
+
+    q, k, v, _ = make(lens, lens, 2, 1, 64, _half(), 3)
+    out, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), _cu(lens).to(DEV))
+    first = _cu(lens)[:-1].long()[torch.tensor(lens) > 0]         # the first query of a sequence sees its own key alone
+    assert torch.equal(out.cpu()[first], v[first].expand(-1, 2, -1))
+
+
+def test_rows_behind_the_last_sequence():
+    from melspec_gpt_vqvae_amd import ops
+
+    dt = _half()
+    q, k, v, do = [x.to(DEV) for x in make([200], [200], 4, 2, 64, dt, 4)]
+    q, k, v, do = q.clone(), k.clone(), v.clone(), do.clone()
+    cu = torch.tensor([10, 50, 131], dtype=torch.int32, device=DEV)             # rows 0..9 and 131..199 belong to nobody
+    for x in (q, k, v, do):
+        x[:10] = float("nan")
+        x[131:] = float("nan")
+    out, lse = ops.packed_attn_fwd(q, k, v, cu)
+    grads = ops.packed_attn_bwd(q, k, v, out, do, lse, cu)
+    base, _ = ops.packed_attn_fwd(q[10:131], k[10:131], v[10:131], cu - 10)
+    assert torch.equal(out[10:131], base)
+    for x in (out,) + grads:
+        assert float(x[:10].abs().max()) == 0.0 and float(x[131:].abs().max()) == 0.0
+        assert torch.isfinite(x.float()).all()
+    assert torch.isinf(lse[:, 131:]).all()
+    given = torch.full_like(out, 5.0)
+    left = [torch.full_like(g, 5.0) for g in grads]
+    ops.packed_attn_fwd(q, k, v, cu, out=given)
+    ops.packed_attn_bwd(q, k, v, given, do, lse, cu, grads=left)
+    for x, y in zip((given, *left), (out, *grads)):
+        assert torch.equal(x[10:131], y[10:131])
+        assert (x[:10] == 5).all() and (x[131:] == 5).all()
+
+
+def test_offsets_out_of_range_stay_inside():
+    from melspec_gpt_vqvae_amd import ops
+
+    q, k, v, do = [x.to(DEV) for x in make([100], [100], 2, 1, 64, _half(), 4)]
+    for cu in ([0, 60, 4000], [-5, 60, 100], [0, 80, 20, 100], [100, 50, 0], [0, 0, 0]):
+        cu = torch.tensor(cu, dtype=torch.int32, device=DEV)
+        out, lse = ops.packed_attn_fwd(q, k, v, cu)
+        ops.packed_attn_bwd(q, k, v, out, do, lse, cu)
+    cu = torch.tensor([0, 60, 4000], dtype=torch.int32, device=DEV)             # the last offset stands for the end
+    good = torch.tensor([0, 60, 100], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.packed_attn_fwd(q, k, v, cu)[0], ops.packed_attn_fwd(q, k, v, good)[0])
+
+
+def test_strides_broadcast_and_no_rows():
+    from melspec_gpt_vqvae_amd import ops
+    from melspec_gpt_vqvae_amd.transformer.packed import packed_attention
+
+    dt = _half()
+    q, k, v, do = [x.to(DEV) for x in make([77, 20], [77, 20], 4, 2, 64, dt, 8)]
+    cu = _cu([77, 20]).to(DEV)
+    base, lse = ops.packed_attn_fwd(q, k, v, cu)
+    heads_out = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)
+    odd = torch.zeros(97 * 4 * 64 + 1, dtype=dt, device=DEV)[1:].view(97, 4, 64)
+    odd.copy_(q)
+    assert torch.equal(ops.packed_attn_fwd(heads_out(q), heads_out(k), heads_out(v), cu)[0], base)
+    assert torch.equal(ops.packed_attn_fwd(odd, k, v, cu)[0], base)
+    g0 = ops.packed_attn_bwd(q, k, v, base, do, lse, cu)
+    block = torch.empty(97, 8 * 64, dtype=dt, device=DEV)          # q | k | v gradients side by side
+    views = (block[:, :256].unflatten(1, (4, 64)), block[:, 256:384].unflatten(1, (2, 64)), block[:, 384:].unflatten(1, (2, 64)))
+    ops.packed_attn_bwd(heads_out(q), heads_out(k), v, heads_out(base), heads_out(do), lse, cu, grads=views)
+    assert all(torch.equal(a, b) for a, b in zip(g0, views))
+    # one key head broadcast to two by the caller: its gradient is the sum of both
+    k1, v1 = k[:, :1].clone().requires_grad_(True), v[:, :1].clone().requires_grad_(True)
+    out = packed_attention(q, k1.expand(-1, 2, -1), v1.expand(-1, 2, -1), cu)
+    gk, gv = torch.autograd.grad(out, (k1, v1), do)
+    out2 = packed_attention(q, k1, v1, cu)
+    assert torch.equal(out, out2)
+    hk, hv = torch.autograd.grad(out2, (k1, v1), do)
+    # two halves each rounded, then their rounded sum, against one rounding
+    for a, b in ((gk, hk), (gv, hv)):
+        assert float((a.float() - b.float()).abs().max()) <= 4 * R.half_step(dt) * float(b.float().abs().max())
+    none = torch.zeros(0, 4, 64, dtype=dt, device=DEV)
+    assert packed_attention(none, none[:, :2], none[:, :2], _cu([0, 0]).to(DEV)).shape == (0, 4, 64)
+    o, l = ops.packed_attn_fwd(q, none[:, :2], none[:, :2], cu, _cu([0, 0]).to(DEV))
+    assert float(o.abs().max()) == 0.0 and torch.isinf(l).all()
+    dq, dk, dv = ops.packed_attn_bwd(q, none[:, :2], none[:, :2], o, do, l, cu, _cu([0, 0]).to(DEV))
+    assert float(dq.abs().max()) == 0.0 and dk.shape == (0, 2, 64)
+
+
+def test_gradient_against_differences_and_reproducible():
+    from melspec_gpt_vqvae_amd.transformer.packed import packed_attention
+
+    lens = [40, 1, 75]
+    q, k, v, do = make(lens, lens, 4, 2, 64, torch.float32, 12)
+    cu = _cu(lens).to(DEV)
+    leaves = [x.to(DEV).requires_grad_(True) for x in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention(*leaves, cu), leaves, do.to(DEV))
+    for _ in range(3):
+        again = torch.autograd.grad(packed_attention(*leaves, cu), leaves, do.to(DEV))
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+    def value(x):
+        return sum(float((r["o"] * do[a, h].double()).sum()) for a, b, h, hk, r in reference(*x, lens, lens, 0.125))
+
+    g = torch.Generator().manual_seed(1)
+    base = [x.double() for x in (q, k, v)]
+    for i in range(3):
+        d = torch.randn(base[i].shape, generator=g).double()
+        up, down = list(base), list(base)
+        up[i], down[i] = base[i] + 1e-5 * d, base[i] - 1e-5 * d
+        slope = (value(up) - value(down)) / 2e-5
+        mine = float((grads[i].double().cpu() * d).sum())
+        size = float((grads[i].double().cpu().abs() * d.abs()).sum())
+        assert abs(mine - slope) <= 1e-5 * size, (i, mine, slope, size)   # f32 gradients: D u s_score ~ 128 * 6e-8 relative
+
+
+def test_captured_and_replayed():
+    """forward and backward in a graph, replayed with new inputs and new lengths; other work between the replays"""
+    from melspec_gpt_vqvae_amd import ops
+
+    dt = _half()
+    q, k, v, do = [x.to(DEV).clone() for x in make([150], [150], 4, 2, 128, dt, 1)]
+    cu = torch.tensor([0, 70, 150], dtype=torch.int32, device=DEV)
+
+    def step():
+        out, lse = ops.packed_attn_fwd(q, k, v, cu)
+        return (out, lse) + ops.packed_attn_bwd(q, k, v, out, do, lse, cu)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for i in range(4):
+        q.mul_(0.9)
+        v.add_(0.1 * i)
+        cu[1] = 1 + 40 * i
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_other_stream():
+    from melspec_gpt_vqvae_amd import ops
+
+    q, k, v, do = [x.to(DEV) for x in make([300], [300], 4, 2, 64, _half(), 1)]
+    cu = _cu([300]).to(DEV)
+    want = ops.packed_attn_fwd(q, k, v, cu)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got, lse = ops.packed_attn_fwd(q, k, v, cu)
+        grads = ops.packed_attn_bwd(q, k, v, got, do, lse, cu)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want) and all(torch.isfinite(x.float()).all() for x in grads)
