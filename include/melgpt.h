@@ -594,6 +594,18 @@ int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, con
                            int write_gaps, long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype,
                            void* stream);
 
+/* Attention of one query token per sequence over the cache that melgpt_kv_append fills: q, out (S, Hq, D) with row and head
+ * strides, keys 0 .. lengths[s] - 1 of sequence s through page_table[s * table_ld + j / page_size] (columns beyond `width`
+ * do not exist, a page outside n_pages leaves its keys out; the kernel checks every index), lse (S, Hq) f32.  A sequence
+ * without keys gives 0 (lse -inf).  `splits` workgroups share a (sequence, key head): melgpt_paged_attn_splits proposes it
+ * from the longest length the caller knows of (any value gives the same result up to f32 rounding); with splits > 1
+ * `workspace` holds S * Hq * splits * (D + 2) f32, 16-byte aligned.  D 64 or 128, page_size a power of two. */
+int melgpt_paged_attn_splits(int S, int Hq, int Hk, long long max_length);
+int melgpt_paged_attn_decode(const void* q, long long q_row, long long q_head, const void* k_pages, const void* v_pages,
+                             long long n_pages, int page_size, const int* page_table, long long table_ld, int width,
+                             const int* lengths, int S, void* out, long long o_row, long long o_head, float* lse, int splits,
+                             float* workspace, int Hq, int Hk, int D, float scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,305 @@
+// Attention of one query token per sequence over a paged key / value cache (the reader of melgpt_kv_append's pages).
+//
+//   sequence s: keys 0 .. lengths[s] - 1, key j in page page_table[s][j / page_size], slot j % page_size;
+//   query head h reads key head h / G:  o = sum_j softmax_j(scale q . k_j) v_j,  lse = log sum_j e^(scale q . k_j)
+//
+// Bound by HBM: every key and value is read once, for all G query heads of its key head together - the G queries are the
+// columns of a 16-wide matrix tile (one tile per 16 heads), so grouped heads cost no more reads than one.
+// Keys go from memory straight into the score product's operand (S^T = K Q^T: 16 keys to a fragment, a lane holds 16 bytes
+// of a key row); values take the same lanes' way through a wave's own piece of LDS, whose transposed reads are the operand
+// of O^T = V^T P^T.  The waves of a workgroup share nothing until the end: each walks its own 32-key tiles with a running
+// maximum and sum, one tile's loads in flight under the previous tile's softmax and second product, and the page numbers of
+// the tile after that.  A sequence is split over several workgroups when there are few of them (see `splits`); their
+// partial results are joined by a second kernel in a fixed order.
+#include "mma.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+struct PagedParams {
+  const void* q;
+  long long q_row, q_head;
+  const void *k_pages, *v_pages;
+  const int *table, *lengths;
+  long long table_ld;
+  int width, pages, page_shift, Hq, Hk, G, splits;
+  void* o;
+  long long o_row, o_head;
+  float* lse;     // (S, Hq)
+  float* part;    // (S, Hq, splits, D) sums of e^(s - m) v, then (S, Hq, splits, 2): m (base 2), sum of e^(s - m)
+  long long stats;  // offset of the second part
+  float scale;
+};
+
+template <typename T, int D>
+struct Geo {
+  static constexpr int ES = Tr<T>::ES, RB = D * ES, CP = RB / 16, VEC = 16 / ES, NKS = CP / 4, DT = D / 16;
+  static constexpr int STEPS = ES == 2 ? 1 : 2;
+  static __device__ __forceinline__ int off(int row, int c) {
+    if constexpr (RB == 128) return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
+    else return row * RB + ((c ^ (row & 15)) << 4);
+  }
+  // operand of 16 values (16 dt + (lane & 15)) contracting over 32 keys of the tile (16-bit) or 16 (f32, step st)
+  static __device__ __forceinline__ u32x4 cols(const char* t, int st, int dt, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    if constexpr (ES == 2) {
+      const int r0 = 4 * g + (i >> 2), c = 2 * dt + ((i & 3) >> 1);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off(r0, c) + 8 * (i & 1)));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off(r0 + 16, c) + 8 * (i & 1)));
+      const s16x8 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(u32x4, f);
+    } else {
+      const int col = 16 * dt + i;
+      u32x4 f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = *(const unsigned*)(t + off(16 * st + 4 * g + e, col >> 2) + (col & 3) * 4);
+      return f;
+    }
+  }
+};
+
+__device__ __forceinline__ float over_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float over_groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
+  using L = Geo<T, D>;
+  __shared__ __attribute__((aligned(16))) char lds[4][32 * L::RB];
+  __shared__ float stat[4][2][16];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, i16 = lane & 15;
+  const int hk = blockIdx.x % p.Hk, s = blockIdx.x / p.Hk, split = blockIdx.y, h0 = hk * p.G + 16 * blockIdx.z;
+  const int nh = min(p.G - 16 * (int)blockIdx.z, 16);             // query heads of this workgroup
+  const long long cap = (long long)p.width << p.page_shift;
+  const int len = (int)min((long long)max(p.lengths[s], 0), min(cap, 0x7fffffc0LL));
+  const int tiles = (len + 31) >> 5, per = (tiles + p.splits - 1) / p.splits;
+  const int t0 = split * per, t1 = min(t0 + per, tiles);
+  const int* table = p.table + (long long)s * p.table_ld;
+  const T* kb = (const T*)p.k_pages;
+  const T* vb = (const T*)p.v_pages;
+  const T* qp = (const T*)p.q + s * p.q_row + (h0 + min(i16, nh - 1)) * p.q_head;
+  u32x4 qf[L::NKS];
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * L::VEC);
+  const float c2 = p.scale * LOG2E;
+  char* vt = lds[wave];
+  f32x4 o[L::DT];
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), l = 0.f;
+
+  // rows i16 and 16 + i16 of a tile: page numbers, then the rows themselves
+  const int mask = (1 << p.page_shift) - 1;
+  int page[2];
+  u32x4 kr[2][L::NKS], vr[2][L::NKS];
+  unsigned ok[2];                                                  // bit j: key j of the half tile exists
+  auto pages_of = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) page[i] = table[min(32 * tile + 16 * i + i16, len - 1) >> p.page_shift];
+  };
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = 32 * tile + 16 * i + i16;
+      const bool in = key < len && page[i] >= 0 && page[i] < p.pages;
+      ok[i] = (unsigned)__ballot(in) & 0xffffu;
+      const long long at = in ? ((((long long)page[i] * p.Hk + hk) << p.page_shift) + (key & mask)) * D : 0;
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks) kr[i][ks] = *(const u32x4*)(kb + at + (4 * ks + g) * L::VEC);
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks) vr[i][ks] = *(const u32x4*)(vb + at + (4 * ks + g) * L::VEC);
+    }
+  };
+  int tile = t0 + wave;
+  if (tile < t1) {
+    pages_of(tile);
+    load(tile);
+    pages_of(min(tile + 4, t1 - 1));
+  }
+  for (; tile < t1; tile += 4) {
+    f32x4 sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks) mma<T>(sc[i], kr[i][ks], qf[ks]);
+    }
+    const unsigned seen[2] = {ok[0], ok[1]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool in = (seen[i] >> i16) & 1;                        // (0 * NaN is not 0: rows that do not exist are zero)
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks)
+        *(u32x4*)(vt + L::off(16 * i + i16, 4 * ks + g)) = in ? vr[i][ks] : u32x4{0u, 0u, 0u, 0u};
+    }
+    if (tile + 4 < t1) {
+      load(tile + 4);
+      pages_of(min(tile + 8, t1 - 1));
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[i][r] = (seen[i] >> (4 * g + r)) & 1 ? sc[i][r] * c2 : -__builtin_inff();
+        top = fmaxf(top, sc[i][r]);
+      }
+    top = fmaxf(over_groups_max(top), m);
+    const float base = top == -__builtin_inff() ? 0.f : top;
+    const float keep = __builtin_amdgcn_exp2f(m - base);
+    m = top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[i][r] = __builtin_amdgcn_exp2f(sc[i][r] - base);
+        sum += sc[i][r];
+      }
+    l = l * keep + sum;
+#pragma unroll
+    for (int d = 0; d < L::DT; ++d) o[d] *= keep;
+#pragma unroll
+    for (int e = 0; e < L::STEPS; ++e) {
+      u32x4 pf;
+      if constexpr (L::ES == 2)
+        pf = u32x4{pack_bf16x2(sc[0][0], sc[0][1]), pack_bf16x2(sc[0][2], sc[0][3]), pack_bf16x2(sc[1][0], sc[1][1]),
+                   pack_bf16x2(sc[1][2], sc[1][3])};
+      else
+        pf = __builtin_bit_cast(u32x4, e ? sc[1] : sc[0]);
+#pragma unroll
+      for (int d = 0; d < L::DT; ++d) mma<T>(o[d], L::cols(vt, e, d, lane), pf);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+  l = over_groups_sum(l);
+  // ---- the four waves' results: through LDS (each its own piece, 16 queries x D f32, once its values are read)
+  static_assert(16 * D * 4 <= 32 * L::RB, "a wave's piece holds its result");
+  float* mine = (float*)vt;
+#pragma unroll
+  for (int d = 0; d < L::DT; ++d) *(f32x4*)(mine + i16 * D + 16 * d + 4 * g) = o[d];
+  if (g == 0) {
+    stat[wave][0][i16] = m;
+    stat[wave][1][i16] = l;
+  }
+  __syncthreads();
+  constexpr int TPQ = D / 4;                                       // threads of one query: four values each
+  for (int q = t / TPQ; q < nh; q += 256 / TPQ) {
+    const int d = 4 * (t % TPQ);
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][0][q]);
+    const float base = top == -__builtin_inff() ? 0.f : top;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(stat[w][0][q] - base);
+      a += *(const f32x4*)((const float*)lds[w] + q * D + d) * f;
+      sum += stat[w][1][q] * f;
+    }
+    const long long head = (long long)s * p.Hq + h0 + q;
+    if (p.splits == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T* op = (T*)p.o + s * p.o_row + (h0 + q) * p.o_head + d;
+      if constexpr (L::ES == 2) *(u32x2*)op = u32x2{pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv)};
+      else *(f32x4*)op = a * inv;
+      if (d == 0) p.lse[head] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * LN2;
+    } else {
+      *(f32x4*)(p.part + (head * p.splits + split) * D + d) = a;
+      if (d == 0) {
+        p.part[p.stats + 2 * (head * p.splits + split)] = top;
+        p.part[p.stats + 2 * (head * p.splits + split) + 1] = sum;
+      }
+    }
+  }
+}
+
+// joins the splits of one (sequence, query head): D / 4 lanes, four values each, in split order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, long long heads) {
+  constexpr int TPQ = D / 4;
+  const long long head = (long long)blockIdx.x * (256 / TPQ) + threadIdx.x / TPQ;
+  if (head >= heads) return;
+  const int d = 4 * (threadIdx.x % TPQ);
+  const float* st = p.part + p.stats + 2 * head * p.splits;
+  const float* pp = p.part + head * p.splits * D + d;
+  float top = -__builtin_inff();
+  for (int i = 0; i < p.splits; ++i) top = fmaxf(top, st[2 * i]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < p.splits; ++i) {
+    const float f = __builtin_amdgcn_exp2f(st[2 * i] - base);
+    a += *(const f32x4*)(pp + (long long)i * D) * f;
+    sum += st[2 * i + 1] * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* op = (T*)p.o + (head / p.Hq) * p.o_row + (head % p.Hq) * p.o_head + d;
+  if constexpr (sizeof(T) == 2) *(u32x2*)op = u32x2{pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv)};
+  else *(f32x4*)op = a * inv;
+  if (d == 0) p.lse[head] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * LN2;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename T, int D>
+int launch(const PagedParams& p, int S, hipStream_t s) {
+  hipLaunchKernelGGL((paged_decode_kernel<T, D>), dim3((unsigned)(S * p.Hk), p.splits, (p.G + 15) / 16), dim3(256), 0, s, p);
+  if (p.splits > 1) {
+    const long long heads = (long long)S * p.Hq, per = 256 / (D / 4);
+    hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)((heads + per - 1) / per)), dim3(256), 0, s, p, heads);
+  }
+  return melgpt_launch_status();
+}
+
+}  // namespace
+
+// Workgroups per (sequence, key head): enough of them that the longest sequences do not finish alone, each with at least
+// 256 keys (two tiles per wave).
+extern "C" int melgpt_paged_attn_splits(int S, int Hq, int Hk, long long max_length) {
+  if (S <= 0 || Hk <= 0 || Hq < Hk || max_length <= 0) return 1;
+  const long long base = (long long)S * Hk * ((Hq / Hk + 15) / 16), most = (max_length + 255) / 256;
+  long long n = (4096 + base - 1) / base;
+  if (n > most) n = most;
+  if (n > 128) n = 128;
+  return (int)(n < 1 ? 1 : n);
+}
+
+extern "C" int melgpt_paged_attn_decode(const void* q, long long q_row, long long q_head, const void* k_pages,
+                                        const void* v_pages, long long n_pages, int page_size, const int* page_table,
+                                        long long table_ld, int width, const int* lengths, int S, void* out, long long o_row,
+                                        long long o_head, float* lse, int splits, float* workspace, int Hq, int Hk, int D,
+                                        float scale, int dtype, void* stream) {
+  if (S == 0) return MELGPT_OK;
+  if (S < 0 || Hq <= 0 || Hk <= 0 || width <= 0 || n_pages <= 0 || splits <= 0 || page_size <= 0) return MELGPT_ERR_BAD_ARG;
+  if (!q || !k_pages || !v_pages || !page_table || !lengths || !out || !lse || (splits > 1 && !workspace)) return MELGPT_ERR_BAD_ARG;
+  if (dtype != MELGPT_F32 && dtype != MELGPT_BF16) return MELGPT_ERR_UNSUPPORTED;
+  if ((D != 64 && D != 128) || Hq % Hk || (page_size & (page_size - 1)) || page_size > (1 << 20) || n_pages > 0x7fffffffLL ||
+      splits > 65535 || (long long)S * Hk > 0xffffff || Hq / Hk > 1024)
+    return MELGPT_ERR_UNSUPPORTED;
+  const int vec = dtype == MELGPT_F32 ? 4 : 8;
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(workspace) || q_row % vec ||
+      q_head % vec || o_row % vec || o_head % vec)
+    return MELGPT_ERR_ALIGN;
+  PagedParams p = {};
+  p.q = q; p.q_row = q_row; p.q_head = q_head; p.k_pages = k_pages; p.v_pages = v_pages; p.table = page_table; p.lengths = lengths;
+  p.table_ld = table_ld; p.width = width; p.pages = (int)n_pages; p.Hq = Hq; p.Hk = Hk; p.G = Hq / Hk; p.splits = splits;
+  p.o = out; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.part = workspace; p.stats = (long long)S * Hq * splits * D;
+  p.scale = scale;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == MELGPT_F32) return D == 64 ? launch<float, 64>(p, S, st) : launch<float, 128>(p, S, st);
+  return D == 64 ? launch<bf16_t, 64>(p, S, st) : launch<bf16_t, 128>(p, S, st);
+}

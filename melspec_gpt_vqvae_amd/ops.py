@@ -1185,3 +1185,34 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
              ptr(lse), ptr(delta), ptr(dq), dq.stride(0), dq.stride(1), ptr(dk), dk.stride(0), dk.stride(1), ptr(dv), dv.stride(0),
              dv.stride(1), int(gaps), Mq, Mk, Hq, Hk, D, float(scale if scale is not None else D ** -0.5), dt, stream())
     return dq, dk, dv
+
+
+def paged_attn_decode(q, k_pages, v_pages, page_table, lengths, *, scale=None, max_length=None, out=None):
+    """Attention of one query token per sequence over a paged cache: q (S, Hq, D), any row and head strides; k_pages, v_pages
+    (pages, Hk, page size, D), Hq a multiple of Hk; page_table (S, width) int32; lengths (S,) int32, the keys each sequence
+    has (those of kv_append's last row among them) -> (out (S, Hq, D), lse (S, Hq) f32).  A sequence without keys gives 0; a
+    table entry outside the pages leaves its keys out.  max_length: the longest length, where the caller knows one shorter
+    than the table's width (it only decides how far a sequence is split).  scale: 1 / sqrt(D) unless given."""
+    S, Hq, D = q.shape
+    dt = dtype_code(q.dtype)
+    with _on(q.device):
+        P, Hk, page, Dp = _pages_of(k_pages, v_pages, page_table, q.dtype, q.device)
+        assert D == Dp and D in (64, 128), f"head size {D} (cache {Dp}): 64 or 128"
+        assert Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads over {Hk} key heads"
+        assert page_table.shape[0] == S and lengths.dtype == torch.int32 and lengths.shape == (S,) and lengths.is_contiguous()
+        _same_device(q.device, lengths=lengths, out=out)
+        q = _heads(q, "q")
+        if out is None:
+            out = torch.empty(S, Hq, D, dtype=q.dtype, device=q.device)
+        else:
+            assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        lse = torch.empty(S, Hq, dtype=torch.float32, device=q.device)
+        width = page_table.shape[1]
+        assert S == 0 or (width > 0 and P > 0), "a cache without pages"
+        bound = width * page if max_length is None else min(int(max_length), width * page)
+        splits = _ffi.lib().melgpt_paged_attn_splits(S, Hq, Hk, bound)
+        ws = torch.empty(S * Hq * splits * (D + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        call("melgpt_paged_attn_decode", ptr(q), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages), P, page, ptr(page_table),
+             page_table.stride(0), width, ptr(lengths), S, ptr(out), out.stride(0), out.stride(1), ptr(lse), splits, ptr(ws), Hq, Hk,
+             D, float(scale if scale is not None else D ** -0.5), dt, stream())
+    return out, lse
