@@ -275,6 +275,187 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
   if (g == 0) p.lse[h * p.Mq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
+// ------------------------------------------------------------------------------------- forward, 16-bit operands
+// 256 threads, 128 queries of one head: a wave owns 32 queries (v_mfma_f32_32x32x16: twice the queries per fragment read from
+// LDS, which 16-row tiles are bound by) and walks the keys 64 at a time.
+template <int D>
+struct Tile32 {
+  static constexpr int RB = 2 * D, CP = RB / 16, NKS = D / 16, DB = D / 32;
+  // keys / rows read along D, 32 rows a time
+  static __device__ __forceinline__ int off_r(int row, int c) {
+    if constexpr (RB == 128) return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
+    else return row * RB + ((c ^ (row & 15)) << 4);
+  }
+  // values, read transposed: 8 rows x 64 bytes an instruction, spread over all banks
+  static __device__ __forceinline__ int off_t(int row, int c) {
+    if constexpr (RB == 128) return row * 128 + ((c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3))) << 4);
+    else return row * RB + ((c ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+  }
+  static __device__ __forceinline__ u32x4 rows(const char* t, int blk, int ks, int lane) {
+    return *(const u32x4*)(t + off_r(32 * blk + (lane & 31), 2 * ks + (lane >> 5)));
+  }
+  // 32 columns of block db, contraction over 16 rows, step st: slot j of lane half hh is row 16 st + 8 (j >> 2) + 4 hh + (j & 3),
+  // the order in which accumulators 8 (st & 1) .. + 7 of a 32-row score block hold them
+  static __device__ __forceinline__ u32x4 cols(const char* t, int st, int db, int lane) {
+    const int hh = lane >> 5, q4 = (lane & 15) >> 2, p4 = lane & 3, g1 = (lane >> 4) & 1;
+    const int row = 16 * st + 4 * hh + q4, c = 4 * db + 2 * g1 + (p4 >> 1);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off_t(row, c) + 8 * (p4 & 1)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off_t(row + 8, c) + 8 * (p4 & 1)));
+    const s16x8 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(u32x4, f);
+  }
+};
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+// accumulators 8 st .. 8 st + 7 of a 32-row block as the operand of a 16-row contraction
+__device__ __forceinline__ u32x4 operand16(const f32x16& s, int st) {
+  return u32x4{pack_bf16x2(s[8 * st], s[8 * st + 1]), pack_bf16x2(s[8 * st + 2], s[8 * st + 3]),
+               pack_bf16x2(s[8 * st + 4], s[8 * st + 5]), pack_bf16x2(s[8 * st + 6], s[8 * st + 7])};
+}
+
+// 64 rows of two tensors through registers into LDS (256 threads)
+template <int D>
+struct Stage64 {
+  using L = Tile32<D>;
+  static constexpr int PER = 64 * L::CP / 256;
+  u32x4 a[PER], b[PER];
+  __device__ __forceinline__ void load(const bf16_t* pa, long long ra, const bf16_t* pb, long long rb, int row0, int n, int t) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int q = t + 256 * i, row = min(row0 + q / L::CP, n - 1), c = q % L::CP;
+      a[i] = *(const u32x4*)(pa + row * ra + c * 8);
+      b[i] = *(const u32x4*)(pb + row * rb + c * 8);
+    }
+  }
+  template <bool TA, bool TB>
+  __device__ __forceinline__ void store(char* ta, char* tb, int row0, int n, int t) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int q = t + 256 * i, row = q / L::CP, c = q % L::CP;
+      const bool in = row0 + row < n;
+      const u32x4 z = {0u, 0u, 0u, 0u};
+      *(u32x4*)(ta + (TA ? L::off_t(row, c) : L::off_r(row, c))) = in ? a[i] : z;
+      *(u32x4*)(tb + (TB ? L::off_t(row, c) : L::off_r(row, c))) = in ? b[i] : z;
+    }
+  }
+};
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
+  using L = Tile32<D>;
+  using T = bf16_t;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * L::RB];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
+  int h;
+  head_of(blockIdx.x, p, h);
+  const Rows R = find_rows<128>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  if (!R.any) return;
+  int k_lo, nk;
+  other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
+  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
+  const int w0 = 128 * R.tile + 32 * wave;                         // the wave's first query
+  const int q_in = w0 + (lane & 31);
+  const bool mine = q_in < R.n;
+  const long long row = R.lo + min(q_in, R.n - 1);
+  const int sees = min(max(q_in + nk - R.n + 1, 0), nk);
+  const int last = min(128 * R.tile + 127, R.n - 1);
+  const int most = min(max(last + nk - R.n + 1, 0), nk);
+  // keys that every query of the wave sees, and that any of them does
+  const int full = min(max(w0 + nk - R.n + 1, 0), nk), any = min(max(min(w0 + 31, R.n - 1) + nk - R.n + 1, 0), nk);
+  const T* qp = (const T*)p.q + row * p.q_row + h * p.q_head;
+  u32x4 qf[L::NKS];
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) qf[ks] = *(const u32x4*)(qp + 16 * ks + 8 * hh);
+  const T* kp = (const T*)p.k + (long long)k_lo * p.k_row + (h / p.G) * p.k_head;
+  const T* vp = (const T*)p.v + (long long)k_lo * p.v_row + (h / p.G) * p.v_head;
+  const float c2 = p.scale * LOG2E;
+  f32x16 o[L::DB];
+#pragma unroll
+  for (int d = 0; d < L::DB; ++d) o[d] = zero16();
+  float m = -__builtin_inff(), l = 0.f;
+  if (most > 0) {
+    Stage64<D> st;
+    st.load(kp, p.k_row, vp, p.v_row, 0, nk, t);
+    st.template store<false, true>(lds[0][0], lds[0][1], 0, nk, t);
+    __syncthreads();
+    for (int k0 = 0, buf = 0; k0 < most; k0 += 64, buf ^= 1) {
+      const bool more = k0 + 64 < most;
+      if (more) st.load(kp, p.k_row, vp, p.v_row, k0 + 64, nk, t);
+      const char *kt = lds[buf][0], *vt = lds[buf][1];
+      if (k0 < any) {
+        f32x16 s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < L::NKS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i] = MELGPT_MFMA_32x32x16(L::rows(kt, i, ks, lane), qf[ks], s[i]);
+        if (k0 + 64 > full) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[i][r] = k0 + 32 * i + 8 * (r >> 2) + 4 * hh + (r & 3) < sees ? s[i][r] * c2 : -__builtin_inff();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[i][r] *= c2;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // the running maximum follows only when it is passed by more than 2^8: until then terms up to 2^8 are exact enough in
+        // f32 sums and 16-bit operands alike, and the 16 DB accumulators need no rescaling (rare after the first tiles)
+        if (__any(top > m + 8.f)) {
+          const float now = fmaxf(m, top), base = now == -__builtin_inff() ? 0.f : now;
+          const float keep = __builtin_amdgcn_exp2f(m - base);
+          m = now;
+          l *= keep;
+#pragma unroll
+          for (int d = 0; d < L::DB; ++d) o[d] *= keep;
+        }
+        const float base = m == -__builtin_inff() ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - base);
+            sum += s[i][r];
+          }
+        }
+        l += sum;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u32x4 pf = operand16(s[e >> 1], e & 1);
+#pragma unroll
+          for (int d = 0; d < L::DB; ++d) o[d] = MELGPT_MFMA_32x32x16(L::cols(vt, e, d, lane), pf, o[d]);
+        }
+      }
+      if (more) st.template store<false, true>(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 64, nk, t);
+      __syncthreads();
+    }
+    l += __shfl_xor(l, 32, 64);
+  }
+  if (!mine) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* op = (T*)p.o + row * p.o_row + h * p.o_head;
+#pragma unroll
+  for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      store4<T>(op + 32 * d + 8 * j + 4 * hh, f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv);
+  if (hh == 0) p.lse[h * p.Mq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
 // -------------------------------------------------------------------------------------------------------- backward
 // dq and delta: the forward's walk with a second score product, do . v, on the same tiles
 template <typename T, int D>
@@ -480,9 +661,12 @@ int check(const PackedParams& p, int D, int dtype) {
 
 template <typename T, int D>
 int launch_fwd(const PackedParams& p, hipStream_t s) {
-  const long long tiles = tiles_for(p.Mq, p.S, 64);
+  const long long tiles = tiles_for(p.Mq, p.S, sizeof(T) == 2 ? 128 : 64);
   if (tiles > 65535) return MELGPT_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((packed_fwd_kernel<T, D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
+  if constexpr (sizeof(T) == 2)
+    hipLaunchKernelGGL((packed_fwd32_kernel<D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((packed_fwd_kernel<T, D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
   return melgpt_launch_status();
 }
 
