@@ -317,29 +317,52 @@ __device__ __forceinline__ u32x4 operand16(const f32x16& s, int st) {
                pack_bf16x2(s[8 * st + 4], s[8 * st + 5]), pack_bf16x2(s[8 * st + 6], s[8 * st + 7])};
 }
 
-// 64 rows of two tensors through registers into LDS (256 threads)
-template <int D>
+// 64 rows of two tensors through registers into LDS (256 threads).  A thread's rows are 64 / PER apart and its addresses
+// one base and a uniform step: the 64-bit products of a row's address cost as much as the softmax when formed per row.
+template <int D, bool TA, bool TB>   // TA, TB: laid out for transposed reads
 struct Stage64 {
   using L = Tile32<D>;
-  static constexpr int PER = 64 * L::CP / 256;
+  static constexpr int PER = 64 * L::CP / 256, STEP = 64 / PER;
+  const bf16_t *pa, *pb;
+  long long ra, rb;
+  int row, off_a, off_b;   // first row, its place in LDS (rows STEP apart keep the swizzle: STEP is a multiple of 16)
   u32x4 a[PER], b[PER];
-  __device__ __forceinline__ void load(const bf16_t* pa, long long ra, const bf16_t* pb, long long rb, int row0, int n, int t) {
+  static_assert(STEP % 16 == 0, "rows of a thread share their swizzle");
+  __device__ __forceinline__ Stage64(const bf16_t* a0, long long ra_, const bf16_t* b0, long long rb_, int t) : ra(ra_), rb(rb_) {
+    const int c = t % L::CP;
+    row = t / L::CP;
+    pa = a0 + row * ra + c * 8;
+    pb = b0 + row * rb + c * 8;
+    off_a = TA ? L::off_t(row, c) : L::off_r(row, c);
+    off_b = TB ? L::off_t(row, c) : L::off_r(row, c);
+  }
+  __device__ __forceinline__ void load(int row0, int n) {
+    if (row0 + 64 <= n) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int q = t + 256 * i, row = min(row0 + q / L::CP, n - 1), c = q % L::CP;
-      a[i] = *(const u32x4*)(pa + row * ra + c * 8);
-      b[i] = *(const u32x4*)(pb + row * rb + c * 8);
+      for (int i = 0; i < PER; ++i) {
+        a[i] = *(const u32x4*)(pa + (row0 + STEP * i) * ra);
+        b[i] = *(const u32x4*)(pb + (row0 + STEP * i) * rb);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {   // rows behind the last are the last
+        const long long r = min(row0 + row + STEP * i, n - 1) - row;
+        a[i] = *(const u32x4*)(pa + r * ra);
+        b[i] = *(const u32x4*)(pb + r * rb);
+      }
     }
   }
-  template <bool TA, bool TB>
-  __device__ __forceinline__ void store(char* ta, char* tb, int row0, int n, int t) const {
+  // rows behind the last are zero: their scores are masked, but 0 * NaN is not 0
+  __device__ __forceinline__ void store(char* ta, char* tb, int row0, int n) {
+    if (row0 + 64 > n) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (row0 + row + STEP * i >= n) a[i] = b[i] = u32x4{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int q = t + 256 * i, row = q / L::CP, c = q % L::CP;
-      const bool in = row0 + row < n;
-      const u32x4 z = {0u, 0u, 0u, 0u};
-      *(u32x4*)(ta + (TA ? L::off_t(row, c) : L::off_r(row, c))) = in ? a[i] : z;
-      *(u32x4*)(tb + (TB ? L::off_t(row, c) : L::off_r(row, c))) = in ? b[i] : z;
+      *(u32x4*)(ta + off_a + i * STEP * L::RB) = a[i];
+      *(u32x4*)(tb + off_b + i * STEP * L::RB) = b[i];
     }
   }
 };
@@ -370,21 +393,30 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   u32x4 qf[L::NKS];
 #pragma unroll
   for (int ks = 0; ks < L::NKS; ++ks) qf[ks] = *(const u32x4*)(qp + 16 * ks + 8 * hh);
+  // the maximum is taken over the unscaled products: a negative scale goes into the queries' signs, a zero one (every key
+  // alike, and no 0 * inf at the masked ones) into zero queries
+  if (p.scale <= 0.f) {
+    const unsigned flip = p.scale < 0.f ? 0x80008000u : 0u, keep = p.scale < 0.f ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int ks = 0; ks < L::NKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[ks][e] = (qf[ks][e] ^ flip) & keep;
+  }
   const T* kp = (const T*)p.k + (long long)k_lo * p.k_row + (h / p.G) * p.k_head;
   const T* vp = (const T*)p.v + (long long)k_lo * p.v_row + (h / p.G) * p.v_head;
-  const float c2 = p.scale * LOG2E;
+  const float c2 = p.scale == 0.f ? 1.f : fabsf(p.scale) * LOG2E;
   f32x16 o[L::DB];
 #pragma unroll
   for (int d = 0; d < L::DB; ++d) o[d] = zero16();
-  float m = -__builtin_inff(), l = 0.f;
+  float m = -__builtin_inff(), l[4] = {0.f, 0.f, 0.f, 0.f};        // four partial sums: independent chains
   if (most > 0) {
-    Stage64<D> st;
-    st.load(kp, p.k_row, vp, p.v_row, 0, nk, t);
-    st.template store<false, true>(lds[0][0], lds[0][1], 0, nk, t);
+    Stage64<D, false, true> st(kp, p.k_row, vp, p.v_row, t);
+    st.load(0, nk);
+    st.store(lds[0][0], lds[0][1], 0, nk);
     __syncthreads();
     for (int k0 = 0, buf = 0; k0 < most; k0 += 64, buf ^= 1) {
       const bool more = k0 + 64 < most;
-      if (more) st.load(kp, p.k_row, vp, p.v_row, k0 + 64, nk, t);
+      if (more) st.load(k0 + 64, nk);
       const char *kt = lds[buf][0], *vt = lds[buf][1];
       if (k0 < any) {
         f32x16 s[2];
@@ -395,44 +427,39 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) s[i] = MELGPT_MFMA_32x32x16(L::rows(kt, i, ks, lane), qf[ks], s[i]);
         if (k0 + 64 > full) {
+          const int lim = sees - k0 - 4 * hh;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[i][r] = k0 + 32 * i + 8 * (r >> 2) + 4 * hh + (r & 3) < sees ? s[i][r] * c2 : -__builtin_inff();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] *= c2;
+            for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? s[i][r] : -__builtin_inff();
         }
-        float top = s[0][0];
+        float top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+          for (int r = 0; r < 16; r += 2)   // (asm: fmaxf makes hipcc canonicalise every matrix result first)
+            asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(s[i][r]), "v"(s[i][r + 1]));
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
         // the running maximum follows only when it is passed by more than 2^8: until then terms up to 2^8 are exact enough in
         // f32 sums and 16-bit operands alike, and the 16 DB accumulators need no rescaling (rare after the first tiles)
         if (__any(top > m + 8.f)) {
           const float now = fmaxf(m, top), base = now == -__builtin_inff() ? 0.f : now;
           const float keep = __builtin_amdgcn_exp2f(m - base);
           m = now;
-          l *= keep;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l[i] *= keep;
 #pragma unroll
           for (int d = 0; d < L::DB; ++d) o[d] *= keep;
         }
         const float base = m == -__builtin_inff() ? 0.f : m;
-        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - base);
-            sum += s[i][r];
+            s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c2, -base));
+            l[r & 3] += s[i][r];
           }
         }
-        l += sum;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const u32x4 pf = operand16(s[e >> 1], e & 1);
@@ -440,20 +467,21 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
           for (int d = 0; d < L::DB; ++d) o[d] = MELGPT_MFMA_32x32x16(L::cols(vt, e, d, lane), pf, o[d]);
         }
       }
-      if (more) st.template store<false, true>(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 64, nk, t);
+      if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 64, nk);
       __syncthreads();
     }
-    l += __shfl_xor(l, 32, 64);
   }
+  float sum = (l[0] + l[1]) + (l[2] + l[3]);
+  sum += __shfl_xor(sum, 32, 64);
   if (!mine) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
 #pragma unroll
   for (int d = 0; d < L::DB; ++d)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       store4<T>(op + 32 * d + 8 * j + 4 * hh, f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv);
-  if (hh == 0) p.lse[h * p.Mq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+  if (hh == 0) p.lse[h * p.Mq + row] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
 // -------------------------------------------------------------------------------------------------------- backward
