@@ -14,6 +14,8 @@
 // Row tiles of a sequence: nobody knows the lengths on the host, so sequence s is allotted tiles floor(cu[s] / B) + s up to
 // floor(cu[s+1] / B) + s + 1 - never fewer than it needs, one too many at most - and a workgroup finds its sequence by a
 // 64-way search over the offsets.  The rows in front of the first and behind the last sequence are two sequences without keys.
+#include <type_traits>
+
 #include "mma.h"
 
 namespace {
@@ -311,59 +313,45 @@ __device__ __forceinline__ f32x16 zero16() {
   for (int i = 0; i < 16; ++i) z[i] = 0.f;
   return z;
 }
+// larger of a lane's value and that of the lane 32 away (NaN wins)
+__device__ __forceinline__ float halves_max(float v) {
+  const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 // accumulators 8 st .. 8 st + 7 of a 32-row block as the operand of a 16-row contraction
 __device__ __forceinline__ u32x4 operand16(const f32x16& s, int st) {
   return u32x4{pack_bf16x2(s[8 * st], s[8 * st + 1]), pack_bf16x2(s[8 * st + 2], s[8 * st + 3]),
                pack_bf16x2(s[8 * st + 4], s[8 * st + 5]), pack_bf16x2(s[8 * st + 6], s[8 * st + 7])};
 }
 
-// 64 rows of two tensors through registers into LDS (256 threads).  A thread's rows are 64 / PER apart and its addresses
-// one base and a uniform step: the 64-bit products of a row's address cost as much as the softmax when formed per row.
-template <int D, bool TA, bool TB>   // TA, TB: laid out for transposed reads
+// 64 rows through registers into LDS (256 threads), by buffer loads: the uniform parts of an address cost no vector
+// instruction (a row's 64-bit product per load cost as much as the softmax), and rows behind the last read as zeros (their
+// scores are masked, but 0 * NaN is not 0).
+template <int D, bool TR>   // TR: laid out for transposed reads
 struct Stage64 {
   using L = Tile32<D>;
   static constexpr int PER = 64 * L::CP / 256, STEP = 64 / PER;
-  const bf16_t *pa, *pb;
-  long long ra, rb;
-  int row, off_a, off_b;   // first row, its place in LDS (rows STEP apart keep the swizzle: STEP is a multiple of 16)
-  u32x4 a[PER], b[PER];
+  const bf16_t* base;
+  long long rs;        // row stride, D <= rs (rows do not overlap: the end of the last row bounds them all)
+  unsigned from;       // this thread's first chunk, bytes from a tile's first row
+  int off;             // its place in LDS (rows STEP apart keep the swizzle: STEP is a multiple of 16)
+  u32x4 a[PER];
   static_assert(STEP % 16 == 0, "rows of a thread share their swizzle");
-  __device__ __forceinline__ Stage64(const bf16_t* a0, long long ra_, const bf16_t* b0, long long rb_, int t) : ra(ra_), rb(rb_) {
-    const int c = t % L::CP;
-    row = t / L::CP;
-    pa = a0 + row * ra + c * 8;
-    pb = b0 + row * rb + c * 8;
-    off_a = TA ? L::off_t(row, c) : L::off_r(row, c);
-    off_b = TB ? L::off_t(row, c) : L::off_r(row, c);
+  __device__ __forceinline__ Stage64(const bf16_t* b, long long row_stride, int t) : base(b), rs(row_stride) {
+    const int c = t % L::CP, row = t / L::CP;
+    from = 2u * ((unsigned)row * (unsigned)rs + 8u * c);
+    off = TR ? L::off_t(row, c) : L::off_r(row, c);
   }
   __device__ __forceinline__ void load(int row0, int n) {
-    if (row0 + 64 <= n) {
+    const int left = min(max(n - row0, 0), 64);
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base + row0 * rs, left > 0 ? 2u * ((unsigned)(left - 1) * (unsigned)rs + D) : 0u);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        a[i] = *(const u32x4*)(pa + (row0 + STEP * i) * ra);
-        b[i] = *(const u32x4*)(pb + (row0 + STEP * i) * rb);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {   // rows behind the last are the last
-        const long long r = min(row0 + row + STEP * i, n - 1) - row;
-        a[i] = *(const u32x4*)(pa + r * ra);
-        b[i] = *(const u32x4*)(pb + r * rb);
-      }
-    }
+    for (int i = 0; i < PER; ++i)
+      a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, from, 2u * STEP * i * (unsigned)rs, 0));
   }
-  // rows behind the last are zero: their scores are masked, but 0 * NaN is not 0
-  __device__ __forceinline__ void store(char* ta, char* tb, int row0, int n) {
-    if (row0 + 64 > n) {
+  __device__ __forceinline__ void store(char* t) const {
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (row0 + row + STEP * i >= n) a[i] = b[i] = u32x4{0u, 0u, 0u, 0u};
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      *(u32x4*)(ta + off_a + i * STEP * L::RB) = a[i];
-      *(u32x4*)(tb + off_b + i * STEP * L::RB) = b[i];
-    }
+    for (int i = 0; i < PER; ++i) *(u32x4*)(t + off + i * STEP * L::RB) = a[i];
   }
 };
 
@@ -380,15 +368,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
   if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
-  const int w0 = 128 * R.tile + 32 * wave;                         // the wave's first query
-  const int q_in = w0 + (lane & 31);
-  const bool mine = q_in < R.n;
-  const long long row = R.lo + min(q_in, R.n - 1);
-  const int sees = min(max(q_in + nk - R.n + 1, 0), nk);
+  const int w0 = 128 * R.tile + 32 * wave;                     // the wave's first query
   const int last = min(128 * R.tile + 127, R.n - 1);
   const int most = min(max(last + nk - R.n + 1, 0), nk);
-  // keys that every query of the wave sees, and that any of them does
-  const int full = min(max(w0 + nk - R.n + 1, 0), nk), any = min(max(min(w0 + 31, R.n - 1) + nk - R.n + 1, 0), nk);
+  const int full = min(max(w0 + nk - R.n + 1, 0), nk);             // keys that every query of the wave sees
+  const int q_in = w0 + (lane & 31);
+  const int sees = min(max(q_in + nk - R.n + 1, 0), nk);           // keys 0 .. sees - 1
+  const long long row = R.lo + min(q_in, R.n - 1);
   const T* qp = (const T*)p.q + row * p.q_row + h * p.q_head;
   u32x4 qf[L::NKS];
 #pragma unroll
@@ -408,72 +394,110 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   f32x16 o[L::DB];
 #pragma unroll
   for (int d = 0; d < L::DB; ++d) o[d] = zero16();
-  float m = -__builtin_inff(), l[4] = {0.f, 0.f, 0.f, 0.f};        // four partial sums: independent chains
+  float m = -__builtin_inff(), l[2] = {0.f, 0.f};                  // two partial sums: independent chains
   if (most > 0) {
-    Stage64<D, false, true> st(kp, p.k_row, vp, p.v_row, t);
-    st.load(0, nk);
-    st.store(lds[0][0], lds[0][1], 0, nk);
-    __syncthreads();
-    for (int k0 = 0, buf = 0; k0 < most; k0 += 64, buf ^= 1) {
-      const bool more = k0 + 64 < most;
-      if (more) st.load(k0 + 64, nk);
-      const char *kt = lds[buf][0], *vt = lds[buf][1];
-      if (k0 < any) {
-        f32x16 s[2];
+    Stage64<D, false> ks_(kp, p.k_row, t);
+    Stage64<D, true> vs_(vp, p.v_row, t);
+    const int tiles = (most + 63) >> 6;
+    auto scores = [&](const char* kt, int half, f32x16& s) __attribute__((always_inline)) {
+      s = zero16();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = zero16();
+      for (int ks = 0; ks < L::NKS; ++ks) s = MELGPT_MFMA_32x32x16(L::rows(kt, half, ks, lane), qf[ks], s);
+    };
+    auto weigh = [&](const char* vt, int half, const u32x4 (&pp)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < L::NKS; ++ks)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) s[i] = MELGPT_MFMA_32x32x16(L::rows(kt, i, ks, lane), qf[ks], s[i]);
-        if (k0 + 64 > full) {
-          const int lim = sees - k0 - 4 * hh;
+        for (int d = 0; d < L::DB; ++d) o[d] = MELGPT_MFMA_32x32x16(L::cols(vt, 2 * half + e, d, lane), pp[e], o[d]);
+    };
+    // one step of 32 keys from k0: their scores `s` become probabilities `pn` under this step's matrix products, which are
+    // the next 32 keys' scores `sn` (from kt) and the previous 32 keys' probabilities `pp` times their values (from vt) -
+    // nothing here waits for anything else of the same step
+    auto step = [&](int k0, f32x16& s, f32x16& sn, const char* kt, int khalf, const u32x4 (&pp)[2], u32x4 (&pn)[2], const char* vt,
+                    int vhalf) __attribute__((always_inline)) {
+      if (k0 + 32 > full) {
+        const int lim = sees - k0 - 4 * hh;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? s[i][r] : -__builtin_inff();
-        }
-        float top = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; r += 2)   // (asm: fmaxf makes hipcc canonicalise every matrix result first)
-            asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(s[i][r]), "v"(s[i][r + 1]));
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
-        // the running maximum follows only when it is passed by more than 2^8: until then terms up to 2^8 are exact enough in
-        // f32 sums and 16-bit operands alike, and the 16 DB accumulators need no rescaling (rare after the first tiles)
-        if (__any(top > m + 8.f)) {
-          const float now = fmaxf(m, top), base = now == -__builtin_inff() ? 0.f : now;
-          const float keep = __builtin_amdgcn_exp2f(m - base);
-          m = now;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) l[i] *= keep;
-#pragma unroll
-          for (int d = 0; d < L::DB; ++d) o[d] *= keep;
-        }
-        const float base = m == -__builtin_inff() ? 0.f : m;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c2, -base));
-            l[r & 3] += s[i][r];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const u32x4 pf = operand16(s[e >> 1], e & 1);
-#pragma unroll
-          for (int d = 0; d < L::DB; ++d) o[d] = MELGPT_MFMA_32x32x16(L::cols(vt, e, d, lane), pf, o[d]);
-        }
+        for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < lim ? s[r] : -__builtin_inff();
       }
-      if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 64, nk);
+      scores(kt, khalf, sn);
+      weigh(vt, vhalf, pp);
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = __builtin_elementwise_maximum(top, s[r]);
+      top = halves_max(top) * c2;
+      // the running maximum follows only when it is passed by more than 2^8: until then terms up to 2^8 are exact enough in
+      // f32 sums and 16-bit operands alike, and the accumulators need no rescaling (rare after the first tiles)
+      const float now = top > m + 8.f ? top : m, base = now == -__builtin_inff() ? 0.f : now;
+      const bool moved = now != m;
+      const float keep = moved ? __builtin_amdgcn_exp2f(m - base) : 1.f;   // (no key yet: m is -inf and the sums are 0)
+      m = now;
+      l[0] *= keep;
+      l[1] *= keep;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -base));
+        l[r & 1] += s[r];
+      }
+      pn[0] = operand16(s, 0);
+      pn[1] = operand16(s, 1);
+      // (the exponentials belong under the products above: hipcc would sink them behind the branch)
+      asm volatile("" : "+v"(pn[0]), "+v"(pn[1]), "+v"(l[0]), "+v"(l[1]));
+      // order: fragments ahead, then a matrix instruction, a later fragment, and its share of the softmax; hipcc alone puts
+      // all of the softmax behind the products and waits for every fragment
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+      for (int j = 0; j < L::NKS; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+        if (j > 2) __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * L::DB; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+      }
+      if (__any(moved)) {
+#pragma unroll
+        for (int d = 0; d < L::DB; ++d) o[d] *= keep;
+      }
+    };
+    // K runs one tile ahead of V in LDS: [0] K, [1] V, two slots each, tile i in slot i & 1.  Iteration i's stores go to
+    // slots last read two steps ago, with the previous iteration's barrier in between.
+    ks_.load(0, nk);
+#pragma unroll
+    for (int i = 0; i < 64 * L::RB / (256 * 16); ++i) *(u32x4*)(lds[1][1] + (t + 256 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
+    ks_.store(lds[0][0]);
+    ks_.load(64, nk);
+    vs_.load(0, nk);
+    __syncthreads();
+    f32x16 s0, s1;
+    u32x4 p0[2], p1[2] = {u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}};
+    scores(lds[0][0], 0, s0);
+    auto tile = [&](int i, auto par) __attribute__((always_inline)) {   // par = i & 1, known to the compiler: LDS addresses are constants
+      constexpr int P = decltype(par)::value;
+      step(64 * i, s0, s1, lds[0][P], 1, p1, p0, lds[1][P ^ 1], 1);
+      ks_.store(lds[0][P ^ 1]);                                    // (behind the last tile: zeros, never used)
+      vs_.store(lds[1][P]);
       __syncthreads();
+      ks_.load(64 * i + 128, nk);
+      vs_.load(64 * i + 64, nk);
+      step(64 * i + 32, s1, s0, lds[0][P ^ 1], 0, p0, p1, lds[1][P], 0);
+    };
+    int i = 0;
+    for (; i + 1 < tiles; i += 2) {
+      tile(i, std::integral_constant<int, 0>());
+      tile(i + 1, std::integral_constant<int, 1>());
     }
+    if (i < tiles) tile(i, std::integral_constant<int, 0>());
+    weigh(lds[1][(tiles - 1) & 1], 1, p1);
   }
-  float sum = (l[0] + l[1]) + (l[2] + l[3]);
+  float sum = l[0] + l[1];
   sum += __shfl_xor(sum, 32, 64);
-  if (!mine) return;
+  if (q_in >= R.n) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
 #pragma unroll
@@ -680,6 +704,10 @@ int check(const PackedParams& p, int D, int dtype) {
   const int vec = dtype == MELGPT_F32 ? 4 : 8;
   if (p.Mq > 0 && (!p.q || !p.o || !p.lse)) return MELGPT_ERR_BAD_ARG;
   if (p.Mk > 0 && (!p.k || !p.v)) return MELGPT_ERR_BAD_ARG;
+  // rows do not overlap, and 64 of them lie within 4 GB of each other (the kernels' buffer loads)
+  if ((p.Mk > 1 && (p.k_row < D || p.v_row < D)) || (p.Mq > 1 && p.q_row < D) || p.k_row > (1 << 24) || p.v_row > (1 << 24) ||
+      p.q_row > (1 << 24))
+    return MELGPT_ERR_UNSUPPORTED;
   if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.o)) return MELGPT_ERR_ALIGN;
   if (p.q_row % vec || p.q_head % vec || p.k_row % vec || p.k_head % vec || p.v_row % vec || p.v_head % vec || p.o_row % vec ||
       p.o_head % vec)
@@ -689,7 +717,8 @@ int check(const PackedParams& p, int D, int dtype) {
 
 template <typename T, int D>
 int launch_fwd(const PackedParams& p, hipStream_t s) {
-  const long long tiles = tiles_for(p.Mq, p.S, sizeof(T) == 2 ? 128 : 64);
+  const int bm = sizeof(T) == 2 ? 128 : 64;
+  const long long tiles = tiles_for(p.Mq, p.S, bm);
   if (tiles > 65535) return MELGPT_ERR_UNSUPPORTED;
   if constexpr (sizeof(T) == 2)
     hipLaunchKernelGGL((packed_fwd32_kernel<D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
@@ -745,6 +774,7 @@ extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long 
   if (e) return e;
   if (Mq > 0 && (!dout || !delta || !dq)) return MELGPT_ERR_BAD_ARG;
   if (Mk > 0 && (!dk || !dv)) return MELGPT_ERR_BAD_ARG;
+  if ((Mq > 1 && do_row < D) || do_row > (1 << 24)) return MELGPT_ERR_UNSUPPORTED;
   const int vec = dtype == MELGPT_F32 ? 4 : 8;
   if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_row % vec || do_head % vec || dq_row % vec ||
       dq_head % vec || dk_row % vec || dk_head % vec || dv_row % vec || dv_head % vec)
