@@ -296,6 +296,9 @@ struct Tile32 {
   static __device__ __forceinline__ u32x4 rows(const char* t, int blk, int ks, int lane) {
     return *(const u32x4*)(t + off_r(32 * blk + (lane & 31), 2 * ks + (lane >> 5)));
   }
+  static __device__ __forceinline__ u32x4 rows_t(const char* t, int blk, int ks, int lane) {   // of a tile laid out for transposed reads
+    return *(const u32x4*)(t + off_t(32 * blk + (lane & 31), 2 * ks + (lane >> 5)));
+  }
   // 32 columns of block db, contraction over 16 rows, step st: slot j of lane half hh is row 16 st + 8 (j >> 2) + 4 hh + (j & 3),
   // the order in which accumulators 8 (st & 1) .. + 7 of a 32-row score block hold them
   static __device__ __forceinline__ u32x4 cols(const char* t, int st, int db, int lane) {
@@ -693,6 +696,262 @@ __global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
   }
 }
 
+// ------------------------------------------------------------------------------------ backward, 16-bit operands
+// dq and delta: a wave owns 32 queries, 64 keys a step; K lies in LDS in the order its transposed reads want (its row reads
+// meet no bank twice in that order either)
+template <int D>
+__global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
+  using L = Tile32<D>;
+  using T = bf16_t;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * L::RB];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
+  int h;
+  head_of(blockIdx.x, p, h);
+  const Rows R = find_rows<128>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  if (!R.any) return;
+  int k_lo, nk;
+  other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
+  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
+  const int w0 = 128 * R.tile + 32 * wave, q_in = w0 + (lane & 31);
+  const int last = min(128 * R.tile + 127, R.n - 1);
+  const int most = min(max(last + nk - R.n + 1, 0), nk);
+  const int full = min(max(w0 + nk - R.n + 1, 0), nk), any = min(max(min(w0 + 31, R.n - 1) + nk - R.n + 1, 0), nk);
+  const int sees = min(max(q_in + nk - R.n + 1, 0), nk);
+  const long long row = R.lo + min(q_in, R.n - 1);
+  const T* qp = (const T*)p.q + row * p.q_row + h * p.q_head;
+  const T* gp = (const T*)p.dout + row * p.do_row + h * p.do_head;
+  const T* op = (const T*)p.o + row * p.o_row + h * p.o_head;
+  u32x4 qf[L::NKS], gf[L::NKS];
+  float dl = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) {
+    qf[ks] = *(const u32x4*)(qp + 16 * ks + 8 * hh);
+    gf[ks] = *(const u32x4*)(gp + 16 * ks + 8 * hh);
+    const u32x4 of = *(const u32x4*)(op + 16 * ks + 8 * hh);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dl = fmaf(half_lo(gf[ks][e]), half_lo(of[e]), dl);
+      dl = fmaf(half_hi(gf[ks][e]), half_hi(of[e]), dl);
+    }
+  }
+  dl += __shfl_xor(dl, 32, 64);
+  if (q_in < R.n && hh == 0) p.delta[h * p.Mq + row] = dl;
+  const float lse2 = p.lse[h * p.Mq + row] * LOG2E, c2 = p.scale * LOG2E;
+  const T* kp = (const T*)p.k + (long long)k_lo * p.k_row + (h / p.G) * p.k_head;
+  const T* vp = (const T*)p.v + (long long)k_lo * p.v_row + (h / p.G) * p.v_head;
+  f32x16 dq[L::DB];
+#pragma unroll
+  for (int d = 0; d < L::DB; ++d) dq[d] = zero16();
+  if (most > 0) {
+    Stage64<D, true> ks_(kp, p.k_row, t), vs_(vp, p.v_row, t);
+    ks_.load(0, nk);
+    vs_.load(0, nk);
+    ks_.store(lds[0][0]);
+    vs_.store(lds[0][1]);
+    __syncthreads();
+    auto half = [&](int k0, const char* kt, const char* vt, int i) __attribute__((always_inline)) {
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks) {
+        s = MELGPT_MFMA_32x32x16(L::rows_t(kt, i, ks, lane), qf[ks], s);
+        dp = MELGPT_MFMA_32x32x16(L::rows_t(vt, i, ks, lane), gf[ks], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2)) * (dp[r] - dl);
+      if (k0 + 32 * i + 32 > full) {
+        const int lim = sees - k0 - 32 * i - 4 * hh;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < lim ? s[r] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const u32x4 sf = operand16(s, e);
+#pragma unroll
+        for (int d = 0; d < L::DB; ++d) dq[d] = MELGPT_MFMA_32x32x16(L::cols(kt, 2 * i + e, d, lane), sf, dq[d]);
+      }
+    };
+    auto tile = [&](int k0, auto par) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      const bool more = k0 + 64 < most;
+      if (more) {
+        ks_.load(k0 + 64, nk);
+        vs_.load(k0 + 64, nk);
+      }
+      if (k0 < any) {
+        half(k0, lds[P][0], lds[P][1], 0);
+        half(k0, lds[P][0], lds[P][1], 1);
+      }
+      if (more) {
+        ks_.store(lds[P ^ 1][0]);
+        vs_.store(lds[P ^ 1][1]);
+      }
+      __syncthreads();
+    };
+    for (int k0 = 0; k0 < most; k0 += 128) {
+      tile(k0, std::integral_constant<int, 0>());
+      if (k0 + 64 < most) tile(k0 + 64, std::integral_constant<int, 1>());
+    }
+  }
+  if (q_in >= R.n) return;
+  T* out = (T*)p.dq + row * p.dq_row + h * p.dq_head;
+#pragma unroll
+  for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      store4<T>(out + 32 * d + 8 * j + 4 * hh, f32x4{dq[d][4 * j], dq[d][4 * j + 1], dq[d][4 * j + 2], dq[d][4 * j + 3]} * p.scale);
+}
+
+// dk and dv: 64 keys of one key head; wave (kb, qh) owns keys 32 kb .. + 31, in registers, and of each 64 queries that see
+// them, of each of the G heads, the 32 of half qh; the two halves are added at the end, in LDS.
+template <int D>
+__global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
+  using L = Tile32<D>;
+  using T = bf16_t;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * L::RB];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][64];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
+  const int kb = wave & 1, qh = wave >> 1;
+  const int hk = blockIdx.x;
+  const Rows R = find_rows<64>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
+  if (!R.any) return;
+  int q_lo, nq;
+  other_rows(p.cu_q, p.S, p.Mq, R.seq, q_lo, nq);
+  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
+  const int nk = R.n, w0 = 64 * R.tile + 32 * kb;
+  const int k_in = w0 + (lane & 31);
+  const long long row = R.lo + min(k_in, nk - 1);
+  // query i sees key j <= i + nk - nq: the queries from j - (nk - nq) on; all of the wave's keys from `full` on
+  const int from = max(k_in - (nk - nq), 0), full = max(w0 + 31 - (nk - nq), 0), least = max(w0 - (nk - nq), 0);
+  const int first = max(64 * R.tile - (nk - nq), 0) & ~63;
+  const T* kp = (const T*)p.k + row * p.k_row + hk * p.k_head;
+  const T* vp = (const T*)p.v + row * p.v_row + hk * p.v_head;
+  u32x4 kf[L::NKS], vf[L::NKS];
+#pragma unroll
+  for (int ks = 0; ks < L::NKS; ++ks) {
+    kf[ks] = *(const u32x4*)(kp + 16 * ks + 8 * hh);
+    vf[ks] = *(const u32x4*)(vp + 16 * ks + 8 * hh);
+  }
+  const float c2 = p.scale * LOG2E;
+  f32x16 dk[L::DB], dv[L::DB];
+#pragma unroll
+  for (int d = 0; d < L::DB; ++d) {
+    dk[d] = zero16();
+    dv[d] = zero16();
+  }
+  const int blocks = first < nq ? (nq - first + 63) / 64 : 0, total = blocks * p.G;
+  if (total > 0) {
+    Stage64<D, true> qs_((const T*)p.q, p.q_row, t), gs_((const T*)p.dout, p.do_row, t);
+    float sv = 0.f;
+    int lh = hk * p.G, lq = first;                                 // head and first query of the tile to load next
+    auto load = [&]() __attribute__((always_inline)) {
+      qs_.base = (const T*)p.q + (long long)q_lo * p.q_row + lh * p.q_head;
+      gs_.base = (const T*)p.dout + (long long)q_lo * p.do_row + lh * p.do_head;
+      qs_.load(lq, nq);
+      gs_.load(lq, nq);
+      if (t < 128) {
+        const long long r = lh * p.Mq + q_lo + min(lq + (t & 63), nq - 1);
+        sv = t < 64 ? p.lse[r] * LOG2E : p.delta[r];
+      }
+      lq += 64;
+      if (lq >= nq) {
+        lq = first;
+        ++lh;
+      }
+    };
+    auto store = [&](int buf) __attribute__((always_inline)) {
+      qs_.store(lds[buf][0]);
+      gs_.store(lds[buf][1]);
+      if (t < 128) stat[buf][t >> 6][t & 63] = sv;
+    };
+    auto block = [&](int q0, auto par) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      const char *qt = lds[P][0], *gt = lds[P][1];
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks) {
+        s = MELGPT_MFMA_32x32x16(L::rows_t(qt, qh, ks, lane), kf[ks], s);
+        dp = MELGPT_MFMA_32x32x16(L::rows_t(gt, qh, ks, lane), vf[ks], dp);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                                // accumulators 4 j .. + 3: queries 8 j + 4 hh .. + 3
+        const f32x4 ls = *(const f32x4*)&stat[P][0][32 * qh + 8 * j + 4 * hh];
+        const f32x4 de = *(const f32x4*)&stat[P][1][32 * qh + 8 * j + 4 * hh];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[4 * j + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + r], c2, -ls[r]));
+          dp[4 * j + r] = s[4 * j + r] * (dp[4 * j + r] - de[r]);
+        }
+      }
+      if (q0 < full || q0 + 32 > nq) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int q = q0 + 8 * (r >> 2) + 4 * hh + (r & 3);
+          const bool in = q >= from && q < nq;
+          s[r] = in ? s[r] : 0.f;
+          dp[r] = in ? dp[r] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const u32x4 pf = operand16(s, e), sf = operand16(dp, e);
+#pragma unroll
+        for (int d = 0; d < L::DB; ++d) {
+          dv[d] = MELGPT_MFMA_32x32x16(L::cols(gt, 2 * qh + e, d, lane), pf, dv[d]);
+          dk[d] = MELGPT_MFMA_32x32x16(L::cols(qt, 2 * qh + e, d, lane), sf, dk[d]);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < L::DB; ++d) asm volatile("" : "+a"(dk[d]), "+a"(dv[d]));   // (only matrix instructions touch them in the loop)
+    };
+    load();
+    store(0);
+    __syncthreads();
+    int q0 = first, n = 0;
+    auto tile = [&](auto par) __attribute__((always_inline)) {
+      if (n + 1 < total) load();
+      const int mine = q0 + 32 * qh;                               // this wave's 32 queries
+      if (mine + 31 >= least && mine < nq) block(mine, par);
+      q0 += 64;
+      if (q0 >= nq) q0 = first;
+      if (++n < total) store(decltype(par)::value ^ 1);
+      __syncthreads();
+    };
+    while (n < total) {
+      tile(std::integral_constant<int, 0>());
+      if (n < total) tile(std::integral_constant<int, 1>());
+    }
+  }
+  // the halves: wave (kb, 1) hands over dk, then dv, through LDS (32 keys x D f32 each: the tiles' room)
+  T* ok = (T*)p.dk + row * p.dk_row + hk * p.dk_head;
+  T* ov = (T*)p.dv + row * p.dv_row + hk * p.dv_head;
+  float* room = (float*)&lds[0][0][0] + kb * (32 * D);
+  auto join = [&](f32x16 (&a)[L::DB], T* out, float f) __attribute__((always_inline)) {
+    if (qh == 1) {
+#pragma unroll
+      for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) room[(16 * d + r) * 64 + lane] = a[d][r];
+    }
+    __syncthreads();
+    if (qh == 0) {
+#pragma unroll
+      for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) a[d][r] = (a[d][r] + room[(16 * d + r) * 64 + lane]) * f;
+      if (k_in < nk) {
+#pragma unroll
+        for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            store4<T>(out + 32 * d + 8 * j + 4 * hh, f32x4{a[d][4 * j], a[d][4 * j + 1], a[d][4 * j + 2], a[d][4 * j + 3]});
+      }
+    }
+    __syncthreads();
+  };
+  join(dk, ok, p.scale);
+  join(dv, ov, 1.f);
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int check(const PackedParams& p, int D, int dtype) {
@@ -729,10 +988,16 @@ int launch_fwd(const PackedParams& p, hipStream_t s) {
 
 template <typename T, int D>
 int launch_bwd(const PackedParams& p, hipStream_t s) {
-  const long long tq = tiles_for(p.Mq, p.S, 64), tk = tiles_for(p.Mk, p.S, 64);
+  const long long tq = tiles_for(p.Mq, p.S, sizeof(T) == 2 ? 128 : 64), tk = tiles_for(p.Mk, p.S, 64);
   if (tq > 65535 || tk > 65535) return MELGPT_ERR_UNSUPPORTED;
-  if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_kernel<T, D>), dim3(p.Hq, (unsigned)tq), dim3(256), 0, s, p);
-  if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_kernel<T, D>), dim3(p.Hk, (unsigned)tk), dim3(256), 0, s, p);
+  const dim3 gq(p.Hq, (unsigned)tq), gk(p.Hk, (unsigned)tk);
+  if constexpr (sizeof(T) == 2) {
+    if (p.Mq > 0) hipLaunchKernelGGL((packed_dq32_kernel<D>), gq, dim3(256), 0, s, p);
+    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv32_kernel<D>), gk, dim3(256), 0, s, p);
+  } else {
+    if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_kernel<T, D>), gq, dim3(256), 0, s, p);
+    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_kernel<T, D>), gk, dim3(256), 0, s, p);
+  }
   return melgpt_launch_status();
 }
 
