@@ -53,9 +53,9 @@ struct Rows {
   int tile, tiles;
   bool any;
 };
-// tile number t (of rows of `B`) -> its range and the tile within it, the last tile of a range first (the causal tiles
-// with the most keys start first)
-template <int B>
+// tile number t (of rows of `B`) -> its range and the tile within it; with LAST the last tile of a range comes first: the
+// tiles with the most causal partners (queries: the last, keys: the first) start first
+template <int B, bool LAST>
 __device__ __forceinline__ Rows find_rows(const int* cu, int S, long long M, int t, int lane) {
   // the largest range i of 0 .. S + 1 with bound(i) / B + i <= t, 64 candidates at a time (the lanes of every wave)
   int lo = 0, n = S + 2;
@@ -77,7 +77,7 @@ __device__ __forceinline__ Rows find_rows(const int* cu, int S, long long M, int
   r.tiles = (r.n + B - 1) / B;
   const int at = t - (a / B + lo);
   r.any = at >= 0 && at < r.tiles;
-  r.tile = r.tiles - 1 - at;
+  r.tile = LAST ? r.tiles - 1 - at : at;
   return r;
 }
 // rows of the other side of sequence seq
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
   int h;
   head_of(blockIdx.x, p, h);
-  const Rows R = find_rows<64>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  const Rows R = find_rows<64, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
@@ -345,16 +345,22 @@ struct Stage64 {
     from = 2u * ((unsigned)row * (unsigned)rs + 8u * c);
     off = TR ? L::off_t(row, c) : L::off_r(row, c);
   }
-  __device__ __forceinline__ void load(int row0, int n) {
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int row0, int n) const {
     const int left = min(max(n - row0, 0), 64);
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(base + row0 * rs, left > 0 ? 2u * ((unsigned)(left - 1) * (unsigned)rs + D) : 0u);
+    return make_rsrc(base + row0 * rs, left > 0 ? 2u * ((unsigned)(left - 1) * (unsigned)rs + D) : 0u);
+  }
+  __device__ __forceinline__ void load1(__amdgpu_buffer_rsrc_t r, int i) {
+    a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, from, 2u * STEP * i * (unsigned)rs, 0));
+  }
+  __device__ __forceinline__ void store1(char* t, int i) const { *(u32x4*)(t + off + i * STEP * L::RB) = a[i]; }
+  __device__ __forceinline__ void load(int row0, int n) {
+    const __amdgpu_buffer_rsrc_t r = at(row0, n);
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, from, 2u * STEP * i * (unsigned)rs, 0));
+    for (int i = 0; i < PER; ++i) load1(r, i);
   }
   __device__ __forceinline__ void store(char* t) const {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) *(u32x4*)(t + off + i * STEP * L::RB) = a[i];
+    for (int i = 0; i < PER; ++i) store1(t, i);
   }
 };
 
@@ -366,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
   int h;
   head_of(blockIdx.x, p, h);
-  const Rows R = find_rows<128>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
@@ -520,7 +526,7 @@ __global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
   int h;
   head_of(blockIdx.x, p, h);
-  const Rows R = find_rows<64>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  const Rows R = find_rows<64, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
@@ -607,7 +613,7 @@ __global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
   __shared__ float stat[2][2][32];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
   const int hk = blockIdx.x;
-  const Rows R = find_rows<64>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
+  const Rows R = find_rows<64, false>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
   if (!R.any) return;
   int q_lo, nq;
   other_rows(p.cu_q, p.S, p.Mq, R.seq, q_lo, nq);
@@ -707,7 +713,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
   int h;
   head_of(blockIdx.x, p, h);
-  const Rows R = find_rows<128>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
+  const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
@@ -802,17 +808,22 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
 }
 
 // dk and dv: 64 keys of one key head; wave (kb, qh) owns keys 32 kb .. + 31, in registers, and of each 64 queries that see
-// them, of each of the G heads, the 32 of half qh; the two halves are added at the end, in LDS.
+// them, of each of the G heads, the 32 of half qh; the two halves are added at the end, in LDS.  One wave per SIMD: the
+// keys, the values and both gradients fill half of its 512 registers (the accumulators and operands that only matrix
+// instructions touch are kept in the other half of the file), and what hides its latencies is its own next block: a step
+// forms the next block's products with k and v and adds the previous block's gradients while this block's probabilities
+// are computed.  Four blocks of queries lie in LDS: previous, this, next, and the one being stored.
 template <int D>
 __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
   using L = Tile32<D>;
   using T = bf16_t;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * L::RB];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][64];
+  constexpr int TB = 64 * L::RB;                                   // bytes of a tile: slot i: q at 2 i TB, dout behind it
+  __shared__ __attribute__((aligned(16))) char tiles_[8 * TB];
+  __shared__ __attribute__((aligned(16))) float stat[4 * 128];     // [slot][lse, delta][64]
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
   const int kb = wave & 1, qh = wave >> 1;
   const int hk = blockIdx.x;
-  const Rows R = find_rows<64>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
+  const Rows R = find_rows<64, false>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
   if (!R.any) return;
   int q_lo, nq;
   other_rows(p.cu_q, p.S, p.Mq, R.seq, q_lo, nq);
@@ -821,17 +832,21 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
   const int k_in = w0 + (lane & 31);
   const long long row = R.lo + min(k_in, nk - 1);
   // query i sees key j <= i + nk - nq: the queries from j - (nk - nq) on; all of the wave's keys from `full` on
-  const int from = max(k_in - (nk - nq), 0), full = max(w0 + 31 - (nk - nq), 0), least = max(w0 - (nk - nq), 0);
+  const int from = max(k_in - (nk - nq), 0), full = max(w0 + 31 - (nk - nq), 0);
   const int first = max(64 * R.tile - (nk - nq), 0) & ~63;
   const T* kp = (const T*)p.k + row * p.k_row + hk * p.k_head;
   const T* vp = (const T*)p.v + row * p.v_row + hk * p.v_head;
   u32x4 kf[L::NKS], vf[L::NKS];
+  // masked scores are -inf before the scale: its sign goes into the keys, a zero scale makes them zero (as in the forward)
+  const unsigned flip = p.scale < 0.f ? 0x80008000u : 0u, keep = p.scale == 0.f ? 0u : 0xffffffffu;
 #pragma unroll
   for (int ks = 0; ks < L::NKS; ++ks) {
     kf[ks] = *(const u32x4*)(kp + 16 * ks + 8 * hh);
     vf[ks] = *(const u32x4*)(vp + 16 * ks + 8 * hh);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) kf[ks][e] = (kf[ks][e] ^ flip) & keep;
   }
-  const float c2 = p.scale * LOG2E;
+  const float c2 = p.scale == 0.f ? 1.f : fabsf(p.scale) * LOG2E;
   f32x16 dk[L::DB], dv[L::DB];
 #pragma unroll
   for (int d = 0; d < L::DB; ++d) {
@@ -842,89 +857,168 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
   if (total > 0) {
     Stage64<D, true> qs_((const T*)p.q, p.q_row, t), gs_((const T*)p.dout, p.do_row, t);
     float sv = 0.f;
-    int lh = hk * p.G, lq = first;                                 // head and first query of the tile to load next
-    auto load = [&]() __attribute__((always_inline)) {
+    // head by head, the queries from the last down
+    const int top = first + 64 * (blocks - 1);
+    int lh = hk * p.G, lq = top, left = total;                     // head and first query of the tile to load next, tiles left
+    auto aim = [&]() __attribute__((always_inline)) {              // at the tile to load next (none left: at nothing, zeros)
       qs_.base = (const T*)p.q + (long long)q_lo * p.q_row + lh * p.q_head;
       gs_.base = (const T*)p.dout + (long long)q_lo * p.do_row + lh * p.do_head;
-      qs_.load(lq, nq);
-      gs_.load(lq, nq);
-      if (t < 128) {
+    };
+    auto load_stat = [&]() __attribute__((always_inline)) {
+      if (t < 128 && left > 0) {
         const long long r = lh * p.Mq + q_lo + min(lq + (t & 63), nq - 1);
-        sv = t < 64 ? p.lse[r] * LOG2E : p.delta[r];
+        // a query that sees no key has lse -inf; +inf makes its probabilities 0 instead of NaN
+        const float x = t < 64 ? p.lse[r] * LOG2E : p.delta[r];
+        sv = t < 64 && x == -__builtin_inff() ? __builtin_inff() : x;
       }
-      lq += 64;
-      if (lq >= nq) {
-        lq = first;
-        ++lh;
+      lq -= 64;
+      if (lq < first) {
+        lq = top;
+        lh = min(lh + 1, hk * p.G + p.G - 1);
+      }
+      --left;
+    };
+    auto load = [&]() __attribute__((always_inline)) {
+      aim();
+      qs_.load(lq, left > 0 ? nq : 0);
+      gs_.load(lq, left > 0 ? nq : 0);
+      load_stat();
+    };
+    auto store = [&](int slot) __attribute__((always_inline)) {
+      qs_.store(tiles_ + 2 * slot * TB);
+      gs_.store(tiles_ + (2 * slot + 1) * TB);
+      if (t < 128) stat[128 * slot + t] = sv;
+    };
+    // The matrix instructions of a step, in order: the products of one block (2 NKS), the gradients of another (4 DB); with
+    // each, the fragment of tile rows or columns it takes
+    constexpr int NP = 2 * L::NKS, NM = NP + 4 * L::DB;
+    auto fragment = [&](int i, int prod, int grad) __attribute__((always_inline)) -> u32x4 {
+      if (i < NP) return L::rows_t(tiles_ + (2 * prod + (i & 1)) * TB, qh, i >> 1, lane);
+      const int j = i - NP;
+      return L::cols(tiles_ + (2 * grad + ((j & 1) ^ 1)) * TB, 2 * qh + j / (2 * L::DB), (j >> 1) % L::DB, lane);
+    };
+    auto multiply = [&](int i, const u32x4& f, f32x16& s, f32x16& dp, const u32x4 (&pf)[2], const u32x4 (&sf)[2]) __attribute__((always_inline)) {
+      if (i < NP) {
+        if (i & 1) dp = MELGPT_MFMA_32x32x16(f, vf[i >> 1], dp);
+        else s = MELGPT_MFMA_32x32x16(f, kf[i >> 1], s);
+      } else {
+        const int j = i - NP, e = j / (2 * L::DB), d = (j >> 1) % L::DB;
+        if (j & 1) dk[d] = MELGPT_MFMA_32x32x16(f, sf[e], dk[d]);
+        else dv[d] = MELGPT_MFMA_32x32x16(f, pf[e], dv[d]);
       }
     };
-    auto store = [&](int buf) __attribute__((always_inline)) {
-      qs_.store(lds[buf][0]);
-      gs_.store(lds[buf][1]);
-      if (t < 128) stat[buf][t >> 6][t & 63] = sv;
-    };
-    auto block = [&](int q0, auto par) __attribute__((always_inline)) {
-      constexpr int P = decltype(par)::value;
-      const char *qt = lds[P][0], *gt = lds[P][1];
-      f32x16 s = zero16(), dp = zero16();
+    u32x4 pf[2][2], sf[2][2];                                      // probabilities and ds of this and the previous block
 #pragma unroll
-      for (int ks = 0; ks < L::NKS; ++ks) {
-        s = MELGPT_MFMA_32x32x16(L::rows_t(qt, qh, ks, lane), kf[ks], s);
-        dp = MELGPT_MFMA_32x32x16(L::rows_t(gt, qh, ks, lane), vf[ks], dp);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {                                // accumulators 4 j .. + 3: queries 8 j + 4 hh .. + 3
-        const f32x4 ls = *(const f32x4*)&stat[P][0][32 * qh + 8 * j + 4 * hh];
-        const f32x4 de = *(const f32x4*)&stat[P][1][32 * qh + 8 * j + 4 * hh];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[4 * j + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + r], c2, -ls[r]));
-          dp[4 * j + r] = s[4 * j + r] * (dp[4 * j + r] - de[r]);
-        }
-      }
+    for (int i = 0; i < 2; ++i) pf[1][i] = sf[1][i] = u32x4{0u, 0u, 0u, 0u};
+    f32x16 s[2], dp[2];
+    int q0 = top + 32 * qh;                                        // this wave's queries of the current tile
+    auto step = [&](auto slot_) __attribute__((always_inline)) {
+      constexpr int SL = decltype(slot_)::value, A = SL & 1, B = A ^ 1;
       if (q0 < full || q0 + 32 > nq) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int q = q0 + 8 * (r >> 2) + 4 * hh + (r & 3);
           const bool in = q >= from && q < nq;
-          s[r] = in ? s[r] : 0.f;
-          dp[r] = in ? dp[r] : 0.f;
+          s[A][r] = in ? s[A][r] : -__builtin_inff();
+          dp[A][r] = in ? dp[A][r] : 0.f;
         }
       }
+      s[B] = zero16();
+      dp[B] = zero16();
+      f32x4 ls[4], de[4];                                          // accumulators 4 j .. + 3: queries 8 j + 4 hh .. + 3
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const u32x4 pf = operand16(s, e), sf = operand16(dp, e);
+      for (int j = 0; j < 4; ++j) {
+        ls[j] = *(const f32x4*)&stat[128 * SL + 32 * qh + 8 * j + 4 * hh];
+        de[j] = *(const f32x4*)&stat[128 * SL + 64 + 32 * qh + 8 * j + 4 * hh];
+      }
+      aim();
+      const __amdgpu_buffer_rsrc_t rq = qs_.at(lq, left > 0 ? nq : 0), rg = gs_.at(lq, left > 0 ? nq : 0);
+      // laid out by hand: hipcc on its own reads every fragment right in front of the product that waits for it.  With each
+      // matrix instruction go the read of the fragment five later, its share of the probabilities, and (in the last part) the
+      // stores of the tile loaded during the step before, each followed by the load that refills its registers
+      constexpr int AHEAD = 5, PER = Stage64<D, true>::PER;
+      u32x4 f[NM];
 #pragma unroll
-        for (int d = 0; d < L::DB; ++d) {
-          dv[d] = MELGPT_MFMA_32x32x16(L::cols(gt, 2 * qh + e, d, lane), pf, dv[d]);
-          dk[d] = MELGPT_MFMA_32x32x16(L::cols(qt, 2 * qh + e, d, lane), sf, dk[d]);
+      for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i, (SL + 1) & 3, (SL + 3) & 3);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        if (i + AHEAD < NM) f[i + AHEAD] = fragment(i + AHEAD, (SL + 1) & 3, (SL + 3) & 3);
+        multiply(i, f[i], s[B], dp[B], pf[B], sf[B]);
+#pragma unroll
+        for (int r = 16 * i / NM; r < 16 * (i + 1) / NM; ++r) {
+          s[A][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[A][r], c2, -ls[r >> 2][r & 3]));
+          dp[A][r] = s[A][r] * (dp[A][r] - de[r >> 2][r & 3]);
+          if ((r & 7) == 7) {
+            pf[A][r >> 3] = operand16(s[A], r >> 3);
+            sf[A][r >> 3] = operand16(dp[A], r >> 3);
+          }
         }
+        const int c = i - (NM - 2 * PER - 1);                      // (2 PER chunks in the last 2 PER places but one)
+        if (c >= 0 && c < 2 * PER) {
+          if (c & 1) {
+            gs_.store1(tiles_ + (2 * ((SL + 2) & 3) + 1) * TB, c >> 1);
+            gs_.load1(rg, c >> 1);
+          } else {
+            qs_.store1(tiles_ + 2 * ((SL + 2) & 3) * TB, c >> 1);
+            qs_.load1(rq, c >> 1);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int d = 0; d < L::DB; ++d) asm volatile("" : "+a"(dk[d]), "+a"(dv[d]));   // (only matrix instructions touch them in the loop)
-    };
-    load();
-    store(0);
-    __syncthreads();
-    int q0 = first, n = 0;
-    auto tile = [&](auto par) __attribute__((always_inline)) {
-      if (n + 1 < total) load();
-      const int mine = q0 + 32 * qh;                               // this wave's 32 queries
-      if (mine + 31 >= least && mine < nq) block(mine, par);
-      q0 += 64;
-      if (q0 >= nq) q0 = first;
-      if (++n < total) store(decltype(par)::value ^ 1);
+      for (int e = 0; e < 2; ++e) asm volatile("" : "+v"(pf[A][e]), "+v"(sf[A][e]));
+      // (only matrix instructions touch these in the loop: the half of the register file that is theirs)
+#pragma unroll
+      for (int d = 0; d < L::DB; ++d) asm volatile("" : "+a"(dk[d]), "+a"(dv[d]));
+#pragma unroll
+      for (int ks = 0; ks < L::NKS; ++ks) asm volatile("" : "+a"(kf[ks]), "+a"(vf[ks]));
+      if (t < 128) stat[128 * ((SL + 2) & 3) + t] = sv;
+      load_stat();
+      q0 -= 64;
+      if (q0 < first) q0 = top + 32 * qh;
       __syncthreads();
     };
-    while (n < total) {
-      tile(std::integral_constant<int, 0>());
-      if (n < total) tile(std::integral_constant<int, 1>());
+    // slot 3 stands for the block before the first: zeros (its probabilities are zero too, but 0 * NaN is not)
+#pragma unroll
+    for (int i = 0; i < 2 * TB / (256 * 16); ++i) *(u32x4*)(tiles_ + 6 * TB + (t + 256 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
+    load();
+    store(0);
+    load();
+    store(1);
+    load();
+    __syncthreads();
+    s[0] = zero16();
+    dp[0] = zero16();
+#pragma unroll
+    for (int i = 0; i < NP; ++i) multiply(i, fragment(i, 0, 0), s[0], dp[0], pf[1], sf[1]);
+    int n = 0;
+    for (; n + 4 <= total; n += 4) {
+      step(std::integral_constant<int, 0>());
+      step(std::integral_constant<int, 1>());
+      step(std::integral_constant<int, 2>());
+      step(std::integral_constant<int, 3>());
     }
+    if (n < total) step(std::integral_constant<int, 0>());
+    if (n + 1 < total) step(std::integral_constant<int, 1>());
+    if (n + 2 < total) step(std::integral_constant<int, 2>());
+    auto last = [&](auto slot_) __attribute__((always_inline)) {   // the last block's gradients
+      constexpr int SL = decltype(slot_)::value;
+#pragma unroll
+      for (int i = NP; i < NM; ++i) multiply(i, fragment(i, SL, SL), s[0], dp[0], pf[SL & 1], sf[SL & 1]);
+    };
+    switch ((total - 1) & 3) {
+      case 0: last(std::integral_constant<int, 0>()); break;
+      case 1: last(std::integral_constant<int, 1>()); break;
+      case 2: last(std::integral_constant<int, 2>()); break;
+      default: last(std::integral_constant<int, 3>());
+    }
+    __syncthreads();
   }
   // the halves: wave (kb, 1) hands over dk, then dv, through LDS (32 keys x D f32 each: the tiles' room)
   T* ok = (T*)p.dk + row * p.dk_row + hk * p.dk_head;
   T* ov = (T*)p.dv + row * p.dv_row + hk * p.dv_head;
-  float* room = (float*)&lds[0][0][0] + kb * (32 * D);
+  float* room = (float*)tiles_ + kb * (32 * D);
   auto join = [&](f32x16 (&a)[L::DB], T* out, float f) __attribute__((always_inline)) {
     if (qh == 1) {
 #pragma unroll
