@@ -967,49 +967,56 @@ def conv1d_out1(xp, w, bias, L, K, tanh=True):
 
 
 # --------------------------------------------------------------------------------- packed and cached sequences
-class _NoGuard:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *a):
-        return False
+# (these wrappers are the whole of a small call's time: plain checks, no context managers or keyword dicts on the way)
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-_NO_GUARD = _NoGuard()
-
-
-def _on(device):
-    """context in which the tensors' own device is the current one (its current stream is the one launched on)"""
-    if device.type != "cuda":
+def _device_of(x):
+    i = x.get_device()
+    if i < 0:
         raise _ffi.MelgptError("melgpt kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return i
 
 
-def _heads(x, what):
-    """(rows, heads, D) tensor -> the same or a copy with unit inner stride and 16-byte aligned rows and heads"""
-    assert x.dim() == 3, f"{what}: expected (rows, heads, head size), got {tuple(x.shape)}"
-    vec = 16 // x.element_size()
-    st = x.stride()
-    if st[2] != 1 or st[0] % vec or st[1] % vec or x.data_ptr() % 16:
+def _on(i, fn, *args, **kw):
+    """fn with the tensors' own device as the current one (its current stream is the one launched on)"""
+    with torch.cuda.device(i):
+        return fn(*args, **kw)
+
+
+def _same_device(i, *tensors):
+    for t_ in tensors:
+        assert t_ is None or t_.get_device() == i, f"a tensor is on {t_.device}, expected cuda:{i}"
+
+
+def _heads(x, vec):
+    """(rows, heads, D) tensor -> the same, or a copy where its rows or heads are not 16-byte aligned, its values not side by
+    side or its rows overlap; -> (tensor, row stride, head stride)"""
+    r, h, u = x.stride()
+    if u != 1 or r % vec or h % vec or (r < x.shape[2] and x.shape[0] > 1) or x.data_ptr() & 15:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        r, h, u = x.stride()
+    return x, r, h
 
 
-def _same_device(device, **tensors):
-    for name, t_ in tensors.items():
-        assert t_ is None or t_.device == device, f"{name} is on {t_.device}, expected {device}"
+def _addr(x):
+    return None if x is None else x.data_ptr()
 
 
-def _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, device):
+def _norm_rotary_args(i, M, D, positions, freqs, q_weight, k_weight):
     assert D % 16 == 0 and 16 <= D <= 256, f"head size {D}: a multiple of 16 up to 256"
-    rot = 2 * freqs.numel() if freqs is not None else 0
-    assert rot % 16 == 0 and rot <= D, f"{rot} rotated values of {D}: a multiple of 16 within the head"
-    assert positions.dtype == torch.int32 and positions.shape == (M,) and positions.is_contiguous()
-    assert freqs is None or (freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous())
+    rot = 0
+    if freqs is not None:
+        rot = 2 * freqs.shape[0]
+        assert freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous()
+        assert rot % 16 == 0 and rot <= D, f"{rot} rotated values of {D}: a multiple of 16 within the head"
+    assert positions.dtype == torch.int32 and positions.shape == (M,) and positions.is_contiguous(), "positions: (rows,) int32"
     assert (q_weight is None) == (k_weight is None), "the norm takes both weights or none"
-    for w in (q_weight, k_weight):
-        assert w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous())
-    _same_device(device, positions=positions, freqs=freqs, q_weight=q_weight, k_weight=k_weight)
+    if q_weight is not None:
+        assert q_weight.dtype == k_weight.dtype == torch.float32 and q_weight.shape == k_weight.shape == (D,)
+        assert q_weight.is_contiguous() and k_weight.is_contiguous()
+    _same_device(i, positions, freqs, q_weight, k_weight)
     return rot
 
 
@@ -1017,19 +1024,24 @@ def qk_norm_rotary_fwd(q, k, positions, freqs, *, q_weight=None, k_weight=None, 
     """RMS norm of every query and key head (skipped without weights) and the rotation of its first 2 * freqs.numel() values
     by positions * freqs (freqs None: no rotation), one launch.  q (M, Hq, D), k (M, Hk, D), any row and head strides;
     positions (M,) int32; freqs f64 radians per position; weights (D,) f32 -> (q', k') contiguous."""
+    i = _device_of(q)
+    if i != _current_device():
+        return _on(i, qk_norm_rotary_fwd, q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                   interleaved=interleaved, amplitude=amplitude)
     M, Hq, D = q.shape
     Hk = k.shape[1]
     assert k.shape == (M, Hk, D) and k.dtype == q.dtype and Hq > 0 and Hk > 0, (q.shape, k.shape, q.dtype, k.dtype)
     dt = dtype_code(q.dtype)
-    with _on(q.device):
-        _same_device(q.device, k=k)
-        rot = _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, q.device)
-        q, k = _heads(q, "q"), _heads(k, "k")
-        qo = torch.empty(M, Hq, D, dtype=q.dtype, device=q.device)
-        ko = torch.empty(M, Hk, D, dtype=q.dtype, device=q.device)
-        call("melgpt_qk_norm_rotary_fwd", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(positions),
-             ptr(freqs), rot, int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(qo), ptr(ko), M,
-             Hq, Hk, D, dt, stream())
+    rot = _norm_rotary_args(i, M, D, positions, freqs, q_weight, k_weight)
+    _same_device(i, k)
+    vec = 4 if dt == _ffi.F32 else 8
+    q, qr, qh = _heads(q, vec)
+    k, kr, kh = _heads(k, vec)
+    qo = torch.empty((M, Hq, D), dtype=q.dtype, device=q.device)
+    ko = torch.empty((M, Hk, D), dtype=q.dtype, device=q.device)
+    call("melgpt_qk_norm_rotary_fwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, positions.data_ptr(), _addr(freqs), rot,
+         interleaved, amplitude, _addr(q_weight), _addr(k_weight), eps, qo.data_ptr(), ko.data_ptr(), M, Hq, Hk, D, dt,
+         _raw_stream(i))
     return qo, ko
 
 
@@ -1037,39 +1049,49 @@ def qk_norm_rotary_bwd(dq_out, dk_out, q, k, positions, freqs, *, q_weight=None,
                        amplitude=1.0):
     """gradients of qk_norm_rotary_fwd: dq_out, dk_out like its outputs (any row and head strides), the other arguments its
     inputs -> (dq, dk, d q_weight, d k_weight), the last two f32 (D,) or None without weights."""
+    i = _device_of(q)
+    if i != _current_device():
+        return _on(i, qk_norm_rotary_bwd, dq_out, dk_out, q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                   interleaved=interleaved, amplitude=amplitude)
     M, Hq, D = q.shape
     Hk = k.shape[1]
     assert dq_out.shape == q.shape and dk_out.shape == k.shape == (M, Hk, D) and dq_out.dtype == dk_out.dtype == q.dtype == k.dtype
     dt = dtype_code(q.dtype)
-    with _on(q.device):
-        _same_device(q.device, k=k, dq_out=dq_out, dk_out=dk_out)
-        rot = _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, q.device)
-        q, k, dq_out, dk_out = _heads(q, "q"), _heads(k, "k"), _heads(dq_out, "dq_out"), _heads(dk_out, "dk_out")
-        dq = torch.empty(M, Hq, D, dtype=q.dtype, device=q.device)
-        dk = torch.empty(M, Hk, D, dtype=q.dtype, device=q.device)
-        part = dw = None
-        if q_weight is not None:
-            dw = torch.empty(2, D, dtype=torch.float32, device=q.device)
-            if M == 0:
-                zero_(dw)
-            n = _ffi.lib().melgpt_qk_norm_rotary_bwd_blocks(M)
-            part = torch.empty(n, 2, D, dtype=torch.float32, device=q.device)
-        call("melgpt_qk_norm_rotary_bwd", ptr(dq_out), dq_out.stride(0), dq_out.stride(1), ptr(dk_out), dk_out.stride(0),
-             dk_out.stride(1), ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(positions), ptr(freqs), rot,
-             int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(dq), ptr(dk), ptr(part), M, Hq, Hk,
-             D, dt, stream())
-        if dw is not None and M > 0:
-            call("melgpt_reduce_rows", ptr(part), n, 2 * D, 2 * D, ptr(dw), 0, 1.0, stream())
-    return dq, dk, (dw[0] if dw is not None else None), (dw[1] if dw is not None else None)
+    rot = _norm_rotary_args(i, M, D, positions, freqs, q_weight, k_weight)
+    _same_device(i, k, dq_out, dk_out)
+    vec = 4 if dt == _ffi.F32 else 8
+    q, qr, qh = _heads(q, vec)
+    k, kr, kh = _heads(k, vec)
+    dq_out, gqr, gqh = _heads(dq_out, vec)
+    dk_out, gkr, gkh = _heads(dk_out, vec)
+    dq = torch.empty((M, Hq, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((M, Hk, D), dtype=q.dtype, device=q.device)
+    part = dw = None
+    if q_weight is not None:
+        dw = torch.empty((2, D), dtype=torch.float32, device=q.device)
+        if M == 0:
+            zero_(dw)
+        n = _ffi.lib().melgpt_qk_norm_rotary_bwd_blocks(M)
+        part = torch.empty((n, 2, D), dtype=torch.float32, device=q.device)
+    st = _raw_stream(i)
+    call("melgpt_qk_norm_rotary_bwd", dq_out.data_ptr(), gqr, gqh, dk_out.data_ptr(), gkr, gkh, q.data_ptr(), qr, qh, k.data_ptr(),
+         kr, kh, positions.data_ptr(), _addr(freqs), rot, interleaved, amplitude, _addr(q_weight), _addr(k_weight), eps,
+         dq.data_ptr(), dk.data_ptr(), _addr(part), M, Hq, Hk, D, dt, st)
+    if dw is None:
+        return dq, dk, None, None
+    if M > 0:
+        call("melgpt_reduce_rows", part.data_ptr(), n, 2 * D, 2 * D, dw.data_ptr(), 0, 1.0, st)
+    return dq, dk, dw[0], dw[1]
 
 
-def _pages_of(k_pages, v_pages, page_table, dtype, device):
+def _pages_of(i, k_pages, v_pages, page_table, dtype):
     P, Hk, page, D = k_pages.shape
     assert v_pages.shape == k_pages.shape and k_pages.is_contiguous() and v_pages.is_contiguous()
     assert k_pages.dtype == v_pages.dtype == dtype, (k_pages.dtype, v_pages.dtype, dtype)
     assert page > 0 and page & (page - 1) == 0, f"page size {page}: a power of two"
-    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and (page_table.stride(1) == 1 or page_table.shape[1] == 1)
-    _same_device(device, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    assert page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table: (sequences, width) int32"
+    assert page_table.stride(1) == 1 or page_table.shape[1] <= 1
+    _same_device(i, k_pages, v_pages, page_table)
     return P, Hk, page, D
 
 
@@ -1081,60 +1103,59 @@ def kv_append(k, v, k_pages, v_pages, page_table, sequences, positions, *, q=Non
     size, D); page_table (S, width) int32; row r goes to sequence sequences[r], position positions[r] (both (M,) int32).
     A row of negative sequence or position is padding: nothing is stored, its row of a given q_out stays as it was (of a
     returned new one: zero).  A row that points outside the table or the pages is not stored.  Slots must be distinct."""
+    i = _device_of(k)
+    if i != _current_device():
+        return _on(i, kv_append, k, v, k_pages, v_pages, page_table, sequences, positions, q=q, freqs=freqs, q_weight=q_weight,
+                   k_weight=k_weight, eps=eps, interleaved=interleaved, amplitude=amplitude, q_out=q_out)
     M, Hk, D = k.shape
     assert v.shape == k.shape and v.dtype == k.dtype
     dt = dtype_code(k.dtype)
-    with _on(k.device):
-        P, Hkp, page, Dp = _pages_of(k_pages, v_pages, page_table, k.dtype, k.device)
-        assert (Hkp, Dp) == (Hk, D), (k_pages.shape, k.shape)
-        _same_device(k.device, v=v, q=q, q_out=q_out, sequences=sequences)
-        assert sequences.dtype == torch.int32 and sequences.shape == (M,) and sequences.is_contiguous()
-        if q is None:
-            assert q_weight is None and q_out is None
-            rot = _norm_rotary_args(M, D, positions, freqs, k_weight, k_weight, k.device)
-            Hq = 0
+    P, Hkp, page, Dp = _pages_of(i, k_pages, v_pages, page_table, k.dtype)
+    assert (Hkp, Dp) == (Hk, D), (k_pages.shape, k.shape)
+    assert sequences.dtype == torch.int32 and sequences.shape == (M,) and sequences.is_contiguous(), "sequences: (rows,) int32"
+    vec = 4 if dt == _ffi.F32 else 8
+    _same_device(i, v, q, q_out, sequences)
+    Hq = qr = qh = zero_pad = 0
+    if q is None:
+        assert q_weight is None and q_out is None
+        rot = _norm_rotary_args(i, M, D, positions, freqs, k_weight, k_weight)
+    else:
+        rot = _norm_rotary_args(i, M, D, positions, freqs, q_weight, k_weight)
+        Hq = q.shape[1]
+        assert q.shape == (M, Hq, D) and q.dtype == k.dtype and Hq > 0
+        if q_out is None:
+            zero_pad = 1
+            q_out = torch.empty((M, Hq, D), dtype=k.dtype, device=k.device)
         else:
-            rot = _norm_rotary_args(M, D, positions, freqs, q_weight, k_weight, k.device)
-            Hq = q.shape[1]
-            assert q.shape == (M, Hq, D) and q.dtype == k.dtype and Hq > 0
-            q = _heads(q, "q")
-        zero_pad = q is not None and q_out is None
-        if zero_pad:
-            q_out = torch.empty(M, Hq, D, dtype=k.dtype, device=k.device)
-        elif q is not None:
             assert q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous()
             assert q_out.data_ptr() != q.data_ptr(), "q_out is a buffer of its own"
-        k, v = _heads(k, "k"), _heads(v, "v")
-        if M == 0 or page_table.numel() == 0 or P == 0:
-            assert M == 0, "a cache without pages takes no rows"
-            return q_out
-        qs = q.stride() if q is not None else (0, 0)
-        call("melgpt_kv_append", ptr(q), qs[0], qs[1], ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1),
-             ptr(sequences), ptr(positions), ptr(page_table), page_table.stride(0), page_table.shape[0], page_table.shape[1],
-             ptr(freqs), rot, int(interleaved), float(amplitude), ptr(q_weight), ptr(k_weight), float(eps), ptr(q_out),
-             int(zero_pad), ptr(k_pages), ptr(v_pages), P, page, M, Hq, Hk, D, dt, stream())
+        q, qr, qh = _heads(q, vec)
+    if M == 0:
+        return q_out
+    assert P > 0 and page_table.numel() > 0, "a cache without pages takes no rows"
+    k, kr, kh = _heads(k, vec)
+    v, vr, vh = _heads(v, vec)
+    call("melgpt_kv_append", _addr(q), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, sequences.data_ptr(),
+         positions.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], _addr(freqs),
+         rot, interleaved, amplitude, _addr(q_weight), _addr(k_weight), eps, _addr(q_out), zero_pad, k_pages.data_ptr(),
+         v_pages.data_ptr(), P, page, M, Hq, Hk, D, dt, _raw_stream(i))
     return q_out
 
 
-def _offsets(cu, what, device):
-    assert cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 1 and cu.is_contiguous(), f"{what}: (sequences + 1,) int32"
-    _same_device(device, **{what: cu})
-    return cu.numel() - 1
-
-
-def _packed_args(q, k, v, cu_q, cu_k):
+def _packed_args(i, q, k, v, cu_q, cu_k):
     Mq, Hq, D = q.shape
     Mk, Hk, _ = k.shape
     assert k.shape == v.shape == (Mk, Hk, D) and q.dtype == k.dtype == v.dtype, (q.shape, k.shape, v.shape, q.dtype, k.dtype, v.dtype)
-    assert D in (64, 128), f"head size {D}: 64 or 128"
+    assert D == 64 or D == 128, f"head size {D}: 64 or 128"
     assert Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads over {Hk} key heads"
-    assert max(Mq, Mk) // 64 + cu_q.numel() + 1 <= 65535, "too many rows"
-    S = _offsets(cu_q, "cu_q", q.device)
     if cu_k is None:
         assert Mq == Mk, "queries and keys of different lengths need cu_k"
         cu_k = cu_q
-    assert _offsets(cu_k, "cu_k", q.device) == S, "cu_q and cu_k: one offset per sequence and the end"
-    _same_device(q.device, k=k, v=v)
+    S = cu_q.shape[0] - 1
+    for cu in (cu_q, cu_k):
+        assert cu.dtype == torch.int32 and cu.shape == (S + 1,) and S >= 0 and cu.is_contiguous(), "offsets: (sequences + 1,) int32"
+    assert max(Mq, Mk) // 64 + S + 2 <= 65535, "too many rows"
+    _same_device(i, k, v, cu_q, cu_k)
     return Mq, Mk, Hq, Hk, D, S, cu_k
 
 
@@ -1144,20 +1165,25 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None):
     cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
     -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  Rows behind the last sequence: left as they were in a given `out`, zero in a
     new one.  scale: 1 / sqrt(D) unless given."""
+    i = _device_of(q)
+    if i != _current_device():
+        return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out)
     dt = dtype_code(q.dtype)
-    with _on(q.device):
-        Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(q, k, v, cu_q, cu_k)
-        q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
-        gaps = out is None
-        if gaps:
-            out = torch.empty(Mq, Hq, D, dtype=q.dtype, device=q.device)
-        else:
-            assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
-            _same_device(q.device, out=out)
-        lse = torch.empty(Hq, Mq, dtype=torch.float32, device=q.device)
-        call("melgpt_packed_attn_fwd", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
-             v.stride(1), ptr(cu_q), ptr(cu_k), S, ptr(out), out.stride(0), out.stride(1), ptr(lse), int(gaps), Mq, Mk, Hq, Hk, D,
-             float(scale if scale is not None else D ** -0.5), dt, stream())
+    Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(i, q, k, v, cu_q, cu_k)
+    vec = 4 if dt == _ffi.F32 else 8
+    q, qr, qh = _heads(q, vec)
+    k, kr, kh = _heads(k, vec)
+    v, vr, vh = _heads(v, vec)
+    gaps = out is None
+    if gaps:
+        out = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        _same_device(i, out)
+    lse = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
+    call("melgpt_packed_attn_fwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
+         cu_k.data_ptr(), S, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), gaps, Mq, Mk, Hq, Hk, D,
+         D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
     return out, lse
 
 
@@ -1165,25 +1191,34 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
     """gradients of packed_attn_fwd from its inputs, both its results and dout (any row and head strides) -> (dq, dk, dv),
     contiguous and zero in rows that no sequence owns, unless `grads` gives the three tensors (any row and head strides,
     such rows left as they were)."""
+    i = _device_of(q)
+    if i != _current_device():
+        return _on(i, packed_attn_bwd, q, k, v, out, dout, lse, cu_q, cu_k, scale=scale, grads=grads)
     dt = dtype_code(q.dtype)
-    with _on(q.device):
-        Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(q, k, v, cu_q, cu_k)
-        assert out.shape == q.shape == dout.shape and out.dtype == dout.dtype == q.dtype and out.stride(2) == 1
-        assert lse.shape == (Hq, Mq) and lse.dtype == torch.float32 and lse.is_contiguous()
-        _same_device(q.device, out=out, dout=dout, lse=lse)
-        q, k, v, dout = _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(dout, "dout")
-        gaps = grads is None
-        if gaps:
-            grads = (torch.empty(Mq, Hq, D, dtype=q.dtype, device=q.device), torch.empty(Mk, Hk, D, dtype=q.dtype, device=q.device),
-                     torch.empty(Mk, Hk, D, dtype=q.dtype, device=q.device))
+    Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(i, q, k, v, cu_q, cu_k)
+    assert out.shape == q.shape == dout.shape and out.dtype == dout.dtype == q.dtype and out.stride(2) == 1
+    assert lse.shape == (Hq, Mq) and lse.dtype == torch.float32 and lse.is_contiguous()
+    _same_device(i, out, dout, lse)
+    vec = 4 if dt == _ffi.F32 else 8
+    q, qr, qh = _heads(q, vec)
+    k, kr, kh = _heads(k, vec)
+    v, vr, vh = _heads(v, vec)
+    out, our, ouh = _heads(out, vec)
+    dout, dor, doh = _heads(dout, vec)
+    gaps = grads is None
+    if gaps:
+        dq = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)
+        dk, dv = torch.empty((2, Mk, Hk, D), dtype=q.dtype, device=q.device).unbind(0)
+    else:
         dq, dk, dv = grads
         for g, x in ((dq, q), (dk, k), (dv, v)):
-            assert g.shape == x.shape and g.dtype == x.dtype and g.stride(2) == 1 and g.device == x.device
-        delta = torch.empty(Hq, Mq, dtype=torch.float32, device=q.device)
-        call("melgpt_packed_attn_bwd", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
-             v.stride(1), ptr(cu_q), ptr(cu_k), S, ptr(out), out.stride(0), out.stride(1), ptr(dout), dout.stride(0), dout.stride(1),
-             ptr(lse), ptr(delta), ptr(dq), dq.stride(0), dq.stride(1), ptr(dk), dk.stride(0), dk.stride(1), ptr(dv), dv.stride(0),
-             dv.stride(1), int(gaps), Mq, Mk, Hq, Hk, D, float(scale if scale is not None else D ** -0.5), dt, stream())
+            assert g.shape == x.shape and g.dtype == x.dtype and g.stride(2) == 1
+        _same_device(i, dq, dk, dv)
+    delta = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
+    call("melgpt_packed_attn_bwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
+         cu_k.data_ptr(), S, out.data_ptr(), our, ouh, dout.data_ptr(), dor, doh, lse.data_ptr(), delta.data_ptr(), dq.data_ptr(),
+         dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0), dv.stride(1), gaps, Mq,
+         Mk, Hq, Hk, D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
     return dq, dk, dv
 
 
@@ -1193,26 +1228,32 @@ def paged_attn_decode(q, k_pages, v_pages, page_table, lengths, *, scale=None, m
     has (those of kv_append's last row among them) -> (out (S, Hq, D), lse (S, Hq) f32).  A sequence without keys gives 0; a
     table entry outside the pages leaves its keys out.  max_length: the longest length, where the caller knows one shorter
     than the table's width (it only decides how far a sequence is split).  scale: 1 / sqrt(D) unless given."""
+    i = _device_of(q)
+    if i != _current_device():
+        return _on(i, paged_attn_decode, q, k_pages, v_pages, page_table, lengths, scale=scale, max_length=max_length, out=out)
     S, Hq, D = q.shape
     dt = dtype_code(q.dtype)
-    with _on(q.device):
-        P, Hk, page, Dp = _pages_of(k_pages, v_pages, page_table, q.dtype, q.device)
-        assert D == Dp and D in (64, 128), f"head size {D} (cache {Dp}): 64 or 128"
-        assert Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads over {Hk} key heads"
-        assert page_table.shape[0] == S and lengths.dtype == torch.int32 and lengths.shape == (S,) and lengths.is_contiguous()
-        _same_device(q.device, lengths=lengths, out=out)
-        q = _heads(q, "q")
-        if out is None:
-            out = torch.empty(S, Hq, D, dtype=q.dtype, device=q.device)
-        else:
-            assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
-        lse = torch.empty(S, Hq, dtype=torch.float32, device=q.device)
-        width = page_table.shape[1]
-        assert S == 0 or (width > 0 and P > 0), "a cache without pages"
-        bound = width * page if max_length is None else min(int(max_length), width * page)
-        splits = _ffi.lib().melgpt_paged_attn_splits(S, Hq, Hk, bound)
-        ws = torch.empty(S * Hq * splits * (D + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-        call("melgpt_paged_attn_decode", ptr(q), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages), P, page, ptr(page_table),
-             page_table.stride(0), width, ptr(lengths), S, ptr(out), out.stride(0), out.stride(1), ptr(lse), splits, ptr(ws), Hq, Hk,
-             D, float(scale if scale is not None else D ** -0.5), dt, stream())
+    P, Hk, page, Dp = _pages_of(i, k_pages, v_pages, page_table, q.dtype)
+    assert D == Dp and (D == 64 or D == 128), f"head size {D} (cache {Dp}): 64 or 128"
+    assert Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads over {Hk} key heads"
+    assert page_table.shape[0] == S and lengths.dtype == torch.int32 and lengths.shape == (S,) and lengths.is_contiguous()
+    _same_device(i, lengths, out)
+    q, qr, qh = _heads(q, 4 if dt == _ffi.F32 else 8)
+    if out is None:
+        out = torch.empty((S, Hq, D), dtype=q.dtype, device=q.device)
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+    lse = torch.empty((S, Hq), dtype=torch.float32, device=q.device)
+    if S == 0:
+        return out, lse
+    width = page_table.shape[1]
+    assert width > 0 and P > 0, "a cache without pages"
+    bound = width * page if max_length is None else min(int(max_length), width * page)
+    splits = _ffi.lib().melgpt_paged_attn_splits(S, Hq, Hk, bound)
+    ws = None
+    if splits > 1:   # (a buffer of the call's own: two captured graphs never share it)
+        ws = torch.empty(S * Hq * splits * (D + 2), dtype=torch.float32, device=q.device)
+    call("melgpt_paged_attn_decode", q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), P, page, page_table.data_ptr(),
+         page_table.stride(0), width, lengths.data_ptr(), S, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), splits,
+         _addr(ws), Hq, Hk, D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
     return out, lse

@@ -36,6 +36,10 @@ def rotary_freqs(rot, base=10000.0, *, stretch=1.0, base_stretch=1.0, ramp=None,
     return f.to(device)
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, freqs, eps, interleaved, amplitude):
@@ -56,6 +60,9 @@ class _QkNormRotaryFn(torch.autograd.Function):
 
 def qk_norm_rotary(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
     """ops.qk_norm_rotary_fwd with gradients for q, k and both weights."""
+    if not _wants_grad(q, k, q_weight, k_weight):
+        return ops.qk_norm_rotary_fwd(q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                                      amplitude=amplitude)
     return _QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, freqs, float(eps), bool(interleaved), float(amplitude))
 
 
@@ -76,4 +83,6 @@ class _PackedAttentionFn(torch.autograd.Function):
 
 def packed_attention(q, k, v, cu_q, cu_k=None, *, scale=None):
     """ops.packed_attn_fwd's output with gradients for q, k and v (those of a key head summed over its query heads)."""
+    if not _wants_grad(q, k, v):
+        return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale)[0]
     return _PackedAttentionFn.apply(q, k, v, cu_q, cu_k, scale)
