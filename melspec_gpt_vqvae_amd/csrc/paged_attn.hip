@@ -225,25 +225,37 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
   }
 }
 
-// joins the splits of one (sequence, query head): D / 4 lanes, four values each, in split order
+// joins the splits of one (sequence, query head): 256 / (D / 4) groups of lanes, four values a lane, take every
+// 256 / (D / 4)-th split each, then the groups' sums are added in order (one thread walking 86 splits took 25 us)
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, long long heads) {
-  constexpr int TPQ = D / 4;
-  const long long head = (long long)blockIdx.x * (256 / TPQ) + threadIdx.x / TPQ;
-  if (head >= heads) return;
-  const int d = 4 * (threadIdx.x % TPQ);
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
+  constexpr int TPQ = D / 4, NG = 256 / TPQ;
+  __shared__ __attribute__((aligned(16))) float sh[NG][D];
+  __shared__ float sums[NG];
+  const long long head = blockIdx.x;
+  const int g = threadIdx.x / TPQ, d = 4 * (threadIdx.x % TPQ), lane = threadIdx.x & 63;
   const float* st = p.part + p.stats + 2 * head * p.splits;
   const float* pp = p.part + head * p.splits * D + d;
   float top = -__builtin_inff();
-  for (int i = 0; i < p.splits; ++i) top = fmaxf(top, st[2 * i]);
+  for (int i = lane; i < p.splits; i += 64) top = fmaxf(top, st[2 * i]);
+  top = wave_max(top);
   const float base = top == -__builtin_inff() ? 0.f : top;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < p.splits; ++i) {
+  for (int i = g; i < p.splits; i += NG) {
     const float f = __builtin_amdgcn_exp2f(st[2 * i] - base);
     a += *(const f32x4*)(pp + (long long)i * D) * f;
     sum += st[2 * i + 1] * f;
+  }
+  *(f32x4*)&sh[g][d] = a;
+  if (d == 0) sums[g] = sum;
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int i = 1; i < NG; ++i) {
+    a += *(const f32x4*)&sh[i][d];
+    sum += sums[i];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)p.o + (head / p.Hq) * p.o_row + (head % p.Hq) * p.o_head + d;
@@ -257,10 +269,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <typename T, int D>
 int launch(const PagedParams& p, int S, hipStream_t s) {
   hipLaunchKernelGGL((paged_decode_kernel<T, D>), dim3((unsigned)(S * p.Hk), p.splits, (p.G + 15) / 16), dim3(256), 0, s, p);
-  if (p.splits > 1) {
-    const long long heads = (long long)S * p.Hq, per = 256 / (D / 4);
-    hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)((heads + per - 1) / per)), dim3(256), 0, s, p, heads);
-  }
+  if (p.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)(S * p.Hq)), dim3(256), 0, s, p);
   return melgpt_launch_status();
 }
 
@@ -287,7 +296,7 @@ extern "C" int melgpt_paged_attn_decode(const void* q, long long q_row, long lon
   if (!q || !k_pages || !v_pages || !page_table || !lengths || !out || !lse || (splits > 1 && !workspace)) return MELGPT_ERR_BAD_ARG;
   if (dtype != MELGPT_F32 && dtype != MELGPT_BF16) return MELGPT_ERR_UNSUPPORTED;
   if ((D != 64 && D != 128) || Hq % Hk || (page_size & (page_size - 1)) || page_size > (1 << 20) || n_pages > 0x7fffffffLL ||
-      splits > 65535 || (long long)S * Hk > 0xffffff || Hq / Hk > 1024)
+      splits > 65535 || (long long)S * Hq > 0xffffff || Hq / Hk > 1024)
     return MELGPT_ERR_UNSUPPORTED;
   const int vec = dtype == MELGPT_F32 ? 4 : 8;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(workspace) || q_row % vec ||
