@@ -580,15 +580,17 @@ int melgpt_kv_append(const void* q, long long q_row, long long q_head, const voi
  * with nq and nk of them query i sees keys j <= i + nk - nq, so a prompt's continuation lies at the end of its keys and
  * queries that see nothing give 0 (lse -inf).  out and its gradients have strides of their own.  lse, delta (Hq, Mq) f32:
  * the natural log of the scores' exponential sum; scratch that the backward fills with sum_d dout * out.
+ * out_low (16-bit lane, optional, (Mq, Hq, D) contiguous): what the rounding of out took away, written by the forward and,
+ * given to the backward, restored in its delta.
  * write_gaps: rows of the outputs that no sequence owns are zeroed (lse -inf), otherwise left as they were.
  * D 64 or 128; scale multiplies the scores; at most 4 M rows (65535 tiles of 64 with one more per sequence). */
 int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                            const void* v, long long v_row, long long v_head, const int* cu_q, const int* cu_k, int S, void* out,
-                           long long o_row, long long o_head, float* lse, int write_gaps, long long Mq, long long Mk, int Hq,
+                           long long o_row, long long o_head, void* out_low, float* lse, int write_gaps, long long Mq, long long Mk, int Hq,
                            int Hk, int D, float scale, int dtype, void* stream);
 int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                            const void* v, long long v_row, long long v_head, const int* cu_q, const int* cu_k, int S,
-                           const void* out, long long o_row, long long o_head, const void* dout, long long do_row,
+                           const void* out, long long o_row, long long o_head, const void* out_low, const void* dout, long long do_row,
                            long long do_head, const float* lse, float* delta, void* dq, long long dq_row, long long dq_head,
                            void* dk, long long dk_row, long long dk_head, void* dv, long long dv_row, long long dv_head,
                            int write_gaps, long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype,

@@ -27,6 +27,7 @@ struct PackedParams {
   const void *q, *k, *v;
   long long q_row, q_head, k_row, k_head, v_row, v_head;
   void* o;                       // forward out / backward in
+  void* low;                     // optional, 16-bit: what rounding took from o, (Mq, Hq, D) contiguous
   long long o_row, o_head;
   const void* dout;
   long long do_row, do_head;
@@ -514,6 +515,18 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       store4<T>(op + 32 * d + 8 * j + 4 * hh, f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv);
+  if (p.low) {   // the backward's delta = do . o loses a rounding of o against ds' own size; with both halves it does not
+    T* lp = (T*)p.low + (row * p.Hq + h) * D;
+#pragma unroll
+    for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 x = f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] -= bf16_to_f32(f32_to_bf16(x[r]));
+        store4<T>(lp + 32 * d + 8 * j + 4 * hh, x);
+      }
+  }
   if (hh == 0) p.lse[h * p.Mq + row] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
@@ -738,6 +751,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
     for (int e = 0; e < 4; ++e) {
       dl = fmaf(half_lo(gf[ks][e]), half_lo(of[e]), dl);
       dl = fmaf(half_hi(gf[ks][e]), half_hi(of[e]), dl);
+    }
+    if (p.low) {
+      const u32x4 lf = *(const u32x4*)((const T*)p.low + (row * p.Hq + h) * D + 16 * ks + 8 * hh);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dl = fmaf(half_lo(gf[ks][e]), half_lo(lf[e]), dl);
+        dl = fmaf(half_hi(gf[ks][e]), half_hi(lf[e]), dl);
+      }
     }
   }
   dl += __shfl_xor(dl, 32, 64);
@@ -1061,7 +1082,8 @@ int check(const PackedParams& p, int D, int dtype) {
   if ((p.Mk > 1 && (p.k_row < D || p.v_row < D)) || (p.Mq > 1 && p.q_row < D) || p.k_row > (1 << 24) || p.v_row > (1 << 24) ||
       p.q_row > (1 << 24))
     return MELGPT_ERR_UNSUPPORTED;
-  if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.o)) return MELGPT_ERR_ALIGN;
+  if (p.low && dtype == MELGPT_F32) return MELGPT_ERR_UNSUPPORTED;
+  if (!aligned16(p.low) || !aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.o)) return MELGPT_ERR_ALIGN;
   if (p.q_row % vec || p.q_head % vec || p.k_row % vec || p.k_head % vec || p.v_row % vec || p.v_head % vec || p.o_row % vec ||
       p.o_head % vec)
     return MELGPT_ERR_ALIGN;
@@ -1099,12 +1121,12 @@ int launch_bwd(const PackedParams& p, hipStream_t s) {
 
 extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                       long long k_head, const void* v, long long v_row, long long v_head, const int* cu_q,
-                                      const int* cu_k, int S, void* out, long long o_row, long long o_head, float* lse,
+                                      const int* cu_k, int S, void* out, long long o_row, long long o_head, void* out_low, float* lse,
                                       int write_gaps, long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype,
                                       void* stream) {
   PackedParams p = {};
   p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head;
-  p.v = v; p.v_row = v_row; p.v_head = v_head; p.o = out; p.o_row = o_row; p.o_head = o_head; p.lse = lse;
+  p.v = v; p.v_row = v_row; p.v_head = v_head; p.o = out; p.o_row = o_row; p.o_head = o_head; p.low = out_low; p.lse = lse;
   p.cu_q = cu_q; p.cu_k = cu_k; p.S = S; p.Hq = Hq; p.Hk = Hk; p.write_gaps = write_gaps; p.Mq = Mq; p.Mk = Mk; p.scale = scale;
   const int e = check(p, D, dtype);
   if (e) return e;
@@ -1117,7 +1139,7 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
 
 extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                       long long k_head, const void* v, long long v_row, long long v_head, const int* cu_q,
-                                      const int* cu_k, int S, const void* out, long long o_row, long long o_head,
+                                      const int* cu_k, int S, const void* out, long long o_row, long long o_head, const void* out_low,
                                       const void* dout, long long do_row, long long do_head, const float* lse, float* delta,
                                       void* dq, long long dq_row, long long dq_head, void* dk, long long dk_row,
                                       long long dk_head, void* dv, long long dv_row, long long dv_head, int write_gaps,
@@ -1125,6 +1147,7 @@ extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long 
   PackedParams p = {};
   p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head;
   p.v = v; p.v_row = v_row; p.v_head = v_head; p.o = const_cast<void*>(out); p.o_row = o_row; p.o_head = o_head;
+  p.low = const_cast<void*>(out_low);
   p.lse = const_cast<float*>(lse); p.delta = delta; p.dout = dout; p.do_row = do_row; p.do_head = do_head;
   p.dq = dq; p.dq_row = dq_row; p.dq_head = dq_head; p.dk = dk; p.dk_row = dk_row; p.dk_head = dk_head;
   p.dv = dv; p.dv_row = dv_row; p.dv_head = dv_head;

@@ -1159,15 +1159,16 @@ def _packed_args(i, q, k, v, cu_q, cu_k):
     return Mq, Mk, Hq, Hk, D, S, cu_k
 
 
-def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None):
+def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=False):
     """Causal attention of packed sequences: q (Mq, Hq, D), k, v (Mk, Hk, D), any row and head strides, Hq a multiple of Hk;
     sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
     cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
     -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  Rows behind the last sequence: left as they were in a given `out`, zero in a
-    new one.  scale: 1 / sqrt(D) unless given."""
+    new one.  scale: 1 / sqrt(D) unless given.  want_low: -> (out, lse, low), low what rounding out to 16 bits took from it
+    (None for f32), for packed_attn_bwd."""
     i = _device_of(q)
     if i != _current_device():
-        return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out)
+        return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out, want_low=want_low)
     dt = dtype_code(q.dtype)
     Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(i, q, k, v, cu_q, cu_k)
     vec = 4 if dt == _ffi.F32 else 8
@@ -1181,24 +1182,26 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None):
         assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
         _same_device(i, out)
     lse = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
+    low = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device) if want_low and dt != _ffi.F32 else None
     call("melgpt_packed_attn_fwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
-         cu_k.data_ptr(), S, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), gaps, Mq, Mk, Hq, Hk, D,
-         D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
-    return out, lse
+         cu_k.data_ptr(), S, out.data_ptr(), out.stride(0), out.stride(1), _addr(low), lse.data_ptr(), gaps, Mq, Mk, Hq, Hk,
+         D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
+    return (out, lse, low) if want_low else (out, lse)
 
 
-def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, grads=None):
-    """gradients of packed_attn_fwd from its inputs, both its results and dout (any row and head strides) -> (dq, dk, dv),
-    contiguous and zero in rows that no sequence owns, unless `grads` gives the three tensors (any row and head strides,
+def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, grads=None, low=None):
+    """gradients of packed_attn_fwd from its inputs, its results (out, lse and, if asked for, low) and dout (any row and head
+    strides) -> (dq, dk, dv), contiguous and zero in rows that no sequence owns, unless `grads` gives the three tensors (any row and head strides,
     such rows left as they were)."""
     i = _device_of(q)
     if i != _current_device():
-        return _on(i, packed_attn_bwd, q, k, v, out, dout, lse, cu_q, cu_k, scale=scale, grads=grads)
+        return _on(i, packed_attn_bwd, q, k, v, out, dout, lse, cu_q, cu_k, scale=scale, grads=grads, low=low)
     dt = dtype_code(q.dtype)
     Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(i, q, k, v, cu_q, cu_k)
     assert out.shape == q.shape == dout.shape and out.dtype == dout.dtype == q.dtype and out.stride(2) == 1
     assert lse.shape == (Hq, Mq) and lse.dtype == torch.float32 and lse.is_contiguous()
-    _same_device(i, out, dout, lse)
+    assert low is None or (low.shape == q.shape and low.dtype == q.dtype and low.is_contiguous())
+    _same_device(i, out, dout, lse, low)
     vec = 4 if dt == _ffi.F32 else 8
     q, qr, qh = _heads(q, vec)
     k, kr, kh = _heads(k, vec)
@@ -1216,7 +1219,7 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
         _same_device(i, dq, dk, dv)
     delta = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
     call("melgpt_packed_attn_bwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
-         cu_k.data_ptr(), S, out.data_ptr(), our, ouh, dout.data_ptr(), dor, doh, lse.data_ptr(), delta.data_ptr(), dq.data_ptr(),
+         cu_k.data_ptr(), S, out.data_ptr(), our, ouh, _addr(low), dout.data_ptr(), dor, doh, lse.data_ptr(), delta.data_ptr(), dq.data_ptr(),
          dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0), dv.stride(1), gaps, Mq,
          Mk, Hq, Hk, D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
     return dq, dk, dv

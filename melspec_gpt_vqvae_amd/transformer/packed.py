@@ -69,16 +69,16 @@ def qk_norm_rotary(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=
 class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale):
-        out, lse = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        out, lse, low = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale, want_low=True)
+        ctx.save_for_backward(q, k, v, out, lse, low, cu_q, cu_k)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
-        return ops.packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k, scale=ctx.scale) + (None, None, None)
+        q, k, v, out, lse, low, cu_q, cu_k = ctx.saved_tensors
+        return ops.packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k, scale=ctx.scale, low=low) + (None, None, None)
 
 
 def packed_attention(q, k, v, cu_q, cu_k=None, *, scale=None):

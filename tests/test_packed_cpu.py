@@ -61,8 +61,10 @@ def test_append_refusals(kw, code):
     assert append(**kw) == code
 
 
-def packed(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF):
-    return _lib().melgpt_packed_attn_fwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, lse, 1, Mq, Mk, Hq, Hk, D, 0.125, dt, None)
+def packed(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF,
+           low=None):
+    return _lib().melgpt_packed_attn_fwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, lse, 1, Mq, Mk, Hq, Hk, D, 0.125, dt,
+                                         None)
 
 
 PACKED_REFUSALS = [
@@ -71,7 +73,7 @@ PACKED_REFUSALS = [
     (dict(Hq=9), UNSUPPORTED), (dict(D=96), UNSUPPORTED), (dict(D=32), UNSUPPORTED), (dict(dt=2), UNSUPPORTED),
     (dict(kr=56), UNSUPPORTED), (dict(vr=0), UNSUPPORTED), (dict(qr=8), UNSUPPORTED), (dict(kr=1 << 25), UNSUPPORTED),
     (dict(Mq=1 << 23), UNSUPPORTED), (dict(S=1 << 20), UNSUPPORTED), (dict(Mk=1 << 31), UNSUPPORTED), (dict(q=P + 8), ALIGN),
-    (dict(v=P + 2), ALIGN), (dict(orow=100), ALIGN), (dict(qr=516), ALIGN)]
+    (dict(v=P + 2), ALIGN), (dict(orow=100), ALIGN), (dict(qr=516), ALIGN), (dict(low=P + 8), ALIGN), (dict(low=P, dt=F32), UNSUPPORTED)]
 
 
 @pytest.mark.parametrize("kw,code", PACKED_REFUSALS + [(dict(Mq=0), OK)])
@@ -80,8 +82,8 @@ def test_packed_refusals(kw, code):
 
 
 def packed_bwd(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF,
-               do=P, dor=512, delta=P, dq=P, dqr=512, dk=P, dv=P):
-    return _lib().melgpt_packed_attn_bwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, do, dor, 64, lse, delta, dq, dqr, 64,
+               do=P, dor=512, delta=P, dq=P, dqr=512, dk=P, dv=P, low=P):
+    return _lib().melgpt_packed_attn_bwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, do, dor, 64, lse, delta, dq, dqr, 64,
                                          dk, 256, 64, dv, 256, 64, 1, Mq, Mk, Hq, Hk, D, 0.125, dt, None)
 
 
