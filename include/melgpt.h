@@ -583,11 +583,15 @@ int melgpt_kv_append(const void* q, long long q_row, long long q_head, const voi
  * out_low (16-bit lane, optional, (Mq, Hq, D) contiguous): what the rounding of out took away, written by the forward and,
  * given to the backward, restored in its delta.
  * write_gaps: rows of the outputs that no sequence owns are zeroed (lse -inf), otherwise left as they were.
+ * splits: workgroups that share a row tile's keys (16-bit lane without out_low; 1: one), joined in a fixed order by a second
+ * kernel; melgpt_packed_attn_splits proposes it from the sizes.  With splits > 1 `workspace` holds splits * Hq * Mq * (D + 2)
+ * f32, 16-byte aligned.
  * D 64 or 128; scale multiplies the scores; at most 4 M rows (65535 tiles of 64 with one more per sequence). */
+int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int Hq, int D, int dtype);
 int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                            const void* v, long long v_row, long long v_head, const int* cu_q, const int* cu_k, int S, void* out,
-                           long long o_row, long long o_head, void* out_low, float* lse, int write_gaps, long long Mq, long long Mk, int Hq,
-                           int Hk, int D, float scale, int dtype, void* stream);
+                           long long o_row, long long o_head, void* out_low, float* lse, int write_gaps, int splits, float* workspace,
+                           long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype, void* stream);
 int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                            const void* v, long long v_row, long long v_head, const int* cu_q, const int* cu_k, int S,
                            const void* out, long long o_row, long long o_head, const void* out_low, const void* dout, long long do_row,

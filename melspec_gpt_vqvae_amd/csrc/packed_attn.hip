@@ -35,6 +35,8 @@ struct PackedParams {
   long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
   float *lse, *delta;            // (Hq, Mq)
   const int *cu_q, *cu_k;        // (S + 1)
+  int splits;                    // forward, 16-bit: workgroups that share a row tile's keys
+  float* part;                   // splits > 1: (splits, Hq, Mq, D) sums of e^(s - m) v, then (splits, Hq, Mq, 2): m (base 2), sums
   int S, Hq, Hk, G, write_gaps;  // write_gaps: zero the rows no sequence owns
   long long Mq, Mk;
   float scale;
@@ -160,6 +162,64 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// ---- values that are not finite, at keys that only some queries of a workgroup see.  A masked probability is 0, but
+// 0 * NaN is not: in tiles that the causal border cuts such values are stored as zeros, and what they add to the queries that
+// do see them is added at the end, key by key, outside the matrix instructions.
+template <typename T>
+__device__ __forceinline__ bool finite_bits(unsigned v) {   // of an f32, or of both of two 16-bit values
+  if constexpr (sizeof(T) == 4) return (v & 0x7f800000u) != 0x7f800000u;
+#ifdef MELGPT_HALF_FP16
+  else return (((v & 0x7c007c00u) + 0x04000400u) & 0x80008000u) == 0u;
+#else
+  else return (((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u) == 0u;
+#endif
+}
+template <typename T>
+__device__ __forceinline__ bool finite16(u32x4 v) {
+  return finite_bits<T>(v[0]) && finite_bits<T>(v[1]) && finite_bits<T>(v[2]) && finite_bits<T>(v[3]);
+}
+// zeros in place of the values that are not finite
+template <typename T>
+__device__ __forceinline__ u32x4 finite_part(u32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      if (!finite_bits<T>(v[e])) v[e] = 0u;
+    } else {
+      if (!finite_bits<T>(v[e] & 0xffffu)) v[e] &= 0xffff0000u;
+      if (!finite_bits<T>(v[e] & 0xffff0000u)) v[e] &= 0xffffu;
+    }
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ float value_of(const T* p) { return Elem<T>::ld(p); }
+// adds the contributions of such values at keys k0 .. k1 - 1 to this lane's query (which sees keys below `sees`; running
+// maximum m, base 2): get(i) / add(i, x) for the lane's n accumulators of value column col(i)
+template <typename T, int D, int N, typename Col, typename Add>
+__device__ __forceinline__ void add_not_finite(const T* q, const T* k, long long k_row, const T* v, long long v_row, int k0, int k1,
+                                               int sees, float scale2, float m, int lane, Col col, Add add) {
+  const float base = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll 1
+  for (int j = k0; j < k1; ++j) {
+    bool fine = true;
+    for (int d = lane; d < D; d += 64) {
+      const float x = value_of(v + j * v_row + d);
+      fine = fine && __builtin_isfinite(x);
+    }
+    if (__all(fine)) continue;
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) s = fmaf(value_of(q + d), value_of(k + j * k_row + d), s);
+    const float pr = __builtin_amdgcn_exp2f(fmaf(s, scale2, -base));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = value_of(v + j * v_row + col(i));
+      if (j < sees && !__builtin_isfinite(x)) add(i, pr * x);
+    }
+  }
+}
+
 // 32 rows of two tensors on their way into LDS: the loads of the next pair are in flight under the current pair's products.
 // Rows at and beyond n are zero (their products are masked, but 0 * NaN is not 0).
 template <typename T, int D>
@@ -174,6 +234,16 @@ struct Stage {
       a[i] = *(const u32x4*)(pa + row * ra + c * L::VEC);
       b[i] = *(const u32x4*)(pb + row * rb + c * L::VEC);
     }
+  }
+  // -> whether tensor b had values that are not finite (it has zeros there now)
+  __device__ __forceinline__ bool clean_b() {
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) fine = fine && finite16<T>(b[i]);
+    if (fine) return false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) b[i] = finite_part<T>(b[i]);
+    return true;
   }
   __device__ __forceinline__ void store(char* ta, char* tb, int row0, int n, int t) const {
 #pragma unroll
@@ -195,6 +265,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
   using L = Tile<T, D>;
   __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
+  __shared__ int odd;                                              // a value that is not finite in a tile the causal border cuts
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
   int h;
   head_of(blockIdx.x, p, h);
@@ -222,7 +293,11 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
   float m = -__builtin_inff(), l = 0.f;
   if (most > 0) {
     Stage<T, D> st;
+    const int full = min(max(64 * R.tile + nk - R.n + 1, 0), nk);  // keys that every query of the workgroup sees
+    if (t == 0) odd = 0;
+    __syncthreads();
     st.load(kp, p.k_row, vp, p.v_row, 0, nk, t);
+    if (32 > full && st.clean_b()) odd = 1;
     st.store(lds[0][0], lds[0][1], 0, nk, t);
     __syncthreads();
     for (int k0 = 0, buf = 0; k0 < most; k0 += 32, buf ^= 1) {
@@ -265,10 +340,14 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
 #pragma unroll
         for (int d = 0; d < L::DT; ++d) mma<T>(o[d], L::cols(vt, e, d, lane), pf);
       }
+      if (more && k0 + 64 > full && st.clean_b()) odd = 1;
       if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 32, nk, t);
       __syncthreads();
     }
     l = across_groups_sum(l);
+    if (odd)
+      add_not_finite<T, D, 4 * L::DT>(qp, kp, p.k_row, vp, p.v_row, full & ~31, most, sees, c2, m, lane,
+                                      [&](int i) { return 16 * (i >> 2) + 4 * g + (i & 3); }, [&](int i, float x) { o[i >> 2][i & 3] += x; });
   }
   if (!mine) return;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;        // (NaN stays NaN)
@@ -353,6 +432,15 @@ struct Stage64 {
   __device__ __forceinline__ void load1(__amdgpu_buffer_rsrc_t r, int i) {
     a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, from, 2u * STEP * i * (unsigned)rs, 0));
   }
+  __device__ __forceinline__ bool clean() {   // -> whether there were values that are not finite (there are zeros now)
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) fine = fine && finite16<bf16_t>(a[i]);
+    if (fine) return false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) a[i] = finite_part<bf16_t>(a[i]);
+    return true;
+  }
   __device__ __forceinline__ void store1(char* t, int i) const { *(u32x4*)(t + off + i * STEP * L::RB) = a[i]; }
   __device__ __forceinline__ void load(int row0, int n) {
     const __amdgpu_buffer_rsrc_t r = at(row0, n);
@@ -370,6 +458,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   using L = Tile32<D>;
   using T = bf16_t;
   __shared__ __attribute__((aligned(16))) char lds[2][2][64 * L::RB];
+  __shared__ int odd;                                              // a value that is not finite in a tile the causal border cuts
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
   int h;
   head_of(blockIdx.x, p, h);
@@ -405,10 +494,12 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
 #pragma unroll
   for (int d = 0; d < L::DB; ++d) o[d] = zero16();
   float m = -__builtin_inff(), l[2] = {0.f, 0.f};                  // two partial sums: independent chains
-  if (most > 0) {
+  // this workgroup's share of the key tiles
+  const int every = (most + 63) >> 6, per = (every + p.splits - 1) / p.splits;
+  const int i0 = per * (int)blockIdx.z, tiles = min(every - i0, per), k_first = 64 * i0;
+  if (tiles > 0) {
     Stage64<D, false> ks_(kp, p.k_row, t);
     Stage64<D, true> vs_(vp, p.v_row, t);
-    const int tiles = (most + 63) >> 6;
     auto scores = [&](const char* kt, int half, f32x16& s) __attribute__((always_inline)) {
       s = zero16();
 #pragma unroll
@@ -477,25 +568,28 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
     };
     // K runs one tile ahead of V in LDS: [0] K, [1] V, two slots each, tile i in slot i & 1.  Iteration i's stores go to
     // slots last read two steps ago, with the previous iteration's barrier in between.
-    ks_.load(0, nk);
+    const int all = min(max(128 * R.tile + nk - R.n + 1, 0), nk);  // keys that every query of the workgroup sees
+    if (t == 0) odd = 0;
+    ks_.load(k_first, nk);
 #pragma unroll
     for (int i = 0; i < 64 * L::RB / (256 * 16); ++i) *(u32x4*)(lds[1][1] + (t + 256 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
     ks_.store(lds[0][0]);
-    ks_.load(64, nk);
-    vs_.load(0, nk);
+    ks_.load(k_first + 64, nk);
+    vs_.load(k_first, nk);
     __syncthreads();
     f32x16 s0, s1;
     u32x4 p0[2], p1[2] = {u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}};
     scores(lds[0][0], 0, s0);
     auto tile = [&](int i, auto par) __attribute__((always_inline)) {   // par = i & 1, known to the compiler: LDS addresses are constants
       constexpr int P = decltype(par)::value;
-      step(64 * i, s0, s1, lds[0][P], 1, p1, p0, lds[1][P ^ 1], 1);
+      step(k_first + 64 * i, s0, s1, lds[0][P], 1, p1, p0, lds[1][P ^ 1], 1);
       ks_.store(lds[0][P ^ 1]);                                    // (behind the last tile: zeros, never used)
+      if (k_first + 64 * i + 64 > all && vs_.clean()) odd = 1;
       vs_.store(lds[1][P]);
       __syncthreads();
-      ks_.load(64 * i + 128, nk);
-      vs_.load(64 * i + 64, nk);
-      step(64 * i + 32, s1, s0, lds[0][P ^ 1], 0, p0, p1, lds[1][P], 0);
+      ks_.load(k_first + 64 * i + 128, nk);
+      vs_.load(k_first + 64 * i + 64, nk);
+      step(k_first + 64 * i + 32, s1, s0, lds[0][P ^ 1], 0, p0, p1, lds[1][P], 0);
     };
     int i = 0;
     for (; i + 1 < tiles; i += 2) {
@@ -504,10 +598,24 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
     }
     if (i < tiles) tile(i, std::integral_constant<int, 0>());
     weigh(lds[1][(tiles - 1) & 1], 1, p1);
+    if (odd)
+      add_not_finite<T, D, 16 * L::DB>(qp, kp, p.k_row, vp, p.v_row, max(all & ~63, k_first), min(most, k_first + 64 * tiles), sees, p.scale * LOG2E, m, lane,
+                                       [&](int i) { return 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hh + (i & 3); },
+                                       [&](int i, float x) { o[i >> 4][i & 15] += x; });
   }
   float sum = l[0] + l[1];
   sum += __shfl_xor(sum, 32, 64);
   if (q_in >= R.n) return;
+  if (p.splits > 1) {
+    const long long at = ((long long)blockIdx.z * p.Hq + h) * p.Mq + row;
+#pragma unroll
+    for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(f32x4*)(p.part + at * D + 32 * d + 8 * j + 4 * hh) = f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+    if (hh == 0) *(f32x2*)(p.part + (long long)p.splits * p.Hq * p.Mq * D + 2 * at) = f32x2{m, sum};
+    return;
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
 #pragma unroll
@@ -528,6 +636,34 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
       }
   }
   if (hh == 0) p.lse[h * p.Mq + row] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * LN2;
+}
+
+// joins the splits of a query in their order: D / 4 lanes, four values each
+template <int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
+  using T = bf16_t;
+  constexpr int TPQ = D / 4;
+  const long long n = (long long)blockIdx.x * (256 / TPQ) + threadIdx.x / TPQ, all = (long long)p.Hq * p.Mq;
+  if (n >= all) return;
+  const int d = 4 * (threadIdx.x % TPQ), h = (int)(n / p.Mq);
+  const long long row = n % p.Mq;
+  const bool gap = row < bound_at(p.cu_q, p.S, p.Mq, 1) || row >= bound_at(p.cu_q, p.S, p.Mq, p.S + 1);
+  if (gap && !p.write_gaps) return;
+  const float* st = p.part + (long long)p.splits * all * D + 2 * n;
+  float top = -__builtin_inff();
+  for (int i = 0; i < p.splits; ++i) top = fmaxf(top, st[2 * i * all]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < p.splits; ++i) {
+    const float f = __builtin_amdgcn_exp2f(st[2 * i * all] - base);
+    a += *(const f32x4*)(p.part + (i * all + n) * D + d) * f;
+    sum += st[2 * i * all + 1] * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  store4<T>((T*)p.o + row * p.o_row + h * p.o_head + d, a * inv);
+  if (d == 0) p.lse[n] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
 // -------------------------------------------------------------------------------------------------------- backward
@@ -1095,9 +1231,13 @@ int launch_fwd(const PackedParams& p, hipStream_t s) {
   const int bm = sizeof(T) == 2 ? 128 : 64;
   const long long tiles = tiles_for(p.Mq, p.S, bm);
   if (tiles > 65535) return MELGPT_ERR_UNSUPPORTED;
-  if constexpr (sizeof(T) == 2)
-    hipLaunchKernelGGL((packed_fwd32_kernel<D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
-  else
+  if constexpr (sizeof(T) == 2) {
+    hipLaunchKernelGGL((packed_fwd32_kernel<D>), dim3(p.Hq, (unsigned)tiles, (unsigned)p.splits), dim3(256), 0, s, p);
+    if (p.splits > 1) {
+      const long long per = 256 / (D / 4);
+      hipLaunchKernelGGL((packed_join_kernel<D>), dim3((unsigned)((p.Hq * p.Mq + per - 1) / per)), dim3(256), 0, s, p);
+    }
+  } else
     hipLaunchKernelGGL((packed_fwd_kernel<T, D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
   return melgpt_launch_status();
 }
@@ -1119,17 +1259,44 @@ int launch_bwd(const PackedParams& p, hipStream_t s) {
 
 }  // namespace
 
+// Workgroups that share the keys of a row tile, where the row tiles alone would not fill the card (a prompt's continuation
+// over a long past).  By a model of the launch in microseconds: rounds of the 512 (D 128) or 768 (D 64) workgroups that run
+// at once, times a workgroup's 64-key tiles (1.7 / 0.9 us each with full CUs), plus the join (4 us, and 8 bytes a value and
+// split at 4 TB/s).  Measured in one piece / in the n it takes, 32 heads of 128 over 16000 keys: 1500 queries 516 / 416 us
+// (4), 512: 317 / 151 (4), 256: 312 / 91 (8), 128: 311 / 63 (16); 16 heads of 64, 1000 over 8000: 118 / 57 (6).
+extern "C" int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int Hq, int D, int dtype) {
+  if (dtype != MELGPT_BF16 || Mq <= 0 || Mk <= 0 || S <= 0 || Hq <= 0 || (D != 64 && D != 128)) return 1;
+  const double slots = D == 64 ? 768 : 512, tile_us = D == 64 ? 0.9 : 1.7;
+  const double base = (double)Hq * (double)((Mq + 127) / 128 + (S - 1) / 2), keys = (double)((Mk / S + 63) / 64);
+  if (base > slots) return 1;
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= 16 && n * 4 <= keys + 3; ++n) {
+    const double rounds = (double)(long long)((base * n + slots - 1) / slots), each = (double)(long long)((keys + n - 1) / n);
+    const double us = rounds * each * tile_us + (n > 1 ? 4 + (double)Mq * Hq * n * D * 8 / 4e6 : 0);
+    if (n == 1 || us < least) {
+      least = us;
+      best = n;
+    }
+  }
+  return best;
+}
+
 extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                       long long k_head, const void* v, long long v_row, long long v_head, const int* cu_q,
                                       const int* cu_k, int S, void* out, long long o_row, long long o_head, void* out_low, float* lse,
-                                      int write_gaps, long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype,
-                                      void* stream) {
+                                      int write_gaps, int splits, float* workspace, long long Mq, long long Mk, int Hq, int Hk,
+                                      int D, float scale, int dtype, void* stream) {
   PackedParams p = {};
+  p.splits = splits; p.part = workspace;
   p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head;
   p.v = v; p.v_row = v_row; p.v_head = v_head; p.o = out; p.o_row = o_row; p.o_head = o_head; p.low = out_low; p.lse = lse;
   p.cu_q = cu_q; p.cu_k = cu_k; p.S = S; p.Hq = Hq; p.Hk = Hk; p.write_gaps = write_gaps; p.Mq = Mq; p.Mk = Mk; p.scale = scale;
   const int e = check(p, D, dtype);
   if (e) return e;
+  if (splits < 1 || (splits > 1 && !workspace)) return MELGPT_ERR_BAD_ARG;
+  if (splits > 1 && (dtype == MELGPT_F32 || out_low || splits > 1024 || Hq * Mq > (1LL << 32))) return MELGPT_ERR_UNSUPPORTED;
+  if (!aligned16(workspace)) return MELGPT_ERR_ALIGN;
   if (Mq == 0) return MELGPT_OK;
   p.G = Hq / Hk;
   hipStream_t s = (hipStream_t)stream;

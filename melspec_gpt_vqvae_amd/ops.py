@@ -1183,9 +1183,14 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
         _same_device(i, out)
     lse = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
     low = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device) if want_low and dt != _ffi.F32 else None
+    splits, ws = 1, None
+    if low is None and dt != _ffi.F32:
+        splits = _ffi.lib().melgpt_packed_attn_splits(Mq, Mk, S, Hq, D, dt)
+        if splits > 1:   # (a buffer of the call's own: two captured graphs never share it)
+            ws = torch.empty(splits * Hq * Mq * (D + 2), dtype=torch.float32, device=q.device)
     call("melgpt_packed_attn_fwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
-         cu_k.data_ptr(), S, out.data_ptr(), out.stride(0), out.stride(1), _addr(low), lse.data_ptr(), gaps, Mq, Mk, Hq, Hk,
-         D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
+         cu_k.data_ptr(), S, out.data_ptr(), out.stride(0), out.stride(1), _addr(low), lse.data_ptr(), gaps, splits,
+         _addr(ws), Mq, Mk, Hq, Hk, D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
     return (out, lse, low) if want_low else (out, lse)
 
 

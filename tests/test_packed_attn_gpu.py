@@ -107,6 +107,29 @@ def test_scale_and_large_scores():
     check([50], [50], 2, 2, 64, torch.float32, scale=-0.125)
 
 
+def test_few_queries_over_many_keys():
+    """the keys of a row tile shared by several workgroups"""
+    from melspec_gpt_vqvae_amd import _ffi, ops
+
+    split = _ffi.lib().melgpt_packed_attn_splits
+    for lq, lk, Hq, Hk, D in (([3], [3000], 4, 2, 64), ([130], [1500], 2, 1, 128), ([1, 20, 5], [700, 2000, 3], 4, 1, 128), ([40, 0, 200], [2900, 7, 180], 2, 2, 64)):
+        assert split(sum(lq), sum(lk), len(lq), Hq, D, _ffi.BF16) > 1
+        check(lq, lk, Hq, Hk, D, _half(), backward=False, seed=4)
+        check(lq, lk, Hq, Hk, D, _half(), seed=4)                  # (with gradients: in one piece)
+    # rows of nobody, in a new and a given output
+    q, k, v, _ = [x.to(DEV) for x in make([30], [2100], 4, 2, 64, _half(), 4)]
+    cu_q = torch.tensor([4, 20], dtype=torch.int32, device=DEV)
+    cu_k = torch.tensor([50, 2080], dtype=torch.int32, device=DEV)
+    assert split(30, 2100, 1, 4, 64, _ffi.BF16) > 1
+    out, lse = ops.packed_attn_fwd(q, k, v, cu_q, cu_k)
+    given = torch.full_like(out, 5.0)
+    ops.packed_attn_fwd(q, k, v, cu_q, cu_k, out=given)
+    assert torch.equal(given[4:20], out[4:20]) and (given[:4] == 5).all() and (given[20:] == 5).all()
+    assert (out[:4] == 0).all() and (out[20:] == 0).all() and torch.isinf(lse[:, 20:]).all()
+    want, _, _ = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, want_low=True)
+    assert float((want.float() - out.float()).abs().max()) <= 4 * R.half_step(_half()) * float(want.float().abs().max())
+
+
 def test_many_short_sequences():
     lens = [(7 * i) % 5 for i in range(5000)]                     # more sequences than one 64-way step of the search covers
     check(lens[:300], lens[:300], 2, 1, 64, _half(), seed=2)
@@ -261,3 +284,35 @@ def test_other_stream():
         grads = ops.packed_attn_bwd(q, k, v, got, do, lse, cu)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want) and all(torch.isfinite(x.float()).all() for x in grads)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("n,D", [(200, 64), (200, 128), (130, 128)])
+def test_values_that_are_not_finite_reach_only_the_queries_that_see_them(n, D, dtype):
+    from melspec_gpt_vqvae_amd import ops
+
+    dt = _dt(dtype)
+    more = 40
+    q, k, v, _ = make([n], [n + more], 4, 2, D, dt, 6)
+    cu_q, cu_k = _cu([n]).to(DEV), _cu([n + more]).to(DEV)
+    base, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), cu_q, cu_k)
+    bad_v, bad_k = v.clone(), k.clone()
+    bad_v[more + 100, 0, 3] = float("nan")
+    bad_v[more + 64, 1, D - 1] = float("inf")
+    bad_v[more + 120, 1, 7] = float("-inf")
+    out, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), bad_v.to(DEV), cu_q, cu_k)
+    want = base.clone()
+    want[100:, :2, 3] = float("nan")                     # key 40 + 100 is the last key of query 100
+    want[64:, 2:, D - 1] = float("inf")
+    want[120:, 2:, 7] = float("-inf")
+    same = (out == want) | (torch.isnan(out) & torch.isnan(want))
+    assert same.all(), torch.nonzero(~same)[:5]
+    bad_k[more + 90, 0, 0] = float("nan")
+    out, lse = ops.packed_attn_fwd(q.to(DEV), bad_k.to(DEV), v.to(DEV), cu_q, cu_k)
+    assert torch.equal(out[:90], base[:90]) and torch.equal(out[:, 2:], base[:, 2:]) and torch.isnan(out[90:, :2]).all()
+    assert torch.isnan(lse[:2, 90:]).all()
+    # a value that is not finite in front of every border: all queries of its key head see it
+    bad_v = v.clone()
+    bad_v[0, 0, 5] = float("inf")
+    out, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), bad_v.to(DEV), cu_q, cu_k)
+    assert torch.isinf(out[:, :2, 5]).all() and torch.equal(out[:, 2:], base[:, 2:])

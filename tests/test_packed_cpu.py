@@ -62,9 +62,9 @@ def test_append_refusals(kw, code):
 
 
 def packed(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF,
-           low=None):
-    return _lib().melgpt_packed_attn_fwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, lse, 1, Mq, Mk, Hq, Hk, D, 0.125, dt,
-                                         None)
+           low=None, splits=1, ws=None):
+    return _lib().melgpt_packed_attn_fwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, lse, 1, splits, ws, Mq, Mk, Hq,
+                                         Hk, D, 0.125, dt, None)
 
 
 PACKED_REFUSALS = [
@@ -76,7 +76,9 @@ PACKED_REFUSALS = [
     (dict(v=P + 2), ALIGN), (dict(orow=100), ALIGN), (dict(qr=516), ALIGN), (dict(low=P + 8), ALIGN), (dict(low=P, dt=F32), UNSUPPORTED)]
 
 
-@pytest.mark.parametrize("kw,code", PACKED_REFUSALS + [(dict(Mq=0), OK)])
+@pytest.mark.parametrize("kw,code", PACKED_REFUSALS + [
+    (dict(Mq=0), OK), (dict(splits=0), BAD), (dict(splits=2), BAD), (dict(splits=2, ws=P, dt=F32), UNSUPPORTED),
+    (dict(splits=2, ws=P, low=P), UNSUPPORTED), (dict(splits=2000, ws=P), UNSUPPORTED), (dict(splits=2, ws=P + 4), ALIGN)])
 def test_packed_refusals(kw, code):
     assert packed(**kw) == code
 
@@ -116,6 +118,12 @@ def test_splits():
         s = f(S, Hq, Hk, n)
         assert 1 <= s <= 128 and (s == 1 or n >= 256 * (s - 1))
     assert f(1, 16, 16, 200) == 1 and f(0, 1, 1, 5) == 1 and f(1, 1, 1, 0) == 1
+
+
+def test_packed_splits():
+    f = _lib().melgpt_packed_attn_splits
+    assert f(1500, 16001, 1, 32, 128, F32) == 1 and f(100, 100, 1, 16, 64, HALF) == 1 and f(30000, 30000, 1, 32, 128, HALF) == 1
+    assert f(1, 16000, 1, 32, 128, HALF) > 4 and 1 < f(1500, 16001, 1, 32, 128, HALF) <= 16 and f(0, 5, 1, 1, 64, HALF) == 1
 
 
 def test_cpu_tensors_and_wrong_arguments_are_refused():
