@@ -1012,39 +1012,53 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
   }
   const int blocks = first < nq ? (nq - first + 63) / 64 : 0, total = blocks * p.G;
   if (total > 0) {
+    // Tiles in order: head by head, the queries from the last down.  Addresses and sizes of the tile to load next are kept as
+    // running scalars: one wave per SIMD issues everything itself, and a tile's 64-bit products were a quarter of a step.
+    // Wave parity picks the row of statistics (lse, delta) a wave fetches; both waves of a parity store the same.
     Stage64<D, true> qs_((const T*)p.q, p.q_row, t), gs_((const T*)p.dout, p.do_row, t);
+    const int top = first + 64 * (blocks - 1), st_row = wave & 1;
+    const long long q_at = (long long)(q_lo + top) * p.q_row + (long long)hk * p.G * p.q_head;
+    const long long g_at = (long long)(q_lo + top) * p.do_row + (long long)hk * p.G * p.do_head;
+    const T *qa = (const T*)p.q + q_at, *ga = (const T*)p.dout + g_at;
+    const float* sa = (st_row ? p.delta : p.lse) + (long long)hk * p.G * p.Mq + q_lo + top;
+    const long long q_down = 64 * p.q_row, g_down = 64 * p.do_row, q_next = (long long)(top - first) * p.q_row + p.q_head,
+                    g_next = (long long)(top - first) * p.do_row + p.do_head, s_next = top - first + p.Mq;
+    const unsigned rest = (unsigned)min(nq - top, 64);             // rows of a head's last tile
+    const unsigned q_rest = 2u * ((rest - 1) * (unsigned)p.q_row + D), g_rest = 2u * ((rest - 1) * (unsigned)p.do_row + D);
+    const unsigned q_full = 2u * (63u * (unsigned)p.q_row + D), g_full = 2u * (63u * (unsigned)p.do_row + D);
+    const float s_mul = st_row ? 1.f : LOG2E;
+    int lq = top, left = total;                                    // first query of the tile to load next, tiles left
     float sv = 0.f;
-    // head by head, the queries from the last down
-    const int top = first + 64 * (blocks - 1);
-    int lh = hk * p.G, lq = top, left = total;                     // head and first query of the tile to load next, tiles left
-    auto aim = [&]() __attribute__((always_inline)) {              // at the tile to load next (none left: at nothing, zeros)
-      qs_.base = (const T*)p.q + (long long)q_lo * p.q_row + lh * p.q_head;
-      gs_.base = (const T*)p.dout + (long long)q_lo * p.do_row + lh * p.do_head;
-    };
-    auto load_stat = [&]() __attribute__((always_inline)) {
-      if (t < 128 && left > 0) {
-        const long long r = lh * p.Mq + q_lo + min(lq + (t & 63), nq - 1);
-        // a query that sees no key has lse -inf; +inf makes its probabilities 0 instead of NaN
-        const float x = t < 64 ? p.lse[r] * LOG2E : p.delta[r];
-        sv = t < 64 && x == -__builtin_inff() ? __builtin_inff() : x;
-      }
-      lq -= 64;
-      if (lq < first) {
-        lq = top;
-        lh = min(lh + 1, hk * p.G + p.G - 1);
-      }
+    auto next = [&]() __attribute__((always_inline)) {
+      const bool wrap = lq == first;
+      qa += wrap ? q_next : -q_down;
+      ga += wrap ? g_next : -g_down;
+      sa += wrap ? s_next : -64;
+      lq = wrap ? top : lq - 64;
       --left;
     };
+    auto q_tile = [&]() __attribute__((always_inline)) { return make_rsrc(qa, left <= 0 ? 0u : lq == top ? q_rest : q_full); };
+    auto g_tile = [&]() __attribute__((always_inline)) { return make_rsrc(ga, left <= 0 ? 0u : lq == top ? g_rest : g_full); };
+    auto load_stat = [&]() __attribute__((always_inline)) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(sa, left <= 0 ? 0u : lq == top ? 4u * rest : 256u);
+      const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4u * lane, 0, 0)) * s_mul;
+      // a query that sees no key has lse -inf; +inf makes its probabilities 0 instead of NaN
+      sv = !st_row && x == -__builtin_inff() ? __builtin_inff() : x;
+    };
     auto load = [&]() __attribute__((always_inline)) {
-      aim();
-      qs_.load(lq, left > 0 ? nq : 0);
-      gs_.load(lq, left > 0 ? nq : 0);
+      const __amdgpu_buffer_rsrc_t rq = q_tile(), rg = g_tile();
+#pragma unroll
+      for (int i = 0; i < Stage64<D, true>::PER; ++i) {
+        qs_.load1(rq, i);
+        gs_.load1(rg, i);
+      }
       load_stat();
+      next();
     };
     auto store = [&](int slot) __attribute__((always_inline)) {
       qs_.store(tiles_ + 2 * slot * TB);
       gs_.store(tiles_ + (2 * slot + 1) * TB);
-      if (t < 128) stat[128 * slot + t] = sv;
+      stat[128 * slot + 64 * st_row + lane] = sv;
     };
     // The matrix instructions of a step, in order: the products of one block (2 NKS), the gradients of another (4 DB); with
     // each, the fragment of tile rows or columns it takes
@@ -1083,17 +1097,16 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
       s[B] = zero16();
       dp[B] = zero16();
       f32x4 ls[4], de[4];                                          // accumulators 4 j .. + 3: queries 8 j + 4 hh .. + 3
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      auto stats = [&](int j) __attribute__((always_inline)) {
         ls[j] = *(const f32x4*)&stat[128 * SL + 32 * qh + 8 * j + 4 * hh];
         de[j] = *(const f32x4*)&stat[128 * SL + 64 + 32 * qh + 8 * j + 4 * hh];
-      }
-      aim();
-      const __amdgpu_buffer_rsrc_t rq = qs_.at(lq, left > 0 ? nq : 0), rg = gs_.at(lq, left > 0 ? nq : 0);
+      };
+      stats(0);
+      const __amdgpu_buffer_rsrc_t rq = q_tile(), rg = g_tile();
       // laid out by hand: hipcc on its own reads every fragment right in front of the product that waits for it.  With each
-      // matrix instruction go the read of the fragment five later, its share of the probabilities, and (in the last part) the
+      // matrix instruction go the read of the fragment four later, its share of the probabilities, and (in the last part) the
       // stores of the tile loaded during the step before, each followed by the load that refills its registers
-      constexpr int AHEAD = 5, PER = Stage64<D, true>::PER;
+      constexpr int AHEAD = 4, PER = Stage64<D, true>::PER;
       u32x4 f[NM];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i, (SL + 1) & 3, (SL + 3) & 3);
@@ -1104,6 +1117,7 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
         multiply(i, f[i], s[B], dp[B], pf[B], sf[B]);
 #pragma unroll
         for (int r = 16 * i / NM; r < 16 * (i + 1) / NM; ++r) {
+          if ((r & 3) == 0 && r < 12) stats(r / 4 + 1);
           s[A][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[A][r], c2, -ls[r >> 2][r & 3]));
           dp[A][r] = s[A][r] * (dp[A][r] - de[r >> 2][r & 3]);
           if ((r & 7) == 7) {
@@ -1130,8 +1144,9 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
       for (int d = 0; d < L::DB; ++d) asm volatile("" : "+a"(dk[d]), "+a"(dv[d]));
 #pragma unroll
       for (int ks = 0; ks < L::NKS; ++ks) asm volatile("" : "+a"(kf[ks]), "+a"(vf[ks]));
-      if (t < 128) stat[128 * ((SL + 2) & 3) + t] = sv;
+      stat[128 * ((SL + 2) & 3) + 64 * st_row + lane] = sv;
       load_stat();
+      next();
       q0 -= 64;
       if (q0 < first) q0 = top + 32 * qh;
       __syncthreads();
