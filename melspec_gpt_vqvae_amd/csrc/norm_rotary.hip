@@ -15,6 +15,8 @@
 // Angles are formed in 64 bits in TURNS (pos * freqs / 2 pi, the whole turns dropped): in 32 bits a position of 10^6 has
 // lost a twentieth of a radian.  The sine and cosine of the remaining fraction are taken in 32 bits where the outputs have
 // 16 (error 2^-22, a rounding of the output is 2^-9) and in 64 where they have 32.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -33,7 +35,7 @@ struct NormRotaryParams {
   HeadTensor t[2];              // queries, keys
   const int* pos;               // (M)
   const double* freqs;          // (rot / 2) radians per position
-  float amplitude, eps;
+  float amplitude, eps, inv_d;  // inv_d: 1 / D
   long long M;
   int D, rot, lp, hsplit;       // lanes per head; parts a row's steps are split into
   float* dw_part;               // backward: (blocks, 2, D) or null
@@ -104,6 +106,21 @@ struct Lane {
   static __device__ __forceinline__ int hi(int e) { return INTERLEAVED ? 2 * e + 1 : N + e; }
 };
 
+// sine and cosine of t turns, |t| <= 1/2: the nearest quarter turn dropped, Taylor sums to x^9 / x^8 on |x| <= pi / 4 (the
+// next terms are below 2^-25), the quarter put back by exchange and signs.  Half the instructions of a general routine, which
+// were a third of the kernel at 16 heads of 64.
+__device__ __forceinline__ void turn_sincos(float t, float& s, float& c) {
+  const float k = rintf(4.f * t), x = (t - 0.25f * k) * 6.283185307179586f, y = x * x;
+  const float sn = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -1.6666667e-1f), 1.f);
+  const float cs = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 2.4801587e-5f, -1.3888889e-3f), 4.1666667e-2f), -0.5f), 1.f);
+  const int q = (int)k;
+  const bool odd = q & 1;
+  s = odd ? cs : sn;
+  c = odd ? sn : cs;
+  if (q & 2) s = -s;
+  if ((q + 1) & 2) c = -c;
+}
+
 template <typename T>
 __device__ __forceinline__ void cos_sin(int pos, const double* turns_per_pos, float amplitude, bool turns, float* c, float* s) {
   constexpr int N = V16<T>::N;
@@ -112,7 +129,7 @@ __device__ __forceinline__ void cos_sin(int pos, const double* turns_per_pos, fl
     double t = (double)pos * turns_per_pos[e];
     t -= rint(t);
     if constexpr (sizeof(T) == 2) {
-      sincospif(2.0f * (float)t, &s[e], &c[e]);
+      turn_sincos((float)t, s[e], c[e]);
     } else {
       double sd, cd;
       sincospi(2.0 * t, &sd, &cd);
@@ -159,7 +176,7 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
   double freq[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) freq[e] = at.turns ? p.freqs[at.pair0 + e] * INV_2PI : 0.0;
-  float w[2][2 * N];
+  float w[2][2 * N] = {};
   if constexpr (NORM) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -173,8 +190,13 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
   const int part = (total + p.hsplit - 1) / p.hsplit;
   const long long items = p.M * p.hsplit, stride = (long long)gridDim.x * 4;
   for (long long item = (long long)blockIdx.x * 4 + wave; item < items; item += stride) {
-    const long long row = item / p.hsplit;
-    const int s0 = (int)(item % p.hsplit) * part, s1 = min(s0 + part, total);
+    long long row = item;
+    int s0 = 0, s1 = total;
+    if (p.hsplit > 1) {   // (few rows then: 32 bits do)
+      row = (int)item / p.hsplit;
+      s0 = ((int)item % p.hsplit) * part;
+      s1 = min(s0 + part, total);
+    }
     const int pos = p.pos[row];
     long long page_row = -1;   // PAGED: element offset of the row's slot in a page of one head (without the head's part)
     bool pad = false;
@@ -222,31 +244,36 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
           }
           continue;
         }
-        const int i = st < nq ? 0 : 1;
-        const int h = (st - (i ? nq : 0)) * hpw + slot;
-        float x[2 * N];
-        V16<T>::to_f32(ra[u], x);
-        V16<T>::to_f32(rb[u], x + N);
-        if constexpr (NORM) {
-          float q = 0.f;
+        // (one body per tensor: a choice of weights inside one costs a select per value)
+        auto head = [&](auto which, const float (&wt)[2 * N]) __attribute__((always_inline)) {
+          constexpr int i = decltype(which)::value;
+          const int h = (st - (i ? nq : 0)) * hpw + slot;
+          float x[2 * N];
+          V16<T>::to_f32(ra[u], x);
+          V16<T>::to_f32(rb[u], x + N);
+          if constexpr (NORM) {
+            float q = 0.f;
 #pragma unroll
-          for (int e = 0; e < 2 * N; ++e) q += x[e] * x[e];
-          const float r = rsqrtf(head_sum(at.active ? q : 0.f, lp) / (float)p.D + p.eps);
+            for (int e = 0; e < 2 * N; ++e) q += x[e] * x[e];
+            const float r = rsqrtf(head_sum(at.active ? q : 0.f, lp) * p.inv_d + p.eps);
 #pragma unroll
-          for (int e = 0; e < 2 * N; ++e) x[e] *= r * (i ? w[1][e] : w[0][e]);
-        }
-        turn<T, INTERLEAVED>(x, c, s);
-        if (!at.active || h >= p.t[i].H) continue;
-        T* o;
-        if (PAGED && i == 1) {
-          if (page_row < 0) continue;
-          o = (T*)p.k_pages + page_row + (((long long)h * p.D) << p.page_shift);
-        } else {
-          o = (T*)p.t[i].out + (row * p.t[i].H + h) * p.D;
-        }
-        const bool z = PAGED && pad;
-        *(u32x4*)(o + at.a) = z ? u32x4{0u, 0u, 0u, 0u} : V16<T>::from_f32(x);
-        *(u32x4*)(o + at.b) = z ? u32x4{0u, 0u, 0u, 0u} : V16<T>::from_f32(x + N);
+            for (int e = 0; e < 2 * N; ++e) x[e] *= r * wt[e];
+          }
+          turn<T, INTERLEAVED>(x, c, s);
+          if (!at.active || h >= p.t[i].H) return;
+          T* o;
+          if (PAGED && i == 1) {
+            if (page_row < 0) return;
+            o = (T*)p.k_pages + page_row + (((long long)h * p.D) << p.page_shift);
+          } else {
+            o = (T*)p.t[i].out + (row * p.t[i].H + h) * p.D;
+          }
+          const bool z = PAGED && pad;
+          *(u32x4*)(o + at.a) = z ? u32x4{0u, 0u, 0u, 0u} : V16<T>::from_f32(x);
+          *(u32x4*)(o + at.b) = z ? u32x4{0u, 0u, 0u, 0u} : V16<T>::from_f32(x + N);
+        };
+        if (st < nq) head(std::integral_constant<int, 0>(), w[0]);
+        else head(std::integral_constant<int, 1>(), w[1]);
       }
     }
   }
@@ -265,7 +292,7 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(NormRotaryParams p
   double freq[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) freq[e] = at.turns ? p.freqs[at.pair0 + e] * INV_2PI : 0.0;
-  float w[2][2 * N], dw[2][2 * N];
+  float w[2][2 * N] = {}, dw[2][2 * N] = {};
   if constexpr (NORM) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -280,8 +307,13 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(NormRotaryParams p
   const int part = (total + p.hsplit - 1) / p.hsplit;
   const long long items = p.M * p.hsplit, stride = (long long)gridDim.x * 4;
   for (long long item = (long long)blockIdx.x * 4 + wave; item < items; item += stride) {
-    const long long row = item / p.hsplit;
-    const int s0 = (int)(item % p.hsplit) * part, s1 = min(s0 + part, total);
+    long long row = item;
+    int s0 = 0, s1 = total;
+    if (p.hsplit > 1) {   // (few rows then: 32 bits do)
+      row = (int)item / p.hsplit;
+      s0 = ((int)item % p.hsplit) * part;
+      s1 = min(s0 + part, total);
+    }
     float c[N], s[N];
     cos_sin<T>(p.pos[row], freq, p.amplitude, at.turns, c, s);
     for (int st0 = s0; st0 < s1; st0 += U) {
@@ -304,38 +336,40 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(NormRotaryParams p
       for (int u = 0; u < U; ++u) {
         const int st = st0 + u;
         if (st >= s1) break;
-        const int i = st < nq ? 0 : 1;
-        const int h = (st - (i ? nq : 0)) * hpw + slot;
-        const bool mine = at.active && h < p.t[i].H;
-        float g[2 * N];
-        V16<T>::to_f32(ga[u], g);
-        V16<T>::to_f32(gb[u], g + N);
-        turn_back<T, INTERLEAVED>(g, c, s);
-        if constexpr (NORM) {
-          float x[2 * N], q = 0.f;
-          V16<T>::to_f32(ra[u], x);
-          V16<T>::to_f32(rb[u], x + N);
+        auto head = [&](auto which, const float (&wt)[2 * N], float (&dwt)[2 * N]) __attribute__((always_inline)) {
+          constexpr int i = decltype(which)::value;
+          const int h = (st - (i ? nq : 0)) * hpw + slot;
+          const bool mine = at.active && h < p.t[i].H;
+          float g[2 * N];
+          V16<T>::to_f32(ga[u], g);
+          V16<T>::to_f32(gb[u], g + N);
+          turn_back<T, INTERLEAVED>(g, c, s);
+          if constexpr (NORM) {
+            float x[2 * N], q = 0.f;
+            V16<T>::to_f32(ra[u], x);
+            V16<T>::to_f32(rb[u], x + N);
 #pragma unroll
-          for (int e = 0; e < 2 * N; ++e) q += x[e] * x[e];
-          const float r = rsqrtf(head_sum(at.active ? q : 0.f, lp) / (float)p.D + p.eps);
-          float m = 0.f;
+            for (int e = 0; e < 2 * N; ++e) q += x[e] * x[e];
+            const float r = rsqrtf(head_sum(at.active ? q : 0.f, lp) * p.inv_d + p.eps);
+            float m = 0.f;
 #pragma unroll
-          for (int e = 0; e < 2 * N; ++e) {
-            x[e] *= r;
-            const float d = mine ? g[e] * x[e] : 0.f;
-            if (i) dw[1][e] += d;
-            else dw[0][e] += d;
-            g[e] *= i ? w[1][e] : w[0][e];
-            m += g[e] * x[e];
+            for (int e = 0; e < 2 * N; ++e) {
+              x[e] *= r;
+              dwt[e] += mine ? g[e] * x[e] : 0.f;
+              g[e] *= wt[e];
+              m += g[e] * x[e];
+            }
+            m = head_sum(at.active ? m : 0.f, lp) * p.inv_d;
+#pragma unroll
+            for (int e = 0; e < 2 * N; ++e) g[e] = r * (g[e] - x[e] * m);
           }
-          m = head_sum(at.active ? m : 0.f, lp) / (float)p.D;
-#pragma unroll
-          for (int e = 0; e < 2 * N; ++e) g[e] = r * (g[e] - x[e] * m);
-        }
-        if (!mine) continue;
-        T* o = (T*)p.t[i].out + (row * p.t[i].H + h) * p.D;
-        *(u32x4*)(o + at.a) = V16<T>::from_f32(g);
-        *(u32x4*)(o + at.b) = V16<T>::from_f32(g + N);
+          if (!mine) return;
+          T* o = (T*)p.t[i].out + (row * p.t[i].H + h) * p.D;
+          *(u32x4*)(o + at.a) = V16<T>::from_f32(g);
+          *(u32x4*)(o + at.b) = V16<T>::from_f32(g + N);
+        };
+        if (st < nq) head(std::integral_constant<int, 0>(), w[0], dw[0]);
+        else head(std::integral_constant<int, 1>(), w[1], dw[1]);
       }
     }
   }
@@ -391,6 +425,7 @@ int check_common(const NormRotaryParams& p, int dtype) {
 // the row's sines again): about 2 waves per SIMD of the 256 CUs.
 void plan(NormRotaryParams& p, int dtype, int steps_extra) {
   p.lp = lanes_per_head(p.D, dtype);
+  p.inv_d = 1.f / (float)p.D;
   const int hpw = 64 / p.lp;
   for (int i = 0; i < 2; ++i) p.t[i].steps = (p.t[i].H + hpw - 1) / hpw;
   const int total = p.t[0].steps + p.t[1].steps + (steps_extra ? p.t[1].steps : 0);

@@ -912,12 +912,25 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
     ks_.store(lds[0][0]);
     vs_.store(lds[0][1]);
     __syncthreads();
+    // laid out by hand: with each matrix instruction goes the read of a later fragment (hipcc reads it right in front
+    // of the product that waits for it), as far ahead as the registers reach; the first of K^T are in flight under the probabilities
+    constexpr int NP = 2 * L::NKS, NM = NP + 2 * L::DB, AHEAD = D == 64 ? 5 : 2;
     auto half = [&](int k0, const char* kt, const char* vt, int i) __attribute__((always_inline)) {
-      f32x16 s = zero16(), dp = zero16();
+      auto fragment = [&](int x) __attribute__((always_inline)) -> u32x4 {
+        if (x < NP) return L::rows_t(x & 1 ? vt : kt, i, x >> 1, lane);
+        return L::cols(kt, 2 * i + (x - NP) / L::DB, (x - NP) % L::DB, lane);
+      };
+      u32x4 f[NM];
 #pragma unroll
-      for (int ks = 0; ks < L::NKS; ++ks) {
-        s = MELGPT_MFMA_32x32x16(L::rows_t(kt, i, ks, lane), qf[ks], s);
-        dp = MELGPT_MFMA_32x32x16(L::rows_t(vt, i, ks, lane), gf[ks], dp);
+      for (int x = 0; x < AHEAD; ++x) f[x] = fragment(x);
+      f32x16 s = zero16(), dp = zero16();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < NP; ++x) {
+        if (x + AHEAD < NM) f[x + AHEAD] = fragment(x + AHEAD);
+        if (x & 1) dp = MELGPT_MFMA_32x32x16(f[x], gf[x >> 1], dp);
+        else s = MELGPT_MFMA_32x32x16(f[x], qf[x >> 1], s);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2)) * (dp[r] - dl);
@@ -926,11 +939,13 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < lim ? s[r] : 0.f;
       }
+      const u32x4 sf[2] = {operand16(s, 0), operand16(s, 1)};
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const u32x4 sf = operand16(s, e);
-#pragma unroll
-        for (int d = 0; d < L::DB; ++d) dq[d] = MELGPT_MFMA_32x32x16(L::cols(kt, 2 * i + e, d, lane), sf, dq[d]);
+      for (int x = NP; x < NM; ++x) {
+        if (x + AHEAD < NM) f[x + AHEAD] = fragment(x + AHEAD);
+        dq[(x - NP) % L::DB] = MELGPT_MFMA_32x32x16(f[x], sf[(x - NP) / L::DB], dq[(x - NP) % L::DB]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
     auto tile = [&](int k0, auto par) __attribute__((always_inline)) {
