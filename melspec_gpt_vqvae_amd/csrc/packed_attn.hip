@@ -407,13 +407,13 @@ __device__ __forceinline__ u32x4 operand16(const f32x16& s, int st) {
                pack_bf16x2(s[8 * st + 4], s[8 * st + 5]), pack_bf16x2(s[8 * st + 6], s[8 * st + 7])};
 }
 
-// 64 rows through registers into LDS (256 threads), by buffer loads: the uniform parts of an address cost no vector
+// 64 rows through registers into LDS (NT threads), by buffer loads: the uniform parts of an address cost no vector
 // instruction (a row's 64-bit product per load cost as much as the softmax), and rows behind the last read as zeros (their
 // scores are masked, but 0 * NaN is not 0).
-template <int D, bool TR>   // TR: laid out for transposed reads
+template <int D, bool TR, int NT = 256>   // TR: laid out for transposed reads
 struct Stage64 {
   using L = Tile32<D>;
-  static constexpr int PER = 64 * L::CP / 256, STEP = 64 / PER;
+  static constexpr int PER = 64 * L::CP / NT, STEP = 64 / PER;
   const bf16_t* base;
   long long rs;        // row stride, D <= rs (rows do not overlap: the end of the last row bounds them all)
   unsigned from;       // this thread's first chunk, bytes from a tile's first row
@@ -979,21 +979,27 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
       store4<T>(out + 32 * d + 8 * j + 4 * hh, f32x4{dq[d][4 * j], dq[d][4 * j + 1], dq[d][4 * j + 2], dq[d][4 * j + 3]} * p.scale);
 }
 
-// dk and dv: 64 keys of one key head; wave (kb, qh) owns keys 32 kb .. + 31, in registers, and of each 64 queries that see
-// them, of each of the G heads, the 32 of half qh; the two halves are added at the end, in LDS.  One wave per SIMD: the
-// keys, the values and both gradients fill half of its 512 registers (the accumulators and operands that only matrix
-// instructions touch are kept in the other half of the file), and what hides its latencies is its own next block: a step
-// forms the next block's products with k and v and adds the previous block's gradients while this block's probabilities
-// are computed.  Four blocks of queries lie in LDS: previous, this, next, and the one being stored.
+// dk and dv: 64 keys of one key head, 512 threads.  Pair (kb, qh) of waves owns keys 32 kb .. + 31, in registers, and of each
+// 64 queries that see them, of each of the G heads, the 32 of half qh.  The two waves of a pair, on one SIMD, share a block's
+// work so that each holds only one gradient (64 + 32 registers at 128 values a head instead of 128 + 64: two waves per SIMD
+// fit) and one multiplies while the other computes:
+//   wave A, block n:  scores of block n and dv of block n - 1, then the probabilities of block n, left in LDS for B
+//   wave B, block n:  ds of block n - 1 from A's probabilities, then do . v of block n and dk of block n - 1
+// one barrier a block.  Three tiles of queries and output gradients lie in LDS (the last, this one, the one being stored).
+// The halves qh are added at the end, in LDS.  (One wave for both gradients, one to a SIMD, took 386 us where this takes less:
+// it issues every instruction of a block itself, and 400 of them need longer than its 32 products.)
 template <int D>
-__global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
+__global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   using L = Tile32<D>;
   using T = bf16_t;
+  using St = Stage64<D, true, 512>;
   constexpr int TB = 64 * L::RB;                                   // bytes of a tile: slot i: q at 2 i TB, dout behind it
-  __shared__ __attribute__((aligned(16))) char tiles_[8 * TB];
-  __shared__ __attribute__((aligned(16))) float stat[4 * 128];     // [slot][lse, delta][64]
+  __shared__ __attribute__((aligned(16))) char tiles_[6 * TB];
+  __shared__ __attribute__((aligned(16))) float prob[3][4][4][64][4];   // [slot][pair][accumulators 4 j ..][lane]
+  __shared__ __attribute__((aligned(16))) float stat[3 * 128];     // [slot][lse, delta][64]
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
-  const int kb = wave & 1, qh = wave >> 1;
+  const int pair = wave & 3, kb = pair & 1, qh = pair >> 1;
+  const bool second = wave >= 4;                                   // wave B
   const int hk = blockIdx.x;
   const Rows R = find_rows<64, false>(p.cu_k, p.S, p.Mk, blockIdx.y, lane);
   if (!R.any) return;
@@ -1006,31 +1012,26 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
   // query i sees key j <= i + nk - nq: the queries from j - (nk - nq) on; all of the wave's keys from `full` on
   const int from = max(k_in - (nk - nq), 0), full = max(w0 + 31 - (nk - nq), 0);
   const int first = max(64 * R.tile - (nk - nq), 0) & ~63;
-  const T* kp = (const T*)p.k + row * p.k_row + hk * p.k_head;
-  const T* vp = (const T*)p.v + row * p.v_row + hk * p.v_head;
-  u32x4 kf[L::NKS], vf[L::NKS];
-  // masked scores are -inf before the scale: its sign goes into the keys, a zero scale makes them zero (as in the forward)
-  const unsigned flip = p.scale < 0.f ? 0x80008000u : 0u, keep = p.scale == 0.f ? 0u : 0xffffffffu;
+  // A: keys, B: values.  Masked scores are -inf before the scale: its sign goes into the keys, a zero scale makes them zero
+  // (as in the forward)
+  u32x4 kv[L::NKS];
+  const T* kvp = second ? (const T*)p.v + row * p.v_row + hk * p.v_head : (const T*)p.k + row * p.k_row + hk * p.k_head;
+  const unsigned flip = !second && p.scale < 0.f ? 0x80008000u : 0u, keep = !second && p.scale == 0.f ? 0u : 0xffffffffu;
 #pragma unroll
   for (int ks = 0; ks < L::NKS; ++ks) {
-    kf[ks] = *(const u32x4*)(kp + 16 * ks + 8 * hh);
-    vf[ks] = *(const u32x4*)(vp + 16 * ks + 8 * hh);
+    kv[ks] = *(const u32x4*)(kvp + 16 * ks + 8 * hh);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) kf[ks][e] = (kf[ks][e] ^ flip) & keep;
+    for (int e = 0; e < 4; ++e) kv[ks][e] = (kv[ks][e] ^ flip) & keep;
   }
   const float c2 = p.scale == 0.f ? 1.f : fabsf(p.scale) * LOG2E;
-  f32x16 dk[L::DB], dv[L::DB];
+  f32x16 grad[L::DB];                                              // A: dv, B: dk
 #pragma unroll
-  for (int d = 0; d < L::DB; ++d) {
-    dk[d] = zero16();
-    dv[d] = zero16();
-  }
+  for (int d = 0; d < L::DB; ++d) grad[d] = zero16();
   const int blocks = first < nq ? (nq - first + 63) / 64 : 0, total = blocks * p.G;
   if (total > 0) {
     // Tiles in order: head by head, the queries from the last down.  Addresses and sizes of the tile to load next are kept as
-    // running scalars: one wave per SIMD issues everything itself, and a tile's 64-bit products were a quarter of a step.
-    // Wave parity picks the row of statistics (lse, delta) a wave fetches; both waves of a parity store the same.
-    Stage64<D, true> qs_((const T*)p.q, p.q_row, t), gs_((const T*)p.dout, p.do_row, t);
+    // running scalars.  Wave parity picks the row of statistics (lse, delta) a wave fetches; waves of a parity store the same.
+    St qs_((const T*)p.q, p.q_row, t), gs_((const T*)p.dout, p.do_row, t);
     const int top = first + 64 * (blocks - 1), st_row = wave & 1;
     const long long q_at = (long long)(q_lo + top) * p.q_row + (long long)hk * p.G * p.q_head;
     const long long g_at = (long long)(q_lo + top) * p.do_row + (long long)hk * p.G * p.do_head;
@@ -1044,7 +1045,17 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
     const float s_mul = st_row ? 1.f : LOG2E;
     int lq = top, left = total;                                    // first query of the tile to load next, tiles left
     float sv = 0.f;
-    auto next = [&]() __attribute__((always_inline)) {
+    auto load = [&]() __attribute__((always_inline)) {             // (no tile left: zeros)
+      const bool any = left > 0, part = lq == top;
+      const __amdgpu_buffer_rsrc_t rq = make_rsrc(qa, !any ? 0u : part ? q_rest : q_full);
+      const __amdgpu_buffer_rsrc_t rg = make_rsrc(ga, !any ? 0u : part ? g_rest : g_full);
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(sa, !any ? 0u : part ? 4u * rest : 256u);
+#pragma unroll
+      for (int i = 0; i < St::PER; ++i) {
+        qs_.load1(rq, i);
+        gs_.load1(rg, i);
+      }
+      sv = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4u * lane, 0, 0));
       const bool wrap = lq == first;
       qa += wrap ? q_next : -q_down;
       ga += wrap ? g_next : -g_down;
@@ -1052,185 +1063,142 @@ __global__ __launch_bounds__(256, 1) void packed_dkv32_kernel(PackedParams p) {
       lq = wrap ? top : lq - 64;
       --left;
     };
-    auto q_tile = [&]() __attribute__((always_inline)) { return make_rsrc(qa, left <= 0 ? 0u : lq == top ? q_rest : q_full); };
-    auto g_tile = [&]() __attribute__((always_inline)) { return make_rsrc(ga, left <= 0 ? 0u : lq == top ? g_rest : g_full); };
-    auto load_stat = [&]() __attribute__((always_inline)) {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(sa, left <= 0 ? 0u : lq == top ? 4u * rest : 256u);
-      const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4u * lane, 0, 0)) * s_mul;
-      // a query that sees no key has lse -inf; +inf makes its probabilities 0 instead of NaN
-      sv = !st_row && x == -__builtin_inff() ? __builtin_inff() : x;
-    };
-    auto load = [&]() __attribute__((always_inline)) {
-      const __amdgpu_buffer_rsrc_t rq = q_tile(), rg = g_tile();
-#pragma unroll
-      for (int i = 0; i < Stage64<D, true>::PER; ++i) {
-        qs_.load1(rq, i);
-        gs_.load1(rg, i);
-      }
-      load_stat();
-      next();
-    };
     auto store = [&](int slot) __attribute__((always_inline)) {
       qs_.store(tiles_ + 2 * slot * TB);
       gs_.store(tiles_ + (2 * slot + 1) * TB);
-      stat[128 * slot + 64 * st_row + lane] = sv;
+      // a query that sees no key has lse -inf; +inf makes its probabilities 0 instead of NaN
+      stat[128 * slot + 64 * st_row + lane] = !st_row && sv == -__builtin_inff() ? __builtin_inff() : sv * s_mul;
     };
-    // The matrix instructions of a step, in order: the products of one block (2 NKS), the gradients of another (4 DB); with
-    // each, the fragment of tile rows or columns it takes
-    constexpr int NP = 2 * L::NKS, NM = NP + 4 * L::DB;
-    auto fragment = [&](int i, int prod, int grad) __attribute__((always_inline)) -> u32x4 {
-      if (i < NP) return L::rows_t(tiles_ + (2 * prod + (i & 1)) * TB, qh, i >> 1, lane);
-      const int j = i - NP;
-      return L::cols(tiles_ + (2 * grad + ((j & 1) ^ 1)) * TB, 2 * qh + j / (2 * L::DB), (j >> 1) % L::DB, lane);
-    };
-    auto multiply = [&](int i, const u32x4& f, f32x16& s, f32x16& dp, const u32x4 (&pf)[2], const u32x4 (&sf)[2]) __attribute__((always_inline)) {
-      if (i < NP) {
-        if (i & 1) dp = MELGPT_MFMA_32x32x16(f, vf[i >> 1], dp);
-        else s = MELGPT_MFMA_32x32x16(f, kf[i >> 1], s);
-      } else {
-        const int j = i - NP, e = j / (2 * L::DB), d = (j >> 1) % L::DB;
-        if (j & 1) dk[d] = MELGPT_MFMA_32x32x16(f, sf[e], dk[d]);
-        else dv[d] = MELGPT_MFMA_32x32x16(f, pf[e], dv[d]);
+    // slot 2 stands for the block before the first: zeros (what they multiply is zero too, but 0 * NaN is not)
+#pragma unroll
+    for (int i = 0; i < 2 * TB / (512 * 16); ++i) *(u32x4*)(tiles_ + 4 * TB + (t + 512 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *(u32x4*)((char*)&prob[2] + (t + 512 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
+    if (t < 128) stat[256 + t] = 0.f;
+    load();
+    store(0);
+    load();
+    __syncthreads();
+    int q0 = top + 32 * qh;                                        // this wave's queries of the current tile
+    f32x16 acc = zero16();                                         // A: scores, B: do . v
+    u32x4 w[2] = {u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}};   // A: probabilities, B: ds, as operands
+    // The matrix instructions of a block, alternating: product i with the keys (or values) of tile rows, gradient i from tile
+    // columns; laid out by hand, the fragment of the one four later read with each (hipcc reads it in front of its product)
+    constexpr int NP = L::NKS, NM = NP + 2 * L::DB, AHEAD = 4;
+    auto multiply = [&](auto slot_) __attribute__((always_inline)) {
+      constexpr int SL = decltype(slot_)::value, PV = (SL + 2) % 3;
+      // A: q rows of this tile, dout columns of the last; B: dout rows of this, q columns of the last
+      const char* rows = tiles_ + (second ? (2 * SL + 1) * TB : 2 * SL * TB);
+      const char* cols = tiles_ + (second ? 2 * PV * TB : (2 * PV + 1) * TB);
+      static_assert(NP == 2 * L::DB, "one gradient instruction to a product");
+      auto fragment = [&](int i) __attribute__((always_inline)) -> u32x4 {
+        if (i & 1) return L::cols(cols, 2 * qh + (i >> 1) / L::DB, (i >> 1) % L::DB, lane);
+        return L::rows_t(rows, qh, i >> 1, lane);
+      };
+      u32x4 f[NM];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i);
+      acc = zero16();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        if (i + AHEAD < NM) f[i + AHEAD] = fragment(i + AHEAD);
+        if (i & 1) grad[(i >> 1) % L::DB] = MELGPT_MFMA_32x32x16(f[i], w[(i >> 1) / L::DB], grad[(i >> 1) % L::DB]);
+        else acc = MELGPT_MFMA_32x32x16(f[i], kv[i >> 1], acc);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
-    u32x4 pf[2][2], sf[2][2];                                      // probabilities and ds of this and the previous block
-#pragma unroll
-    for (int i = 0; i < 2; ++i) pf[1][i] = sf[1][i] = u32x4{0u, 0u, 0u, 0u};
-    f32x16 s[2], dp[2];
-    int q0 = top + 32 * qh;                                        // this wave's queries of the current tile
-    auto step = [&](auto slot_) __attribute__((always_inline)) {
-      constexpr int SL = decltype(slot_)::value, A = SL & 1, B = A ^ 1;
+    auto probabilities = [&](auto slot_) __attribute__((always_inline)) {   // of this block (A)
+      constexpr int SL = decltype(slot_)::value;
       if (q0 < full || q0 + 32 > nq) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int q = q0 + 8 * (r >> 2) + 4 * hh + (r & 3);
-          const bool in = q >= from && q < nq;
-          s[A][r] = in ? s[A][r] : -__builtin_inff();
-          dp[A][r] = in ? dp[A][r] : 0.f;
+          acc[r] = q >= from && q < nq ? acc[r] : -__builtin_inff();
         }
       }
-      s[B] = zero16();
-      dp[B] = zero16();
-      f32x4 ls[4], de[4];                                          // accumulators 4 j .. + 3: queries 8 j + 4 hh .. + 3
-      auto stats = [&](int j) __attribute__((always_inline)) {
-        ls[j] = *(const f32x4*)&stat[128 * SL + 32 * qh + 8 * j + 4 * hh];
-        de[j] = *(const f32x4*)&stat[128 * SL + 64 + 32 * qh + 8 * j + 4 * hh];
-      };
-      stats(0);
-      const __amdgpu_buffer_rsrc_t rq = q_tile(), rg = g_tile();
-      // laid out by hand: hipcc on its own reads every fragment right in front of the product that waits for it.  With each
-      // matrix instruction go the read of the fragment four later, its share of the probabilities, and (in the last part) the
-      // stores of the tile loaded during the step before, each followed by the load that refills its registers
-      constexpr int AHEAD = 4, PER = Stage64<D, true>::PER;
-      u32x4 f[NM];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i, (SL + 1) & 3, (SL + 3) & 3);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < 4; ++j) {                                // accumulators 4 j .. + 3: queries 8 j + 4 hh .. + 3
+        const f32x4 ls = *(const f32x4*)&stat[128 * SL + 32 * qh + 8 * j + 4 * hh];
+        f32x4 pr;
 #pragma unroll
-      for (int i = 0; i < NM; ++i) {
-        if (i + AHEAD < NM) f[i + AHEAD] = fragment(i + AHEAD, (SL + 1) & 3, (SL + 3) & 3);
-        multiply(i, f[i], s[B], dp[B], pf[B], sf[B]);
-#pragma unroll
-        for (int r = 16 * i / NM; r < 16 * (i + 1) / NM; ++r) {
-          if ((r & 3) == 0 && r < 12) stats(r / 4 + 1);
-          s[A][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[A][r], c2, -ls[r >> 2][r & 3]));
-          dp[A][r] = s[A][r] * (dp[A][r] - de[r >> 2][r & 3]);
-          if ((r & 7) == 7) {
-            pf[A][r >> 3] = operand16(s[A], r >> 3);
-            sf[A][r >> 3] = operand16(dp[A], r >> 3);
-          }
+        for (int r = 0; r < 4; ++r) {
+          pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * j + r], c2, -ls[r]));
+          acc[4 * j + r] = pr[r];
         }
-        const int c = i - (NM - 2 * PER - 1);                      // (2 PER chunks in the last 2 PER places but one)
-        if (c >= 0 && c < 2 * PER) {
-          if (c & 1) {
-            gs_.store1(tiles_ + (2 * ((SL + 2) & 3) + 1) * TB, c >> 1);
-            gs_.load1(rg, c >> 1);
-          } else {
-            qs_.store1(tiles_ + 2 * ((SL + 2) & 3) * TB, c >> 1);
-            qs_.load1(rq, c >> 1);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        *(f32x4*)&prob[SL][pair][j][lane][0] = pr;
       }
+      w[0] = operand16(acc, 0);
+      w[1] = operand16(acc, 1);
+    };
+    auto score_gradients = [&](auto slot_) __attribute__((always_inline)) {   // of the block in slot_ (B)
+      constexpr int SL = decltype(slot_)::value;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) asm volatile("" : "+v"(pf[A][e]), "+v"(sf[A][e]));
-      // (only matrix instructions touch these in the loop: the half of the register file that is theirs)
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 de = *(const f32x4*)&stat[128 * SL + 64 + 32 * qh + 8 * j + 4 * hh];
+        const f32x4 pr = *(const f32x4*)&prob[SL][pair][j][lane][0];
 #pragma unroll
-      for (int d = 0; d < L::DB; ++d) asm volatile("" : "+a"(dk[d]), "+a"(dv[d]));
-#pragma unroll
-      for (int ks = 0; ks < L::NKS; ++ks) asm volatile("" : "+a"(kf[ks]), "+a"(vf[ks]));
-      stat[128 * ((SL + 2) & 3) + 64 * st_row + lane] = sv;
-      load_stat();
-      next();
+        for (int r = 0; r < 4; ++r) acc[4 * j + r] = pr[r] * (acc[4 * j + r] - de[r]);
+      }
+      w[0] = operand16(acc, 0);
+      w[1] = operand16(acc, 1);
+    };
+    auto block = [&](auto slot_) __attribute__((always_inline)) {
+      constexpr int SL = decltype(slot_)::value;
+      if (second) score_gradients(std::integral_constant<int, (SL + 2) % 3>());
+      multiply(slot_);
+      store((SL + 1) % 3);
+      load();
+      if (!second) probabilities(slot_);
       q0 -= 64;
       if (q0 < first) q0 = top + 32 * qh;
       __syncthreads();
     };
-    // slot 3 stands for the block before the first: zeros (its probabilities are zero too, but 0 * NaN is not)
-#pragma unroll
-    for (int i = 0; i < 2 * TB / (256 * 16); ++i) *(u32x4*)(tiles_ + 6 * TB + (t + 256 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
-    load();
-    store(0);
-    load();
-    store(1);
-    load();
-    __syncthreads();
-    s[0] = zero16();
-    dp[0] = zero16();
-#pragma unroll
-    for (int i = 0; i < NP; ++i) multiply(i, fragment(i, 0, 0), s[0], dp[0], pf[1], sf[1]);
-    int n = 0;
-    for (; n + 4 <= total; n += 4) {
-      step(std::integral_constant<int, 0>());
-      step(std::integral_constant<int, 1>());
-      step(std::integral_constant<int, 2>());
-      step(std::integral_constant<int, 3>());
-    }
-    if (n < total) step(std::integral_constant<int, 0>());
-    if (n + 1 < total) step(std::integral_constant<int, 1>());
-    if (n + 2 < total) step(std::integral_constant<int, 2>());
-    auto last = [&](auto slot_) __attribute__((always_inline)) {   // the last block's gradients
+    auto last = [&](auto slot_) __attribute__((always_inline)) {   // what the last block still owes
       constexpr int SL = decltype(slot_)::value;
+      if (second) score_gradients(slot_);
+      const char* cols = tiles_ + (second ? 2 * SL * TB : (2 * SL + 1) * TB);
 #pragma unroll
-      for (int i = NP; i < NM; ++i) multiply(i, fragment(i, SL, SL), s[0], dp[0], pf[SL & 1], sf[SL & 1]);
+      for (int i = 0; i < 2 * L::DB; ++i)
+        grad[i % L::DB] = MELGPT_MFMA_32x32x16(L::cols(cols, 2 * qh + i / L::DB, i % L::DB, lane), w[i / L::DB], grad[i % L::DB]);
     };
-    switch ((total - 1) & 3) {
-      case 0: last(std::integral_constant<int, 0>()); break;
-      case 1: last(std::integral_constant<int, 1>()); break;
-      case 2: last(std::integral_constant<int, 2>()); break;
-      default: last(std::integral_constant<int, 3>());
+    int n = 0;
+    for (; n + 3 <= total; n += 3) {
+      block(std::integral_constant<int, 0>());
+      block(std::integral_constant<int, 1>());
+      block(std::integral_constant<int, 2>());
+    }
+    if (n < total) block(std::integral_constant<int, 0>());
+    if (n + 1 < total) block(std::integral_constant<int, 1>());
+    switch (total % 3) {
+      case 1: last(std::integral_constant<int, 0>()); break;
+      case 2: last(std::integral_constant<int, 1>()); break;
+      default: last(std::integral_constant<int, 2>());
     }
     __syncthreads();
   }
-  // the halves: wave (kb, 1) hands over dk, then dv, through LDS (32 keys x D f32 each: the tiles' room)
-  T* ok = (T*)p.dk + row * p.dk_row + hk * p.dk_head;
-  T* ov = (T*)p.dv + row * p.dv_row + hk * p.dv_head;
-  float* room = (float*)tiles_ + kb * (32 * D);
-  auto join = [&](f32x16 (&a)[L::DB], T* out, float f) __attribute__((always_inline)) {
-    if (qh == 1) {
+  // the halves: waves of qh 1 hand over their 32 keys x D sums through LDS
+  float* room = (float*)tiles_ + (2 * (int)second + kb) * (32 * D);
+  static_assert(4 * 32 * D * 4 <= 6 * TB, "the tiles' room holds the sums");
+  if (qh == 1) {
 #pragma unroll
-      for (int d = 0; d < L::DB; ++d)
+    for (int d = 0; d < L::DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) room[(16 * d + r) * 64 + lane] = a[d][r];
+      for (int r = 0; r < 16; ++r) room[(16 * d + r) * 64 + lane] = grad[d][r];
+  }
+  __syncthreads();
+  if (qh == 1 || k_in >= nk) return;
+  T* out = second ? (T*)p.dk + row * p.dk_row + hk * p.dk_head : (T*)p.dv + row * p.dv_row + hk * p.dv_head;
+  const float f = second ? p.scale : 1.f;
+#pragma unroll
+  for (int d = 0; d < L::DB; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f32x4 x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = (grad[d][4 * j + r] + room[(16 * d + 4 * j + r) * 64 + lane]) * f;
+      store4<T>(out + 32 * d + 8 * j + 4 * hh, x);
     }
-    __syncthreads();
-    if (qh == 0) {
-#pragma unroll
-      for (int d = 0; d < L::DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) a[d][r] = (a[d][r] + room[(16 * d + r) * 64 + lane]) * f;
-      if (k_in < nk) {
-#pragma unroll
-        for (int d = 0; d < L::DB; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            store4<T>(out + 32 * d + 8 * j + 4 * hh, f32x4{a[d][4 * j], a[d][4 * j + 1], a[d][4 * j + 2], a[d][4 * j + 3]});
-      }
-    }
-    __syncthreads();
-  };
-  join(dk, ok, p.scale);
-  join(dv, ov, 1.f);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1279,7 +1247,7 @@ int launch_bwd(const PackedParams& p, hipStream_t s) {
   const dim3 gq(p.Hq, (unsigned)tq), gk(p.Hk, (unsigned)tk);
   if constexpr (sizeof(T) == 2) {
     if (p.Mq > 0) hipLaunchKernelGGL((packed_dq32_kernel<D>), gq, dim3(256), 0, s, p);
-    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv32_kernel<D>), gk, dim3(256), 0, s, p);
+    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv32_kernel<D>), gk, dim3(512), 0, s, p);
   } else {
     if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_kernel<T, D>), gq, dim3(256), 0, s, p);
     if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_kernel<T, D>), gk, dim3(256), 0, s, p);
