@@ -364,15 +364,13 @@ template <int D>
 struct Tile32 {
   static constexpr int RB = 2 * D, CP = RB / 16, NKS = D / 16, DB = D / 32;
   // keys / rows read along D, 32 rows a time
-  static __device__ __forceinline__ int off_r(int row, int c) {
-    if constexpr (RB == 128) return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
-    else return row * RB + ((c ^ (row & 15)) << 4);
-  }
+  static __device__ __forceinline__ int swz_r(int row) { return RB == 128 ? (row >> 1) & 7 : row & 15; }
   // values, read transposed: 8 rows x 64 bytes an instruction, spread over all banks
-  static __device__ __forceinline__ int off_t(int row, int c) {
-    if constexpr (RB == 128) return row * 128 + ((c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3))) << 4);
-    else return row * RB + ((c ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+  static __device__ __forceinline__ int swz_t(int row) {
+    return RB == 128 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
   }
+  static __device__ __forceinline__ int off_r(int row, int c) { return row * RB + ((c ^ swz_r(row)) << 4); }
+  static __device__ __forceinline__ int off_t(int row, int c) { return row * RB + ((c ^ swz_t(row)) << 4); }
   static __device__ __forceinline__ u32x4 rows(const char* t, int blk, int ks, int lane) {
     return *(const u32x4*)(t + off_r(32 * blk + (lane & 31), 2 * ks + (lane >> 5)));
   }
@@ -407,51 +405,63 @@ __device__ __forceinline__ u32x4 operand16(const f32x16& s, int st) {
                pack_bf16x2(s[8 * st + 4], s[8 * st + 5]), pack_bf16x2(s[8 * st + 6], s[8 * st + 7])};
 }
 
-// 64 rows through registers into LDS (NT threads), by buffer loads: the uniform parts of an address cost no vector
-// instruction (a row's 64-bit product per load cost as much as the softmax), and rows behind the last read as zeros (their
-// scores are masked, but 0 * NaN is not 0).
-template <int D, bool TR, int NT = 256>   // TR: laid out for transposed reads
-struct Stage64 {
+// 64 rows straight from memory into LDS (NW waves), 1 KB an instruction: LDS takes 32 bytes a cycle from registers
+// (ds_write_b128: 14 ns a KB on a CU, measured) but gives 240 - a tile's stores took longer than all its reads - and the
+// registers of a tile in flight are free.  An instruction's lanes fill 1 KB of LDS in order, so the swizzle is applied to
+// which chunk a lane fetches.  Rows behind the last are out of the buffer's range and arrive as zeros (their scores are
+// masked, but 0 * NaN is not 0).  (asm: the compiler would hold every LDS read until the builtin's data had arrived; the
+// counterpart is arrive() in front of the barrier.)
+typedef u32x4 buffer_t;
+__device__ __forceinline__ buffer_t make_buffer(const void* base, unsigned bytes) {
+  const unsigned long long a = (unsigned long long)base;
+  return buffer_t{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu),
+                  (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+__device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int D, bool TR, int NW = 4>   // TR: laid out for transposed reads
+struct Fetch64 {
   using L = Tile32<D>;
-  static constexpr int PER = 64 * L::CP / NT, STEP = 64 / PER;
-  const bf16_t* base;
-  long long rs;        // row stride, D <= rs (rows do not overlap: the end of the last row bounds them all)
-  unsigned from;       // this thread's first chunk, bytes from a tile's first row
-  int off;             // its place in LDS (rows STEP apart keep the swizzle: STEP is a multiple of 16)
-  u32x4 a[PER];
-  static_assert(STEP % 16 == 0, "rows of a thread share their swizzle");
-  __device__ __forceinline__ Stage64(const bf16_t* b, long long row_stride, int t) : base(b), rs(row_stride) {
-    const int c = t % L::CP, row = t / L::CP;
+  static constexpr int PER = L::CP / NW, STEP = 64 / PER;   // instructions of a wave, rows between them
+  static_assert(STEP % 16 == 0, "a lane's rows share their swizzle");
+  unsigned from, step;                                      // bytes: this lane's first chunk, its next
+  int at;                                                   // the wave's place in a tile
+  __device__ __forceinline__ Fetch64(long long rs, int wave, int lane) {
+    const int row = (64 / L::CP) * wave + lane / L::CP, c = (lane % L::CP) ^ (TR ? L::swz_t(row) : L::swz_r(row));
     from = 2u * ((unsigned)row * (unsigned)rs + 8u * c);
-    off = TR ? L::off_t(row, c) : L::off_r(row, c);
+    step = 2u * STEP * (unsigned)rs;
+    at = 1024 * wave;
   }
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int row0, int n) const {
+  // rows row0 .. of n (row stride rs) -> tile
+  __device__ __forceinline__ void operator()(char* tile, const bf16_t* base, long long rs, int row0, int n) const {
     const int left = min(max(n - row0, 0), 64);
-    return make_rsrc(base + row0 * rs, left > 0 ? 2u * ((unsigned)(left - 1) * (unsigned)rs + D) : 0u);
+    (*this)(tile, make_buffer(base + row0 * rs, left > 0 ? 2u * ((unsigned)(left - 1) * (unsigned)rs + D) : 0u));
   }
-  __device__ __forceinline__ void load1(__amdgpu_buffer_rsrc_t r, int i) {
-    a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, from, 2u * STEP * i * (unsigned)rs, 0));
-  }
-  __device__ __forceinline__ bool clean() {   // -> whether there were values that are not finite (there are zeros now)
-    bool fine = true;
+  __device__ __forceinline__ void operator()(char* tile, buffer_t b) const {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) fine = fine && finite16<bf16_t>(a[i]);
-    if (fine) return false;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) a[i] = finite_part<bf16_t>(a[i]);
-    return true;
-  }
-  __device__ __forceinline__ void store1(char* t, int i) const { *(u32x4*)(t + off + i * STEP * L::RB) = a[i]; }
-  __device__ __forceinline__ void load(int row0, int n) {
-    const __amdgpu_buffer_rsrc_t r = at(row0, n);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) load1(r, i);
-  }
-  __device__ __forceinline__ void store(char* t) const {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) store1(t, i);
+    for (int i = 0; i < PER; ++i) {
+      const unsigned m0 = (unsigned)(size_t)LDS_PTR(char, tile + at + 1024 * NW * i);
+      asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :
+                   : "s"(m0), "v"(from + i * step), "s"(b)
+                   : "memory", "m0");
+    }
   }
 };
+// zeros in place of values that are not finite in a tile in LDS (256 threads) -> whether this thread found any
+template <int D>
+__device__ __forceinline__ bool clean_tile(char* tile, int t) {
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 64 * Tile32<D>::RB / (256 * 16); ++i) {
+    u32x4* c = (u32x4*)(tile + (t + 256 * i) * 16);
+    const u32x4 v = *c;
+    if (!finite16<bf16_t>(v)) {
+      *c = finite_part<bf16_t>(v);
+      found = true;
+    }
+  }
+  return found;
+}
 
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
@@ -498,8 +508,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   const int every = (most + 63) >> 6, per = (every + p.splits - 1) / p.splits;
   const int i0 = per * (int)blockIdx.z, tiles = min(every - i0, per), k_first = 64 * i0;
   if (tiles > 0) {
-    Stage64<D, false> ks_(kp, p.k_row, t);
-    Stage64<D, true> vs_(vp, p.v_row, t);
+    const Fetch64<D, false> fetch_k(p.k_row, wave, lane);
+    const Fetch64<D, true> fetch_v(p.v_row, wave, lane);
     auto scores = [&](const char* kt, int half, f32x16& s) __attribute__((always_inline)) {
       s = zero16();
 #pragma unroll
@@ -566,16 +576,16 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
         for (int d = 0; d < L::DB; ++d) o[d] *= keep;
       }
     };
-    // K runs one tile ahead of V in LDS: [0] K, [1] V, two slots each, tile i in slot i & 1.  Iteration i's stores go to
-    // slots last read two steps ago, with the previous iteration's barrier in between.
+    // K runs one tile ahead of V in LDS: [0] K, [1] V, two slots each, tile i in slot i & 1.  Iteration i's fetches go to
+    // slots last read before its barrier and are waited for in front of the next.
     const int all = min(max(128 * R.tile + nk - R.n + 1, 0), nk);  // keys that every query of the workgroup sees
     if (t == 0) odd = 0;
-    ks_.load(k_first, nk);
+    fetch_k(lds[0][0], kp, p.k_row, k_first, nk);
+    fetch_k(lds[0][1], kp, p.k_row, k_first + 64, nk);
+    fetch_v(lds[1][0], vp, p.v_row, k_first, nk);
 #pragma unroll
     for (int i = 0; i < 64 * L::RB / (256 * 16); ++i) *(u32x4*)(lds[1][1] + (t + 256 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
-    ks_.store(lds[0][0]);
-    ks_.load(k_first + 64, nk);
-    vs_.load(k_first, nk);
+    arrive();
     __syncthreads();
     f32x16 s0, s1;
     u32x4 p0[2], p1[2] = {u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}};
@@ -583,12 +593,14 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
     auto tile = [&](int i, auto par) __attribute__((always_inline)) {   // par = i & 1, known to the compiler: LDS addresses are constants
       constexpr int P = decltype(par)::value;
       step(k_first + 64 * i, s0, s1, lds[0][P], 1, p1, p0, lds[1][P ^ 1], 1);
-      ks_.store(lds[0][P ^ 1]);                                    // (behind the last tile: zeros, never used)
-      if (k_first + 64 * i + 64 > all && vs_.clean()) odd = 1;
-      vs_.store(lds[1][P]);
+      arrive();
       __syncthreads();
-      ks_.load(k_first + 64 * i + 128, nk);
-      vs_.load(k_first + 64 * i + 64, nk);
+      fetch_k(lds[0][P], kp, p.k_row, k_first + 64 * i + 128, nk);   // (behind the last tile: zeros, never used)
+      fetch_v(lds[1][P ^ 1], vp, p.v_row, k_first + 64 * i + 64, nk);
+      if (k_first + 64 * i + 64 > all) {
+        if (clean_tile<D>(lds[1][P], t)) odd = 1;
+        __syncthreads();
+      }
       step(k_first + 64 * i + 32, s1, s0, lds[0][P ^ 1], 0, p0, p1, lds[1][P], 0);
     };
     int i = 0;
@@ -598,6 +610,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
     }
     if (i < tiles) tile(i, std::integral_constant<int, 0>());
     weigh(lds[1][(tiles - 1) & 1], 1, p1);
+    arrive();                                                      // (nothing lands in LDS that is not this workgroup's any more)
     if (odd)
       add_not_finite<T, D, 16 * L::DB>(qp, kp, p.k_row, vp, p.v_row, max(all & ~63, k_first), min(most, k_first + 64 * tiles), sees, p.scale * LOG2E, m, lane,
                                        [&](int i) { return 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hh + (i & 3); },
@@ -906,11 +919,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
 #pragma unroll
   for (int d = 0; d < L::DB; ++d) dq[d] = zero16();
   if (most > 0) {
-    Stage64<D, true> ks_(kp, p.k_row, t), vs_(vp, p.v_row, t);
-    ks_.load(0, nk);
-    vs_.load(0, nk);
-    ks_.store(lds[0][0]);
-    vs_.store(lds[0][1]);
+    const Fetch64<D, true> fetch_k(p.k_row, wave, lane), fetch_v(p.v_row, wave, lane);
+    fetch_k(lds[0][0], kp, p.k_row, 0, nk);
+    fetch_v(lds[0][1], vp, p.v_row, 0, nk);
+    arrive();
     __syncthreads();
     // laid out by hand: with each matrix instruction goes the read of a later fragment (hipcc reads it right in front
     // of the product that waits for it), as far ahead as the registers reach; the first of K^T are in flight under the probabilities
@@ -952,17 +964,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
       constexpr int P = decltype(par)::value;
       const bool more = k0 + 64 < most;
       if (more) {
-        ks_.load(k0 + 64, nk);
-        vs_.load(k0 + 64, nk);
+        fetch_k(lds[P ^ 1][0], kp, p.k_row, k0 + 64, nk);
+        fetch_v(lds[P ^ 1][1], vp, p.v_row, k0 + 64, nk);
       }
       if (k0 < any) {
         half(k0, lds[P][0], lds[P][1], 0);
         half(k0, lds[P][0], lds[P][1], 1);
       }
-      if (more) {
-        ks_.store(lds[P ^ 1][0]);
-        vs_.store(lds[P ^ 1][1]);
-      }
+      arrive();
       __syncthreads();
     };
     for (int k0 = 0; k0 < most; k0 += 128) {
@@ -992,7 +1001,6 @@ template <int D>
 __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   using L = Tile32<D>;
   using T = bf16_t;
-  using St = Stage64<D, true, 512>;
   constexpr int TB = 64 * L::RB;                                   // bytes of a tile: slot i: q at 2 i TB, dout behind it
   __shared__ __attribute__((aligned(16))) char tiles_[6 * TB];
   __shared__ __attribute__((aligned(16))) float prob[3][4][4][64][4];   // [slot][pair][accumulators 4 j ..][lane]
@@ -1031,7 +1039,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   if (total > 0) {
     // Tiles in order: head by head, the queries from the last down.  Addresses and sizes of the tile to load next are kept as
     // running scalars.  Wave parity picks the row of statistics (lse, delta) a wave fetches; waves of a parity store the same.
-    St qs_((const T*)p.q, p.q_row, t), gs_((const T*)p.dout, p.do_row, t);
+    const Fetch64<D, true, 8> fetch_q(p.q_row, wave, lane), fetch_g(p.do_row, wave, lane);
     const int top = first + 64 * (blocks - 1), st_row = wave & 1;
     const long long q_at = (long long)(q_lo + top) * p.q_row + (long long)hk * p.G * p.q_head;
     const long long g_at = (long long)(q_lo + top) * p.do_row + (long long)hk * p.G * p.do_head;
@@ -1045,16 +1053,11 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
     const float s_mul = st_row ? 1.f : LOG2E;
     int lq = top, left = total;                                    // first query of the tile to load next, tiles left
     float sv = 0.f;
-    auto load = [&]() __attribute__((always_inline)) {             // (no tile left: zeros)
+    auto load = [&](int slot) __attribute__((always_inline)) {     // (no tile left: zeros)
       const bool any = left > 0, part = lq == top;
-      const __amdgpu_buffer_rsrc_t rq = make_rsrc(qa, !any ? 0u : part ? q_rest : q_full);
-      const __amdgpu_buffer_rsrc_t rg = make_rsrc(ga, !any ? 0u : part ? g_rest : g_full);
+      fetch_q(tiles_ + 2 * slot * TB, make_buffer(qa, !any ? 0u : part ? q_rest : q_full));
+      fetch_g(tiles_ + (2 * slot + 1) * TB, make_buffer(ga, !any ? 0u : part ? g_rest : g_full));
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(sa, !any ? 0u : part ? 4u * rest : 256u);
-#pragma unroll
-      for (int i = 0; i < St::PER; ++i) {
-        qs_.load1(rq, i);
-        gs_.load1(rg, i);
-      }
       sv = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4u * lane, 0, 0));
       const bool wrap = lq == first;
       qa += wrap ? q_next : -q_down;
@@ -1063,11 +1066,10 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
       lq = wrap ? top : lq - 64;
       --left;
     };
-    auto store = [&](int slot) __attribute__((always_inline)) {
-      qs_.store(tiles_ + 2 * slot * TB);
-      gs_.store(tiles_ + (2 * slot + 1) * TB);
+    auto settle = [&](int slot) __attribute__((always_inline)) {   // the tile being loaded is there
       // a query that sees no key has lse -inf; +inf makes its probabilities 0 instead of NaN
       stat[128 * slot + 64 * st_row + lane] = !st_row && sv == -__builtin_inff() ? __builtin_inff() : sv * s_mul;
+      arrive();
     };
     // slot 2 stands for the block before the first: zeros (what they multiply is zero too, but 0 * NaN is not)
 #pragma unroll
@@ -1075,9 +1077,8 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) *(u32x4*)((char*)&prob[2] + (t + 512 * i) * 16) = u32x4{0u, 0u, 0u, 0u};
     if (t < 128) stat[256 + t] = 0.f;
-    load();
-    store(0);
-    load();
+    load(0);
+    settle(0);
     __syncthreads();
     int q0 = top + 32 * qh;                                        // this wave's queries of the current tile
     f32x16 acc = zero16();                                         // A: scores, B: do . v
@@ -1145,11 +1146,11 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
     };
     auto block = [&](auto slot_) __attribute__((always_inline)) {
       constexpr int SL = decltype(slot_)::value;
+      load((SL + 1) % 3);
       if (second) score_gradients(std::integral_constant<int, (SL + 2) % 3>());
       multiply(slot_);
-      store((SL + 1) % 3);
-      load();
       if (!second) probabilities(slot_);
+      settle((SL + 1) % 3);
       q0 -= 64;
       if (q0 < first) q0 = top + 32 * qh;
       __syncthreads();
