@@ -556,7 +556,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
       asm volatile("" : "+v"(pn[0]), "+v"(pn[1]), "+v"(l[0]), "+v"(l[1]));
       // order: fragments ahead, then a matrix instruction, a later fragment, and its share of the softmax; hipcc alone puts
       // all of the softmax behind the products and waits for every fragment
-      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 5, 0);
 #pragma unroll
       for (int j = 0; j < L::NKS; ++j) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -924,9 +924,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
     fetch_v(lds[0][1], vp, p.v_row, 0, nk);
     arrive();
     __syncthreads();
-    // laid out by hand: with each matrix instruction goes the read of a later fragment (hipcc reads it right in front
-    // of the product that waits for it), as far ahead as the registers reach; the first of K^T are in flight under the probabilities
-    constexpr int NP = 2 * L::NKS, NM = NP + 2 * L::DB, AHEAD = D == 64 ? 5 : 2;
+    // laid out by hand: with each matrix instruction goes the read of the fragment five later (hipcc reads it right in front
+    // of the product that waits for it); the first of K^T are in flight under the probabilities
+    constexpr int NP = 2 * L::NKS, NM = NP + 2 * L::DB, AHEAD = 5;
     auto half = [&](int k0, const char* kt, const char* vt, int i) __attribute__((always_inline)) {
       auto fragment = [&](int x) __attribute__((always_inline)) -> u32x4 {
         if (x < NP) return L::rows_t(x & 1 ? vt : kt, i, x >> 1, lane);
