@@ -1163,8 +1163,8 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     """Causal attention of packed sequences: q (Mq, Hq, D), k, v (Mk, Hk, D), any row and head strides, Hq a multiple of Hk;
     sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
     cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
-    -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  Rows behind the last sequence: left as they were in a given `out`, zero in a
-    new one.  scale: 1 / sqrt(D) unless given.  want_low: -> (out, lse, low), low what rounding out to 16 bits took from it
+    -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  `out`, where given, is a buffer of its own.  Rows behind the last sequence: left
+    as they were in a given `out`, zero in a new one.  scale: 1 / sqrt(D) unless given.  want_low: -> (out, lse, low), low what rounding out to 16 bits took from it
     (None for f32), for packed_attn_bwd."""
     i = _device_of(q)
     if i != _current_device():
@@ -1216,7 +1216,8 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
     gaps = grads is None
     if gaps:
         dq = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)
-        dk, dv = torch.empty((2, Mk, Hk, D), dtype=q.dtype, device=q.device).unbind(0)
+        dk = torch.empty((Mk, Hk, D), dtype=q.dtype, device=q.device)
+        dv = torch.empty((Mk, Hk, D), dtype=q.dtype, device=q.device)
     else:
         dq, dk, dv = grads
         for g, x in ((dq, q), (dk, k), (dv, v)):

@@ -27,6 +27,8 @@ def main():
         pa.check([64, 1, 63, 65, 200], [64, 1, 63, 65, 200], 4, 2, D, H)
         pa.check([5, 300, 129], [40, 301, 129], 4, 1, D, H)
         pa.check([70, 33, 3], [10, 0, 3], 4, 2, D, H)
+    pa.test_values_that_are_not_finite_reach_only_the_queries_that_see_them(200, 128, "half")
+    pa.test_few_queries_over_many_keys()
     print("packed attention ok", flush=True)
     for D in (64, 128):
         pg.check([0, 1, 31, 129, 0, 500], 16, 2, D, 16, H)

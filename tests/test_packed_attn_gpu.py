@@ -105,6 +105,9 @@ def test_scale_and_large_scores():
     check([130], [130], 2, 1, 64, _half(), scale=0.5, std=4.0)
     check([130], [130], 2, 1, 128, torch.float32, scale=1.0, std=3.0)
     check([50], [50], 2, 2, 64, torch.float32, scale=-0.125)
+    check([150, 20], [170, 20], 4, 2, 128, _half(), scale=-0.125)
+    for dt in (torch.float32, _half()):                            # every visible key alike
+        check([70, 3], [70, 5], 2, 1, 64, dt, scale=0.0)
 
 
 def test_few_queries_over_many_keys():
@@ -269,6 +272,55 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_calls_at_once():
+    """forward and backward on two streams side by side, over and over, against the same calls one after the other"""
+    from melspec_gpt_vqvae_amd import ops
+
+    a = [x.to(DEV) for x in make([900, 40], [900, 40], 4, 2, 128, _half(), 1)]
+    b = [x.to(DEV) for x in make([20], [3000], 8, 2, 128, _half(), 2)]
+    cu_a, cu_q, cu_k = _cu([900, 40]).to(DEV), _cu([20]).to(DEV), _cu([3000]).to(DEV)
+
+    def first():
+        out, lse = ops.packed_attn_fwd(*a[:3], cu_a)
+        return (out, lse) + ops.packed_attn_bwd(*a[:3], out, a[3], lse, cu_a)
+
+    def other():
+        out, lse = ops.packed_attn_fwd(*b[:3], cu_q, cu_k)         # (keys shared by several workgroups)
+        return (out, lse) + ops.packed_attn_bwd(*b[:3], out, b[3], lse, cu_q, cu_k)
+
+    want_a, want_b = first(), other()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(streams[0]):
+            x = first()
+        with torch.cuda.stream(streams[1]):
+            y = other()
+        got.append((x, y))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert all(torch.equal(p, q) for p, q in zip(x, want_a)) and all(torch.equal(p, q) for p, q in zip(y, want_b))
+
+
+def test_backward_through_a_broadcast_sum_and_one_input():
+    """a gradient that is one value expanded, and inputs of which only one wants a gradient"""
+    from melspec_gpt_vqvae_amd.transformer.packed import packed_attention
+
+    q, k, v, _ = [x.to(DEV) for x in make([90], [90], 4, 2, 64, _half(), 3)]
+    cu = _cu([90]).to(DEV)
+    v = v.detach().clone().requires_grad_(True)
+    packed_attention(q, k, v, cu).sum().backward()
+    one = v.grad.clone()
+    v.grad = None
+    packed_attention(q, k, v, cu).backward(torch.ones_like(q))
+    assert torch.equal(v.grad, one) and q.grad is None
+    # every query hands out a total weight of 1: the values' gradients of a column add up to the queries (rounded once each,
+    # probabilities to the tensors' type before)
+    total = v.grad.double().sum((0, 1))
+    assert float((total - 4 * 90).abs().max()) <= 4 * 90 * 2 * R.half_step(_half())
 
 
 def test_other_stream():
