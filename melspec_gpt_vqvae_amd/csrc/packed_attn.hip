@@ -102,52 +102,30 @@ __device__ __forceinline__ void head_of(int w, const PackedParams& p, int& h) {
   h = kv * p.G + g;
 }
 
-// ------------------------------------------------------------------------------------------------- tiles in LDS
-// R rows of D values, 16-byte chunks xor-swizzled by the row so that neither row reads (16 rows, one chunk) nor transposed
-// reads pile up on banks.
-template <typename T, int D>
+// ---------------------------------------------------------------------------------------------- tiles in LDS, f32 lane
+// R rows of D values, 16-byte chunks xor-swizzled by the row so that neither row reads (16 rows, one chunk) nor reads along
+// columns pile up on banks.
+template <int D>
 struct Tile {
-  static constexpr int ES = Tr<T>::ES, RB = D * ES, CP = RB / 16, VEC = 16 / ES;
+  static constexpr int RB = 4 * D, CP = RB / 16;
   static constexpr int NKS = CP / 4;           // fragments along D
   static constexpr int DT = D / 16;            // 16-column tiles
-  static constexpr int STEPS = ES == 2 ? 1 : 2;   // contraction steps along 32 rows
-  static __device__ __forceinline__ int off(int row, int c) {
-    if constexpr (RB == 128) return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
-    else return row * RB + ((c ^ (row & 15)) << 4);
-  }
+  static __device__ __forceinline__ int off(int row, int c) { return row * RB + ((c ^ (row & 15)) << 4); }
   // fragment of 16 rows (16 tile16 + (lane & 15)), contraction along D
   static __device__ __forceinline__ u32x4 rows(const char* t, int tile16, int ks, int lane) {
     return *(const u32x4*)(t + off(16 * tile16 + (lane & 15), 4 * ks + (lane >> 4)));
   }
-  // fragment of 16 columns (16 dt + (lane & 15)), contraction along rows, step st: 32 rows for 16-bit types (slot j < 4: row
-  // 32 st + 4 g + j, else 32 st + 16 + 4 g + j - 4), 16 for f32 (slot e: row 16 st + 4 g + e) - the order in which the
-  // accumulators of the score products hold them, so those are the other operand as they stand
+  // fragment of 16 columns (16 dt + (lane & 15)), contraction along rows 16 st .. + 15 (slot e: row 16 st + 4 g + e) - the
+  // order in which the accumulators of the score products hold them, so those are the other operand as they stand
   static __device__ __forceinline__ u32x4 cols(const char* t, int st, int dt, int lane) {
-    const int i = lane & 15, g = lane >> 4;
-    if constexpr (ES == 2) {
-      const int r0 = 32 * st + 4 * g + (i >> 2), c = 2 * dt + ((i & 3) >> 1);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off(r0, c) + 8 * (i & 1)));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, t + off(r0 + 16, c) + 8 * (i & 1)));
-      const s16x8 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      return __builtin_bit_cast(u32x4, f);
-    } else {
-      const int col = 16 * dt + i;
-      u32x4 f;
+    const int g = lane >> 4, col = 16 * dt + (lane & 15);
+    u32x4 f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = *(const unsigned*)(t + off(16 * st + 4 * g + e, col >> 2) + (col & 3) * 4);
-      return f;
-    }
+    for (int e = 0; e < 4; ++e) f[e] = *(const unsigned*)(t + off(16 * st + 4 * g + e, col >> 2) + (col & 3) * 4);
+    return f;
   }
 };
 
-// accumulators of 32 rows as operands that contract over them: one for 16-bit types, two for f32
-template <typename T>
-__device__ __forceinline__ u32x4 operand(const f32x4& lo, const f32x4& hi, int step) {
-  if constexpr (Tr<T>::ES == 2)
-    return u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
-  else
-    return __builtin_bit_cast(u32x4, step ? hi : lo);
-}
 template <typename T>
 __device__ __forceinline__ void store4(T* p, f32x4 v) {
   if constexpr (Tr<T>::ES == 2) *(u32x2*)p = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
@@ -222,17 +200,18 @@ __device__ __forceinline__ void add_not_finite(const T* q, const T* k, long long
 
 // 32 rows of two tensors on their way into LDS: the loads of the next pair are in flight under the current pair's products.
 // Rows at and beyond n are zero (their products are masked, but 0 * NaN is not 0).
-template <typename T, int D>
+template <int D>
 struct Stage {
-  using L = Tile<T, D>;
+  using T = float;
+  using L = Tile<D>;
   static constexpr int PER = 32 * L::CP / 256;   // chunks per thread
   u32x4 a[PER], b[PER];
   __device__ __forceinline__ void load(const T* pa, long long ra, const T* pb, long long rb, int row0, int n, int t) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int q = t + 256 * i, row = min(row0 + q / L::CP, n - 1), c = q % L::CP;
-      a[i] = *(const u32x4*)(pa + row * ra + c * L::VEC);
-      b[i] = *(const u32x4*)(pb + row * rb + c * L::VEC);
+      a[i] = *(const u32x4*)(pa + row * ra + c * 4);
+      b[i] = *(const u32x4*)(pb + row * rb + c * 4);
     }
   }
   // -> whether tensor b had values that are not finite (it has zeros there now)
@@ -257,13 +236,14 @@ struct Stage {
   }
 };
 
-// -------------------------------------------------------------------------------------------------------- forward
+// --------------------------------------------------------------------------------------------- forward, f32 lane
 // 256 threads, 64 queries of one head: a wave owns 16 queries and walks the keys 32 at a time.  S^T = K Q^T puts the query
 // on the lane: its maximum and sum are in registers and two exchanges away, and the probabilities are the operand of
 // O^T = V^T P^T as they stand.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
-  using L = Tile<T, D>;
+template <int D>
+__global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
+  using T = float;
+  using L = Tile<D>;
   __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
   __shared__ int odd;                                              // a value that is not finite in a tile the causal border cuts
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
@@ -283,7 +263,7 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
   const T* qp = (const T*)p.q + row * p.q_row + h * p.q_head;
   u32x4 qf[L::NKS];
 #pragma unroll
-  for (int ks = 0; ks < L::NKS; ++ks) qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * L::VEC);
+  for (int ks = 0; ks < L::NKS; ++ks) qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * 4);
   const T* kp = (const T*)p.k + (long long)k_lo * p.k_row + (h / p.G) * p.k_head;
   const T* vp = (const T*)p.v + (long long)k_lo * p.v_row + (h / p.G) * p.v_head;
   const float c2 = p.scale * LOG2E;
@@ -292,7 +272,7 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
   for (int d = 0; d < L::DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -__builtin_inff(), l = 0.f;
   if (most > 0) {
-    Stage<T, D> st;
+    Stage<D> st;
     const int full = min(max(64 * R.tile + nk - R.n + 1, 0), nk);  // keys that every query of the workgroup sees
     if (t == 0) odd = 0;
     __syncthreads();
@@ -335,11 +315,9 @@ __global__ __launch_bounds__(256) void packed_fwd_kernel(PackedParams p) {
 #pragma unroll
       for (int d = 0; d < L::DT; ++d) o[d] *= keep;
 #pragma unroll
-      for (int e = 0; e < L::STEPS; ++e) {
-        const u32x4 pf = operand<T>(s[0], s[1], e);
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int d = 0; d < L::DT; ++d) mma<T>(o[d], L::cols(vt, e, d, lane), pf);
-      }
+        for (int d = 0; d < L::DT; ++d) mma<T>(o[d], L::cols(vt, e, d, lane), __builtin_bit_cast(u32x4, s[e]));
       if (more && k0 + 64 > full && st.clean_b()) odd = 1;
       if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 32, nk, t);
       __syncthreads();
@@ -679,11 +657,12 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
   if (d == 0) p.lse[n] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// -------------------------------------------------------------------------------------------------------- backward
+// --------------------------------------------------------------------------------------------- backward, f32 lane
 // dq and delta: the forward's walk with a second score product, do . v, on the same tiles
-template <typename T, int D>
-__global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
-  using L = Tile<T, D>;
+template <int D>
+__global__ __launch_bounds__(256) void packed_dq_f32_kernel(PackedParams p) {
+  using T = float;
+  using L = Tile<D>;
   __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
   int h;
@@ -706,18 +685,11 @@ __global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
   float dl = 0.f;
 #pragma unroll
   for (int ks = 0; ks < L::NKS; ++ks) {
-    qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * L::VEC);
-    gf[ks] = *(const u32x4*)(gp + (4 * ks + g) * L::VEC);
-    const u32x4 of = *(const u32x4*)(op + (4 * ks + g) * L::VEC);
+    qf[ks] = *(const u32x4*)(qp + (4 * ks + g) * 4);
+    gf[ks] = *(const u32x4*)(gp + (4 * ks + g) * 4);
+    const u32x4 of = *(const u32x4*)(op + (4 * ks + g) * 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (L::ES == 2) {
-        dl = fmaf(half_lo(gf[ks][e]), half_lo(of[e]), dl);
-        dl = fmaf(half_hi(gf[ks][e]), half_hi(of[e]), dl);
-      } else {
-        dl = fmaf(__uint_as_float(gf[ks][e]), __uint_as_float(of[e]), dl);
-      }
-    }
+    for (int e = 0; e < 4; ++e) dl = fmaf(__uint_as_float(gf[ks][e]), __uint_as_float(of[e]), dl);
   }
   dl = across_groups_sum(dl);
   if (mine && g == 0) p.delta[h * p.Mq + row] = dl;
@@ -729,7 +701,7 @@ __global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
 #pragma unroll
   for (int d = 0; d < L::DT; ++d) dq[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (most > 0) {
-    Stage<T, D> st;
+    Stage<D> st;
     st.load(kp, p.k_row, vp, p.v_row, 0, nk, t);
     st.store(lds[0][0], lds[0][1], 0, nk, t);
     __syncthreads();
@@ -751,11 +723,9 @@ __global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
           s[i][r] = k0 + 16 * i + 4 * g + r < sees ? __builtin_amdgcn_exp2f(s[i][r] * c2 - lse2) * (dp[i][r] - dl) : 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < L::STEPS; ++e) {
-        const u32x4 sf = operand<T>(s[0], s[1], e);
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int d = 0; d < L::DT; ++d) mma<T>(dq[d], L::cols(kt, e, d, lane), sf);
-      }
+        for (int d = 0; d < L::DT; ++d) mma<T>(dq[d], L::cols(kt, e, d, lane), __builtin_bit_cast(u32x4, s[e]));
       if (more) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], k0 + 32, nk, t);
       __syncthreads();
     }
@@ -768,9 +738,10 @@ __global__ __launch_bounds__(256) void packed_dq_kernel(PackedParams p) {
 
 // dk and dv: 64 keys of one key head, a wave owns 16 keys (in registers) and walks the queries of its G heads that see
 // them, 32 at a time.  S = Q K^T puts the key on the lane; P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
-  using L = Tile<T, D>;
+template <int D>
+__global__ __launch_bounds__(256) void packed_dkv_f32_kernel(PackedParams p) {
+  using T = float;
+  using L = Tile<D>;
   __shared__ __attribute__((aligned(16))) char lds[2][2][32 * L::RB];
   __shared__ float stat[2][2][32];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4;
@@ -792,8 +763,8 @@ __global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
   u32x4 kf[L::NKS], vf[L::NKS];
 #pragma unroll
   for (int ks = 0; ks < L::NKS; ++ks) {
-    kf[ks] = *(const u32x4*)(kp + (4 * ks + g) * L::VEC);
-    vf[ks] = *(const u32x4*)(vp + (4 * ks + g) * L::VEC);
+    kf[ks] = *(const u32x4*)(kp + (4 * ks + g) * 4);
+    vf[ks] = *(const u32x4*)(vp + (4 * ks + g) * 4);
   }
   const float c2 = p.scale * LOG2E;
   f32x4 dk[L::DT], dv[L::DT];
@@ -801,7 +772,7 @@ __global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
   for (int d = 0; d < L::DT; ++d) dk[d] = dv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int blocks = first < nq ? (nq - first + 31) / 32 : 0, total = blocks * p.G;
   if (total > 0) {
-    Stage<T, D> st;
+    Stage<D> st;
     float sv = 0.f;
     auto load = [&](int n) {
       const int h = hk * p.G + n / blocks, q0 = first + 32 * (n % blocks);
@@ -842,14 +813,12 @@ __global__ __launch_bounds__(256) void packed_dkv_kernel(PackedParams p) {
         }
       }
 #pragma unroll
-      for (int e = 0; e < L::STEPS; ++e) {
-        const u32x4 pf = operand<T>(s[0], s[1], e), sf = operand<T>(dp[0], dp[1], e);
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int d = 0; d < L::DT; ++d) {
-          mma<T>(dv[d], L::cols(gt, e, d, lane), pf);
-          mma<T>(dk[d], L::cols(qt, e, d, lane), sf);
+          mma<T>(dv[d], L::cols(gt, e, d, lane), __builtin_bit_cast(u32x4, s[e]));
+          mma<T>(dk[d], L::cols(qt, e, d, lane), __builtin_bit_cast(u32x4, dp[e]));
         }
-      }
       if (n + 1 < total) store(n + 1, buf ^ 1);
       __syncthreads();
     }
@@ -1237,7 +1206,7 @@ int launch_fwd(const PackedParams& p, hipStream_t s) {
       hipLaunchKernelGGL((packed_join_kernel<D>), dim3((unsigned)((p.Hq * p.Mq + per - 1) / per)), dim3(256), 0, s, p);
     }
   } else
-    hipLaunchKernelGGL((packed_fwd_kernel<T, D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((packed_fwd_f32_kernel<D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
   return melgpt_launch_status();
 }
 
@@ -1250,8 +1219,8 @@ int launch_bwd(const PackedParams& p, hipStream_t s) {
     if (p.Mq > 0) hipLaunchKernelGGL((packed_dq32_kernel<D>), gq, dim3(256), 0, s, p);
     if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv32_kernel<D>), gk, dim3(512), 0, s, p);
   } else {
-    if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_kernel<T, D>), gq, dim3(256), 0, s, p);
-    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_kernel<T, D>), gk, dim3(256), 0, s, p);
+    if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_f32_kernel<D>), gq, dim3(256), 0, s, p);
+    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_f32_kernel<D>), gk, dim3(256), 0, s, p);
   }
   return melgpt_launch_status();
 }
@@ -1294,7 +1263,7 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
   const int e = check(p, D, dtype);
   if (e) return e;
   if (splits < 1 || (splits > 1 && !workspace)) return MELGPT_ERR_BAD_ARG;
-  if (splits > 1 && (dtype == MELGPT_F32 || out_low || splits > 1024 || Hq * Mq > (1LL << 32))) return MELGPT_ERR_UNSUPPORTED;
+  if (splits > 1 && (dtype == MELGPT_F32 || out_low || splits > 1024 || Hq * Mq > (1LL << 26))) return MELGPT_ERR_UNSUPPORTED;
   if (!aligned16(workspace)) return MELGPT_ERR_ALIGN;
   if (Mq == 0) return MELGPT_OK;
   p.G = Hq / Hk;

@@ -1000,6 +1000,18 @@ def _heads(x, vec):
     return x, r, h
 
 
+def _into(x, like, *inputs):
+    """x: a caller's (rows, heads, D) buffer for a result shaped as `like`: its rows and heads must not overlap, and it must
+    not start where an input or another result does"""
+    assert x.shape == like.shape and x.dtype == like.dtype, (x.shape, like.shape, x.dtype, like.dtype)
+    M, H, D = x.shape
+    r, h, u = x.stride()
+    assert u == 1 and (H <= 1 or h >= D) and (M <= 1 or r >= D) and \
+        (M <= 1 or H <= 1 or r >= (H - 1) * h + D or h >= (M - 1) * r + D), f"strides {(r, h, u)}: rows or heads of a result overlap"
+    p = x.data_ptr()
+    assert p == 0 or all(p != y.data_ptr() for y in inputs), "a result is a buffer of its own"
+
+
 def _addr(x):
     return None if x is None else x.data_ptr()
 
@@ -1164,8 +1176,9 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
     cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
     -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  `out`, where given, is a buffer of its own.  Rows behind the last sequence: left
-    as they were in a given `out`, zero in a new one.  scale: 1 / sqrt(D) unless given.  want_low: -> (out, lse, low), low what rounding out to 16 bits took from it
-    (None for f32), for packed_attn_bwd."""
+    as they were in a given `out`, zero in a new one.  scale: 1 / sqrt(D) unless given.  want_low: -> (out, lse, low), low
+    what rounding out to 16 bits took from it (None for f32), for packed_attn_bwd.  Values that are not finite reach the
+    queries that see them and no others."""
     i = _device_of(q)
     if i != _current_device():
         return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out, want_low=want_low)
@@ -1179,7 +1192,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     if gaps:
         out = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)
     else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        _into(out, q, q, k, v)
         _same_device(i, out)
     lse = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
     low = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device) if want_low and dt != _ffi.F32 else None
@@ -1196,8 +1209,9 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
 
 def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, grads=None, low=None):
     """gradients of packed_attn_fwd from its inputs, its results (out, lse and, if asked for, low) and dout (any row and head
-    strides) -> (dq, dk, dv), contiguous and zero in rows that no sequence owns, unless `grads` gives the three tensors (any row and head strides,
-    such rows left as they were)."""
+    strides) -> (dq, dk, dv), contiguous and zero in rows that no sequence owns, unless `grads` gives the three tensors (any
+    row and head strides, buffers of their own, such rows left as they were).  A value that is not finite may reach every
+    gradient of its sequence (a weight of 0 times it), none of another's."""
     i = _device_of(q)
     if i != _current_device():
         return _on(i, packed_attn_bwd, q, k, v, out, dout, lse, cu_q, cu_k, scale=scale, grads=grads, low=low)
@@ -1220,8 +1234,9 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
         dv = torch.empty((Mk, Hk, D), dtype=q.dtype, device=q.device)
     else:
         dq, dk, dv = grads
-        for g, x in ((dq, q), (dk, k), (dv, v)):
-            assert g.shape == x.shape and g.dtype == x.dtype and g.stride(2) == 1
+        _into(dq, q, q, k, v, out, dout, dk, dv)
+        _into(dk, k, q, k, v, out, dout, dv)
+        _into(dv, v, q, k, v, out, dout)
         _same_device(i, dq, dk, dv)
     delta = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
     call("melgpt_packed_attn_bwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
@@ -1234,7 +1249,7 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
 def paged_attn_decode(q, k_pages, v_pages, page_table, lengths, *, scale=None, max_length=None, out=None):
     """Attention of one query token per sequence over a paged cache: q (S, Hq, D), any row and head strides; k_pages, v_pages
     (pages, Hk, page size, D), Hq a multiple of Hk; page_table (S, width) int32; lengths (S,) int32, the keys each sequence
-    has (those of kv_append's last row among them) -> (out (S, Hq, D), lse (S, Hq) f32).  A sequence without keys gives 0; a
+    has (those of kv_append's last row among them; what the table's width does not hold is not there) -> (out (S, Hq, D), lse (S, Hq) f32).  A sequence without keys gives 0; a
     table entry outside the pages leaves its keys out.  max_length: the longest length, where the caller knows one shorter
     than the table's width (it only decides how far a sequence is split).  scale: 1 / sqrt(D) unless given."""
     i = _device_of(q)
@@ -1251,7 +1266,7 @@ def paged_attn_decode(q, k_pages, v_pages, page_table, lengths, *, scale=None, m
     if out is None:
         out = torch.empty((S, Hq, D), dtype=q.dtype, device=q.device)
     else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        _into(out, q, q)
     lse = torch.empty((S, Hq), dtype=torch.float32, device=q.device)
     if S == 0:
         return out, lse

@@ -287,3 +287,41 @@ def test_captured_and_replayed_append():
         ref_q, ref_k = ops.qk_norm_rotary_fwd(q, k, pos, f, q_weight=wq, k_weight=wk)
         assert torch.equal(out, ref_q)
         assert torch.equal(kp[0, :, 3 * i + 1], ref_k[0]) and torch.equal(vp[6, :, 3 * i + 1], v[3])
+
+
+def test_captured_forward_and_backward_and_two_streams():
+    """a captured pass replayed with new inputs, and the same pass on two streams side by side: the eager bits every time"""
+    from melspec_gpt_vqvae_amd import ops
+    from melspec_gpt_vqvae_amd.transformer.packed import rotary_freqs
+
+    M, Hq, Hk, D = 700, 8, 2, 64
+    g = torch.Generator().manual_seed(11)
+    q, k, dq, dk = [torch.randn(M, h, D, generator=g).to(_half()).to(DEV) for h in (Hq, Hk, Hq, Hk)]
+    w = [torch.rand(D, generator=g).to(DEV) + 0.5 for _ in range(2)]
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)
+    f = rotary_freqs(D, device=DEV)
+
+    def run():
+        kw = dict(q_weight=w[0], k_weight=w[1])
+        return ops.qk_norm_rotary_fwd(q, k, pos, f, **kw) + ops.qk_norm_rotary_bwd(dq, dk, q, k, pos, f, **kw)
+
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(run())
+    torch.cuda.synchronize()
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for i in range(3):
+        q.mul_(0.5)
+        pos.add_(100000)
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), i

@@ -323,6 +323,25 @@ def test_backward_through_a_broadcast_sum_and_one_input():
     assert float((total - 4 * 90).abs().max()) <= 4 * 90 * 2 * R.half_step(_half())
 
 
+def test_rows_far_apart():
+    """rows whose offsets pass 2^32 bytes: the same bits as from tensors side by side"""
+    from melspec_gpt_vqvae_amd import ops
+
+    D, M, far = 64, 2500, 1 << 20                                   # (2500 rows of 2^20 values: 5.2 GB)
+    cu = _cu([1100, 1400]).to(DEV)
+    near = [x.to(DEV) for x in make([1100, 1400], [1100, 1400], 2, 1, D, _half(), 7)]
+    room = torch.empty(M * far, dtype=_half(), device=DEV).view(M, far)
+    q, k, v, dout, out, dq, dk, dv = [room[:, 128 * i:128 * i + D * h].view(M, h, D) for i, h in enumerate((2, 1, 1, 2, 2, 2, 1, 1))]
+    for x, y in zip((q, k, v, dout), near):
+        x.copy_(y)
+    want, lse = ops.packed_attn_fwd(*near[:3], cu)
+    got, lse_far = ops.packed_attn_fwd(q, k, v, cu, out=out)
+    assert torch.equal(got, want) and torch.equal(lse, lse_far)
+    for a, b in zip(ops.packed_attn_bwd(q, k, v, out, dout, lse, cu, grads=(dq, dk, dv)),
+                    ops.packed_attn_bwd(*near[:3], want, near[3], lse, cu)):
+        assert torch.equal(a, b)
+
+
 def test_other_stream():
     from melspec_gpt_vqvae_amd import ops
 

@@ -144,6 +144,24 @@ def test_cpu_tensors_and_wrong_arguments_are_refused():
             call()
 
 
+def test_result_buffers_that_overlap_are_refused():
+    from melspec_gpt_vqvae_amd.ops import _into
+
+    x = torch.zeros(6, 4, 64)
+    fused = torch.zeros(6, 3, 4, 64)
+    good = [torch.empty(6, 4, 64), fused[:, 1], torch.empty(4, 6, 64).transpose(0, 1), torch.empty(6, 4, 96)[..., 16:80]]
+    for y in good:
+        _into(y, x, x, fused)
+    _into(torch.empty(0, 4, 64), torch.empty(0, 4, 64), torch.empty(0, 4, 64))
+    _into(torch.zeros(1, 1, 64).expand(1, 1, 64), torch.zeros(1, 1, 64))
+    bad = [x, torch.empty(1, 4, 64).expand(6, 4, 64), torch.empty(6, 1, 64).expand(6, 4, 64), torch.empty(6, 4, 128)[..., ::2],
+           torch.empty(6, 64, 4).transpose(1, 2), torch.empty(6, 4, 32), torch.empty(6, 4, 64, dtype=torch.float64),
+           torch.empty(4000).as_strided((6, 4, 64), (128, 64, 1)), torch.empty(4000).as_strided((6, 4, 64), (64, 128, 1))]
+    for y in bad:
+        with pytest.raises(AssertionError):
+            _into(y, x, x)
+
+
 def test_rotary_freqs():
     from melspec_gpt_vqvae_amd.transformer.packed import rotary_freqs
 
