@@ -24,7 +24,7 @@ struct PagedParams {
   const void *k_pages, *v_pages;
   const int *table, *lengths;
   long long table_ld;
-  int width, pages, page_shift, Hq, Hk, G, splits;
+  int width, pages, page_shift, Hq, Hk, G, splits, least;
   void* o;
   long long o_row, o_head;
   float* lse;     // (S, Hq)
@@ -69,6 +69,19 @@ __device__ __forceinline__ float over_groups_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// Keys of sequence s, and its 32-key tiles to a workgroup: an even share, but no less than `least` - a short sequence among
+// long ones uses fewer of the splits, and the workgroups beyond end at once.  One tile to a wave where (sequence, key head)
+// pairs are few and the longest way counts (one sequence of 4096 keys, 8 key heads of 128: 9.6 us, 14.2 with four to a wave),
+// four from 256 pairs on, where a workgroup's start and its partial result are what more of them cost (one sequence of 65536
+// keys among 63 of 1000: 172 us, 209 with one to a wave; lengths up to 4089 in 256 sequences, 8 splits: 418 / 426).
+__device__ __forceinline__ int length_of(const PagedParams& p, int s) {
+  const long long cap = (long long)p.width << p.page_shift;
+  return (int)min((long long)max(p.lengths[s], 0), min(cap, 0x7fffffc0LL));
+}
+__device__ __forceinline__ int share_of(const PagedParams& p, int len) {
+  return max((((len + 31) >> 5) + p.splits - 1) / p.splits, p.least);
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
   using L = Geo<T, D>;
@@ -77,9 +90,8 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, i16 = lane & 15;
   const int hk = blockIdx.x % p.Hk, s = blockIdx.x / p.Hk, split = blockIdx.y, h0 = hk * p.G + 16 * blockIdx.z;
   const int nh = min(p.G - 16 * (int)blockIdx.z, 16);             // query heads of this workgroup
-  const long long cap = (long long)p.width << p.page_shift;
-  const int len = (int)min((long long)max(p.lengths[s], 0), min(cap, 0x7fffffc0LL));
-  const int tiles = (len + 31) >> 5, per = (tiles + p.splits - 1) / p.splits;
+  const int len = length_of(p, s), tiles = (len + 31) >> 5, per = share_of(p, len);
+  if (split > 0 && (long long)split * per >= tiles) return;        // (the join knows as much)
   const int t0 = split * per, t1 = min(t0 + per, tiles);
   const int* table = p.table + (long long)s * p.table_ld;
   const T* kb = (const T*)p.k_pages;
@@ -234,16 +246,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   __shared__ float sums[NG];
   const long long head = blockIdx.x;
   const int g = threadIdx.x / TPQ, d = 4 * (threadIdx.x % TPQ), lane = threadIdx.x & 63;
+  const int len = length_of(p, (int)(head / p.Hq)), per = share_of(p, len), n = max((((len + 31) >> 5) + per - 1) / per, 1);
   const float* st = p.part + p.stats + 2 * head * p.splits;
   const float* pp = p.part + head * p.splits * D + d;
   float top = -__builtin_inff();
-  for (int i = lane; i < p.splits; i += 64) top = fmaxf(top, st[2 * i]);
+  for (int i = lane; i < n; i += 64) top = fmaxf(top, st[2 * i]);
   top = wave_max(top);
   const float base = top == -__builtin_inff() ? 0.f : top;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
 #pragma unroll 4
-  for (int i = g; i < p.splits; i += NG) {
+  for (int i = g; i < n; i += NG) {
     const float f = __builtin_amdgcn_exp2f(st[2 * i] - base);
     a += *(const f32x4*)(pp + (long long)i * D) * f;
     sum += st[2 * i + 1] * f;
@@ -275,12 +288,14 @@ int launch(const PagedParams& p, int S, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups per (sequence, key head): enough of them that the longest sequences do not finish alone, each with at least
-// 256 keys (two tiles per wave).
+// Workgroups per (sequence, key head): 2048 in all, so that the longest sequences do not finish alone, 128 keys (a tile to a
+// wave) or more each; a cache of up to 512 keys is not split (265 keys, 16 heads of 64: 6.1 us, 7.5 in two).  Measured, heads
+// of 128: one sequence of 4096 keys, 8 key heads 60 us in one piece, 9.6 in 32; three of 100000, 4 key heads 1354 / 117 in 128;
+// 64 sequences of lengths up to 8152, 8 key heads 243 / 211 in 4 / 204 in 8, but all of 4096 191 / 205 in 4 / 224 in 8.
 extern "C" int melgpt_paged_attn_splits(int S, int Hq, int Hk, long long max_length) {
-  if (S <= 0 || Hk <= 0 || Hq < Hk || max_length <= 0) return 1;
-  const long long base = (long long)S * Hk * ((Hq / Hk + 15) / 16), most = (max_length + 255) / 256;
-  long long n = (4096 + base - 1) / base;
+  if (S <= 0 || Hk <= 0 || Hq < Hk || max_length <= 512) return 1;
+  const long long base = (long long)S * Hk * ((Hq / Hk + 15) / 16), most = (max_length + 127) / 128;
+  long long n = (2048 + base - 1) / base;
   if (n > most) n = most;
   if (n > 128) n = 128;
   return (int)(n < 1 ? 1 : n);
@@ -307,6 +322,7 @@ extern "C" int melgpt_paged_attn_decode(const void* q, long long q_row, long lon
   p.table_ld = table_ld; p.width = width; p.pages = (int)n_pages; p.Hq = Hq; p.Hk = Hk; p.G = Hq / Hk; p.splits = splits;
   p.o = out; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.part = workspace; p.stats = (long long)S * Hq * splits * D;
   p.scale = scale;
+  p.least = (long long)S * Hk * ((p.G + 15) / 16) < 256 ? 4 : 16;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == MELGPT_F32) return D == 64 ? launch<float, 64>(p, S, st) : launch<float, 128>(p, S, st);

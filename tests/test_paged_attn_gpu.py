@@ -88,6 +88,21 @@ def test_split_lengths_and_scales():
     check([50], 2, 2, 64, 16, torch.float32, scale=-0.125)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("Hq,Hk,D", [(1, 1, 64), (7, 1, 128), (17, 1, 64), (40, 2, 64), (8, 8, 128)])
+def test_split_heads(Hq, Hk, D, dtype):
+    """few pairs: shares of 128 keys, sequences that fill some, one or none of the splits, shares that end inside a page"""
+    check([300, 0, 128, 129, 1, 1100, 256], Hq, Hk, D, 32, _dt(dtype), seed=3, extra_width=100)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+def test_split_many_sequences(dtype):
+    """256 pairs of sequence and key head or more: shares of 512 keys"""
+    lens = [0, 1, 511, 512, 513, 1025, 2100] + [7 * i % 90 for i in range(60)]
+    check(lens, 4, 4, 64, 16, _dt(dtype), seed=4)
+    check(lens, 8, 4, 128, 64, _dt(dtype), seed=5)
+
+
 def test_no_sequences_strides_and_given_out():
     from melspec_gpt_vqvae_amd import ops
 
