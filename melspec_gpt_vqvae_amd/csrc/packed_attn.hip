@@ -237,7 +237,8 @@ struct Stage {
 };
 
 // --------------------------------------------------------------------------------------------- forward, f32 lane
-// 256 threads, 64 queries of one head: a wave owns 16 queries and walks the keys 32 at a time.  S^T = K Q^T puts the query
+// 256 threads, 64 queries of one head: a wave owns 16 queries and walks the keys 32 at a time (16 heads of 64 at length 266:
+// 18 us, the time of 80 workgroups' chains of 9 steps; at 4000 rows 75 - 80 TFLOP/s, of 154 in a large product).  S^T = K Q^T puts the query
 // on the lane: its maximum and sum are in registers and two exchanges away, and the probabilities are the operand of
 // O^T = V^T P^T as they stand.
 template <int D>
@@ -337,7 +338,10 @@ __global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
 
 // ------------------------------------------------------------------------------------- forward, 16-bit operands
 // 256 threads, 128 queries of one head: a wave owns 32 queries (v_mfma_f32_32x32x16: twice the queries per fragment read from
-// LDS, which 16-row tiles are bound by) and walks the keys 64 at a time.
+// LDS, which 16-row tiles are bound by) and walks the keys 64 at a time.  bf16, 32 heads over 8 of 128: eight prompts of up to
+// 4097 in 304 us (855 TFLOP/s, of 1361 in a large matrix product), 1500 queries over 16001 keys in 381 us (984 TFLOP/s).  It is
+// bound by matrix and vector instructions together: a step's 32 exponentials and 100 others need nearly the time of its 16
+// products, and the clock sinks under both (on zeros the same instructions run 1.4 times as fast).
 template <int D>
 struct Tile32 {
   static constexpr int RB = 2 * D, CP = RB / 16, NKS = D / 16, DB = D / 32;
@@ -835,7 +839,7 @@ __global__ __launch_bounds__(256) void packed_dkv_f32_kernel(PackedParams p) {
 
 // ------------------------------------------------------------------------------------ backward, 16-bit operands
 // dq and delta: a wave owns 32 queries, 64 keys a step; K lies in LDS in the order its transposed reads want (its row reads
-// meet no bank twice in that order either)
+// meet no bank twice in that order either).  Three products, 16 heads over 4 of 128 as below: 205 us, 770 TFLOP/s.
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
   using L = Tile32<D>;
@@ -964,8 +968,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
 //   wave A, block n:  scores of block n and dv of block n - 1, then the probabilities of block n, left in LDS for B
 //   wave B, block n:  ds of block n - 1 from A's probabilities, then do . v of block n and dk of block n - 1
 // one barrier a block.  Three tiles of queries and output gradients lie in LDS (the last, this one, the one being stored).
-// The halves qh are added at the end, in LDS.  (One wave for both gradients, one to a SIMD, took 386 us where this takes less:
-// it issues every instruction of a block itself, and 400 of them need longer than its 32 products.)
+// The halves qh are added at the end, in LDS.  (One wave for both gradients, one to a SIMD, was as fast while tiles came through
+// registers, but it issues every instruction of a block itself, and 400 of them take longer than its 32 products.)
+// 16 heads over 4 of 128 in bf16, sequences of 4096, 265, 1999, 1, 800, 2050: 350 us for its four products (210 GFLOP), 600
+// TFLOP/s; what bounds it is LDS (fragments of four tiles and the probabilities' way from A to B) beside one block in flight.
 template <int D>
 __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   using L = Tile32<D>;

