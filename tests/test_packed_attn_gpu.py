@@ -323,6 +323,24 @@ def test_backward_through_a_broadcast_sum_and_one_input():
     assert float((total - 4 * 90).abs().max()) <= 4 * 90 * 2 * R.half_step(_half())
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_output_in_two_halves(D):
+    """out + low of sequences of up to 64 keys: probabilities and output in two 16-bit halves each (what the first half left
+    out rounded once more: h^2 of the sum of sizes and of the output), f32 otherwise"""
+    from melspec_gpt_vqvae_amd import ops
+
+    dt, lens, scale = _half(), [1, 2, 3, 4, 7, 33, 64, 64, 50], D ** -0.5
+    q, k, v, _ = make(lens, lens, 4, 2, D, dt, 8)
+    out, _, low = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), _cu(lens).to(DEV), want_low=True)
+    plain, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), _cu(lens).to(DEV))
+    both, tiny = out.double().cpu() + low.double().cpu(), R.smallest(dt)
+    h = R.half_step(dt)
+    for a, b, head, _, r in reference(q, k, v, lens, lens, scale):
+        rel = R.attention_relative(D, r["s_score"], b.stop - b.start, torch.float32)[:, None] + h * h
+        R.assert_within(both[a, head], r["o"], (h * h + 4 * R.U) * r["o"].abs() + rel * r["s_o"] + tiny * (2 + r["a_o"]), f"{a} {head}")
+    assert (out - plain).abs().max() <= 4 * h * v.abs().max()       # (two roundings of probabilities, two of the output)
+
+
 def test_rows_far_apart():
     """rows whose offsets pass 2^32 bytes: the same bits as from tensors side by side"""
     from melspec_gpt_vqvae_amd import ops
