@@ -40,6 +40,7 @@ struct NormRotaryParams {
   float amplitude, eps, inv_d;  // inv_d: 1 / D
   long long M;
   int D, rot, lp, hsplit;       // lanes per head; parts a row's steps are split into
+  int rows;                     // rows a wave takes at once (MULTI; a power of two)
   float* dw_part;               // backward: (blocks, 2, D) or null
   // ---- paged cache (append)
   const int *seq, *table;       // (M); (S, width)
@@ -128,8 +129,7 @@ __device__ __forceinline__ void cos_sin(int pos, const double* turns_per_pos, fl
   constexpr int N = V16<T>::N;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    double t = (double)pos * turns_per_pos[e];
-    t -= rint(t);
+    const double whole = rint((double)pos * turns_per_pos[e]), t = fma((double)pos, turns_per_pos[e], -whole);
     if constexpr (sizeof(T) == 2) {
       turn_sincos((float)t, s[e], c[e]);
     } else {
@@ -143,14 +143,16 @@ __device__ __forceinline__ void cos_sin(int pos, const double* turns_per_pos, fl
   }
 }
 
+// (products and sums are fused by hand here and below: left to hipcc, which of them it fuses differs between the kernels, and
+// a key would not have the same bits in a cache as outside)
 template <typename T, bool INTERLEAVED>
 __device__ __forceinline__ void turn(float* x, const float* c, const float* s) {
   using L = Lane<T, INTERLEAVED>;
 #pragma unroll
   for (int e = 0; e < L::N; ++e) {
     const float lo = x[L::lo(e)], hi = x[L::hi(e)];
-    x[L::lo(e)] = lo * c[e] - hi * s[e];
-    x[L::hi(e)] = hi * c[e] + lo * s[e];
+    x[L::lo(e)] = fmaf(lo, c[e], -(hi * s[e]));
+    x[L::hi(e)] = fmaf(hi, c[e], lo * s[e]);
   }
 }
 
@@ -161,19 +163,19 @@ __device__ __forceinline__ void turn_back(float* x, const float* c, const float*
 #pragma unroll
   for (int e = 0; e < L::N; ++e) {
     const float lo = x[L::lo(e)], hi = x[L::hi(e)];
-    x[L::lo(e)] = lo * c[e] + hi * s[e];
-    x[L::hi(e)] = hi * c[e] - lo * s[e];
+    x[L::lo(e)] = fmaf(lo, c[e], hi * s[e]);
+    x[L::hi(e)] = fmaf(hi, c[e], -(lo * s[e]));
   }
 }
 
-// One wave per item = (row, part of its steps), items strided over the grid.  PAGED: the keys go to their page, values
+// One wave per item = (row, part of its steps), or with MULTI per `rows` rows, items strided over the grid.  PAGED: the keys go to their page, values
 // are copied to theirs by further steps, and rows of negative position or sequence are padding.
-template <typename T, bool INTERLEAVED, bool NORM, bool PAGED>
+template <typename T, bool INTERLEAVED, bool NORM, bool PAGED, bool MULTI>
 __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p) {
   using L = Lane<T, INTERLEAVED>;
   constexpr int N = L::N, U = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lp = p.lp, hpw = 64 / lp, slot = lane / lp;
+  const int lp = p.lp, hpw = 64 / lp / (MULTI ? p.rows : 1), slot = MULTI ? lane / lp % hpw : lane / lp;
   const L at(lane % lp, p.D, p.rot);
   double freq[N];
 #pragma unroll
@@ -190,11 +192,13 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
   }
   const int nq = p.t[0].steps, nk = p.t[1].steps, total = nq + nk + (PAGED ? nk : 0);
   const int part = (total + p.hsplit - 1) / p.hsplit;
-  const long long items = p.M * p.hsplit, stride = (long long)gridDim.x * 4;
+  const long long items = MULTI ? (p.M + p.rows - 1) / p.rows : p.M * p.hsplit, stride = (long long)gridDim.x * 4;
   for (long long item = (long long)blockIdx.x * 4 + wave; item < items; item += stride) {
-    long long row = item;
+    long long row = MULTI ? item * p.rows + lane / lp / hpw : item;
     int s0 = 0, s1 = total;
-    if (p.hsplit > 1) {   // (few rows then: 32 bits do)
+    if constexpr (MULTI) {
+      if (row >= p.M) continue;   // (all lanes of a head)
+    } else if (p.hsplit > 1) {   // (few rows then: 32 bits do)
       row = (int)item / p.hsplit;
       s0 = ((int)item % p.hsplit) * part;
       s1 = min(s0 + part, total);
@@ -256,8 +260,8 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
           if constexpr (NORM) {
             float q = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2 * N; ++e) q += x[e] * x[e];
-            const float r = rsqrtf(head_sum(at.active ? q : 0.f, lp) * p.inv_d + p.eps);
+            for (int e = 0; e < 2 * N; ++e) q = fmaf(x[e], x[e], q);
+            const float r = rsqrtf(fmaf(head_sum(at.active ? q : 0.f, lp), p.inv_d, p.eps));
 #pragma unroll
             for (int e = 0; e < 2 * N; ++e) x[e] *= r * wt[e];
           }
@@ -284,12 +288,12 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
 // Backward: the same walk over rows and heads; the weights' gradients are summed per lane over all its rows, then over the
 // workgroup in LDS in a fixed order, and written as one row of partial sums per workgroup (reduced by melgpt_reduce_rows:
 // no atomics, the same bits every time).
-template <typename T, bool INTERLEAVED, bool NORM>
+template <typename T, bool INTERLEAVED, bool NORM, bool MULTI>
 __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(NormRotaryParams p) {
   using L = Lane<T, INTERLEAVED>;
   constexpr int N = L::N, U = 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lp = p.lp, hpw = 64 / lp, slot = lane / lp;
+  const int lp = p.lp, hpw = 64 / lp / (MULTI ? p.rows : 1), slot = MULTI ? lane / lp % hpw : lane / lp;
   const L at(lane % lp, p.D, p.rot);
   double freq[N];
 #pragma unroll
@@ -307,11 +311,13 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(NormRotaryParams p
   }
   const int nq = p.t[0].steps, total = nq + p.t[1].steps;
   const int part = (total + p.hsplit - 1) / p.hsplit;
-  const long long items = p.M * p.hsplit, stride = (long long)gridDim.x * 4;
+  const long long items = MULTI ? (p.M + p.rows - 1) / p.rows : p.M * p.hsplit, stride = (long long)gridDim.x * 4;
   for (long long item = (long long)blockIdx.x * 4 + wave; item < items; item += stride) {
-    long long row = item;
+    long long row = MULTI ? item * p.rows + lane / lp / hpw : item;
     int s0 = 0, s1 = total;
-    if (p.hsplit > 1) {   // (few rows then: 32 bits do)
+    if constexpr (MULTI) {
+      if (row >= p.M) continue;   // (all lanes of a head)
+    } else if (p.hsplit > 1) {   // (few rows then: 32 bits do)
       row = (int)item / p.hsplit;
       s0 = ((int)item % p.hsplit) * part;
       s1 = min(s0 + part, total);
@@ -351,19 +357,19 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(NormRotaryParams p
             V16<T>::to_f32(ra[u], x);
             V16<T>::to_f32(rb[u], x + N);
 #pragma unroll
-            for (int e = 0; e < 2 * N; ++e) q += x[e] * x[e];
-            const float r = rsqrtf(head_sum(at.active ? q : 0.f, lp) * p.inv_d + p.eps);
+            for (int e = 0; e < 2 * N; ++e) q = fmaf(x[e], x[e], q);
+            const float r = rsqrtf(fmaf(head_sum(at.active ? q : 0.f, lp), p.inv_d, p.eps));
             float m = 0.f;
 #pragma unroll
             for (int e = 0; e < 2 * N; ++e) {
               x[e] *= r;
               dwt[e] += mine ? g[e] * x[e] : 0.f;
               g[e] *= wt[e];
-              m += g[e] * x[e];
+              m = fmaf(g[e], x[e], m);
             }
             m = head_sum(at.active ? m : 0.f, lp) * p.inv_d;
 #pragma unroll
-            for (int e = 0; e < 2 * N; ++e) g[e] = r * (g[e] - x[e] * m);
+            for (int e = 0; e < 2 * N; ++e) g[e] = r * fmaf(-x[e], m, g[e]);
           }
           if (!mine) return;
           T* o = (T*)p.t[i].out + (row * p.t[i].H + h) * p.D;
@@ -423,48 +429,69 @@ int check_common(const NormRotaryParams& p, int dtype) {
   return MELGPT_OK;
 }
 
+// Where a wave has twice the room for all heads of a row or more, it takes 2, 4, .. rows at once while 2048 waves (2 a SIMD) of
+// them remain: a row's sines cost its wave as much as two passes of heads.  33920 rows in bf16, one row / several: 1 + 1 heads
+// of 64 40.8 / 8.9 us, of 256 43.8 / 20.5, 16 + 16 heads of 32 47 / 32; backward 69.5 / 25.1, 73.8 / 35.3, 82.7 / 56.9.
 // Steps of a row are shared out over several waves only while there are too few rows to fill the card (a part computes
 // the row's sines again): 2 waves for each SIMD of the 256 CUs.  Measured in bf16, 32 + 8 heads of 128, whole rows / this / 8
 // waves a SIMD: 1 row 6.0 / 4.0 / 3.9 us, 256 rows 6.8 / 5.3 / 5.3, 1024 rows 8.1 / 7.5 / 10.6.
 void plan(NormRotaryParams& p, int dtype, int steps_extra) {
   p.lp = lanes_per_head(p.D, dtype);
   p.inv_d = 1.f / (float)p.D;
-  const int hpw = 64 / p.lp;
+  int hpw = 64 / p.lp;
+  const int heads = p.t[0].H > p.t[1].H ? p.t[0].H : p.t[1].H;
+  p.rows = 1;
+  while (2 * heads <= hpw && p.M >= 4096LL * p.rows) {
+    p.rows *= 2;
+    hpw /= 2;
+  }
   for (int i = 0; i < 2; ++i) p.t[i].steps = (p.t[i].H + hpw - 1) / hpw;
   const int total = p.t[0].steps + p.t[1].steps + (steps_extra ? p.t[1].steps : 0);
   long long want = p.M > 0 ? (2048 + p.M - 1) / p.M : 1;
-  p.hsplit = (int)(want < 1 ? 1 : want > total ? total : want);
+  p.hsplit = (int)(want < 1 ? 1 : want > total ? total : want);   // (1 where a wave takes several rows)
 }
 
 long long blocks_for(const NormRotaryParams& p, long long most) {
-  const long long b = (p.M * p.hsplit + 3) / 4;
+  const long long b = ((p.rows > 1 ? (p.M + p.rows - 1) / p.rows : p.M * p.hsplit) + 3) / 4;
   return b < most ? b : most;
+}
+
+template <typename T, bool INTERLEAVED, bool NORM, bool PAGED>
+void launch_fwd_rows(const NormRotaryParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)blocks_for(p, 2048)), block(256);
+  if (p.rows > 1) hipLaunchKernelGGL((norm_rotary_fwd_kernel<T, INTERLEAVED, NORM, PAGED, true>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((norm_rotary_fwd_kernel<T, INTERLEAVED, NORM, PAGED, false>), grid, block, 0, s, p);
 }
 
 template <typename T, bool PAGED>
 void launch_fwd(const NormRotaryParams& p, int interleaved, hipStream_t s) {
-  const dim3 grid((unsigned)blocks_for(p, 2048)), block(256);
   const bool norm = p.t[1].w != nullptr;
   if (interleaved) {
-    if (norm) hipLaunchKernelGGL((norm_rotary_fwd_kernel<T, true, true, PAGED>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((norm_rotary_fwd_kernel<T, true, false, PAGED>), grid, block, 0, s, p);
+    if (norm) launch_fwd_rows<T, true, true, PAGED>(p, s);
+    else launch_fwd_rows<T, true, false, PAGED>(p, s);
   } else {
-    if (norm) hipLaunchKernelGGL((norm_rotary_fwd_kernel<T, false, true, PAGED>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((norm_rotary_fwd_kernel<T, false, false, PAGED>), grid, block, 0, s, p);
+    if (norm) launch_fwd_rows<T, false, true, PAGED>(p, s);
+    else launch_fwd_rows<T, false, false, PAGED>(p, s);
   }
+}
+
+template <typename T, bool INTERLEAVED, bool NORM>
+void launch_bwd_rows(const NormRotaryParams& p, unsigned blocks, hipStream_t s) {
+  const dim3 grid(blocks), block(256);
+  const size_t lds = NORM ? (size_t)(256 / p.lp) * p.D * sizeof(float) : 0;   // <= 256 * 2 N floats: 16 KB
+  if (p.rows > 1) hipLaunchKernelGGL((norm_rotary_bwd_kernel<T, INTERLEAVED, NORM, true>), grid, block, lds, s, p);
+  else hipLaunchKernelGGL((norm_rotary_bwd_kernel<T, INTERLEAVED, NORM, false>), grid, block, lds, s, p);
 }
 
 template <typename T>
 void launch_bwd(const NormRotaryParams& p, int interleaved, unsigned blocks, hipStream_t s) {
-  const dim3 grid(blocks), block(256);
   const bool norm = p.t[1].w != nullptr;
-  const size_t lds = norm ? (size_t)(256 / p.lp) * p.D * sizeof(float) : 0;   // <= 256 * 2 N floats: 16 KB
   if (interleaved) {
-    if (norm) hipLaunchKernelGGL((norm_rotary_bwd_kernel<T, true, true>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((norm_rotary_bwd_kernel<T, true, false>), grid, block, 0, s, p);
+    if (norm) launch_bwd_rows<T, true, true>(p, blocks, s);
+    else launch_bwd_rows<T, true, false>(p, blocks, s);
   } else {
-    if (norm) hipLaunchKernelGGL((norm_rotary_bwd_kernel<T, false, true>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((norm_rotary_bwd_kernel<T, false, false>), grid, block, 0, s, p);
+    if (norm) launch_bwd_rows<T, false, true>(p, blocks, s);
+    else launch_bwd_rows<T, false, false>(p, blocks, s);
   }
 }
 

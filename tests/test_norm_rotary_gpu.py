@@ -325,3 +325,54 @@ def test_captured_forward_and_backward_and_two_streams():
         want = run()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
+
+
+# few heads and many rows: a wave takes several rows at once (the last one fewer than it could)
+FEW_HEADS = [(4097, 1, 1, 128, 128), (8203, 2, 1, 80, 32), (16385, 1, 1, 32, 16), (4099, 16, 16, 32, 32), (4096, 1, 1, 256, 64),
+             (8195, 3, 3, 16, 16)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("M,Hq,Hk,D,rot", FEW_HEADS)
+def test_few_heads_many_rows(M, Hq, Hk, D, rot, interleaved, dtype):
+    check_forward(M, Hq, Hk, D, rot, interleaved, _dt(dtype), norm=not interleaved or D != 80)
+    check_backward(M, Hq, Hk, D, rot, interleaved, _dt(dtype), norm=not interleaved or D != 80)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+def test_append_few_heads_many_rows(dtype):
+    check_append(_dt(dtype), 1, 1, 64, 64, False, True, 16, [4000, 1, 300], [0, 100, 7])
+    check_append(_dt(dtype), 2, 1, 128, 32, True, True, 64, [8300], [3])
+    check_append(_dt(dtype), 1, 1, 80, 32, True, False, 32, [5000, 77], [1, 0], with_q=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+def test_append_few_heads_padding_among_rows(dtype):
+    """padding and rows that point outside, in the same wave as rows that do not"""
+    from melspec_gpt_vqvae_amd import ops
+
+    dt, M, D, page = _dt(dtype), 9000, 64, 16
+    g = torch.Generator().manual_seed(2)
+    q, k, v = [torch.randn(M, 1, D, generator=g).to(dt).to(DEV) for _ in range(3)]
+    P = -(-M // page)
+    kp, vp = [torch.randn(P, 1, page, D, generator=g).to(dt).to(DEV) for _ in range(2)]
+    table = torch.randperm(P, generator=g).to(torch.int32).view(1, P).to(DEV)
+    pos = torch.arange(M, dtype=torch.int32)
+    seq = torch.zeros(M, dtype=torch.int32)
+    pos[::7], seq[3::11], seq[5::13] = -1, -2, 9                     # padding, padding, no such sequence
+    pad = (pos < 0) | (seq < 0)
+    stored = ~pad & (seq == 0)
+    full_q, full_k = ops.qk_norm_rotary_fwd(q, k, pos.to(DEV), _freqs(64))
+    q_out = torch.full_like(q, 3.0)
+    want_k, want_v = kp.clone(), vp.clone()
+    at = pos[stored].long().to(DEV)
+    want_k[table[0].long()[at // page], 0, at % page] = full_k[stored.to(DEV), 0]
+    want_v[table[0].long()[at // page], 0, at % page] = v[stored.to(DEV), 0]
+    k1, v1 = kp.clone(), vp.clone()
+    ops.kv_append(k, v, k1, v1, table, seq.to(DEV), pos.to(DEV), q=q, freqs=_freqs(64), q_out=q_out)
+    assert torch.equal(k1, want_k) and torch.equal(v1, want_v)
+    p = pad.to(DEV)
+    assert torch.equal(q_out[~p], full_q[~p]) and (q_out[p] == 3.0).all()
+    new = ops.kv_append(k, v, kp, vp, table, seq.to(DEV), pos.to(DEV), q=q, freqs=_freqs(64))
+    assert torch.equal(new[~p], full_q[~p]) and (new[p] == 0).all()
