@@ -1195,7 +1195,8 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int check(const PackedParams& p, int D, int dtype) {
-  if (p.S < 0 || p.Hq <= 0 || p.Hk <= 0 || p.Mq < 0 || p.Mk < 0 || !p.cu_q || !p.cu_k) return MELGPT_ERR_BAD_ARG;
+  if (p.S < 0 || p.Hq <= 0 || p.Hk <= 0 || p.Mq < 0 || p.Mk < 0 || !p.cu_q || !p.cu_k || !__builtin_isfinite(p.scale))
+    return MELGPT_ERR_BAD_ARG;
   if (dtype != MELGPT_F32 && dtype != MELGPT_BF16) return MELGPT_ERR_UNSUPPORTED;
   if ((D != 64 && D != 128) || p.Hq % p.Hk) return MELGPT_ERR_UNSUPPORTED;
   // tile numbers and row numbers are 32-bit, a grid's second dimension ends at 65535

@@ -308,7 +308,8 @@ extern "C" int melgpt_paged_attn_decode(const void* q, long long q_row, long lon
                                         long long o_head, float* lse, int splits, float* workspace, int Hq, int Hk, int D,
                                         float scale, int dtype, void* stream) {
   if (S == 0) return MELGPT_OK;
-  if (S < 0 || Hq <= 0 || Hk <= 0 || width <= 0 || n_pages <= 0 || splits <= 0 || page_size <= 0) return MELGPT_ERR_BAD_ARG;
+  if (S < 0 || Hq <= 0 || Hk <= 0 || width <= 0 || n_pages <= 0 || splits <= 0 || page_size <= 0 || !__builtin_isfinite(scale))
+    return MELGPT_ERR_BAD_ARG;
   if (!q || !k_pages || !v_pages || !page_table || !lengths || !out || !lse || (splits > 1 && !workspace)) return MELGPT_ERR_BAD_ARG;
   if (dtype != MELGPT_F32 && dtype != MELGPT_BF16) return MELGPT_ERR_UNSUPPORTED;
   if ((D != 64 && D != 128) || Hq % Hk || (page_size & (page_size - 1)) || page_size > (1 << 20) || n_pages > 0x7fffffffLL ||

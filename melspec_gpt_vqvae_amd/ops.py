@@ -1124,6 +1124,7 @@ def kv_append(k, v, k_pages, v_pages, page_table, sequences, positions, *, q=Non
     dt = dtype_code(k.dtype)
     P, Hkp, page, Dp = _pages_of(i, k_pages, v_pages, page_table, k.dtype)
     assert (Hkp, Dp) == (Hk, D), (k_pages.shape, k.shape)
+    assert k_pages.data_ptr() != v_pages.data_ptr() or k_pages.numel() == 0, "keys and values want pages of their own"
     assert sequences.dtype == torch.int32 and sequences.shape == (M,) and sequences.is_contiguous(), "sequences: (rows,) int32"
     vec = 4 if dt == _ffi.F32 else 8
     _same_device(i, v, q, q_out, sequences)

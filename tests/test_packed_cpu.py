@@ -62,9 +62,9 @@ def test_append_refusals(kw, code):
 
 
 def packed(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF,
-           low=None, splits=1, ws=None):
+           low=None, splits=1, ws=None, scale=0.125):
     return _lib().melgpt_packed_attn_fwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, lse, 1, splits, ws, Mq, Mk, Hq,
-                                         Hk, D, 0.125, dt, None)
+                                         Hk, D, scale, dt, None)
 
 
 PACKED_REFUSALS = [
@@ -84,9 +84,9 @@ def test_packed_refusals(kw, code):
 
 
 def packed_bwd(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF,
-               do=P, dor=512, delta=P, dq=P, dqr=512, dk=P, dv=P, low=P):
+               do=P, dor=512, delta=P, dq=P, dqr=512, dk=P, dv=P, low=P, scale=0.125):
     return _lib().melgpt_packed_attn_bwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, do, dor, 64, lse, delta, dq, dqr, 64,
-                                         dk, 256, 64, dv, 256, 64, 1, Mq, Mk, Hq, Hk, D, 0.125, dt, None)
+                                         dk, 256, 64, dv, 256, 64, 1, Mq, Mk, Hq, Hk, D, scale, dt, None)
 
 
 @pytest.mark.parametrize("kw,code", [r for r in PACKED_REFUSALS if "Mq" not in r[0] or r[0]["Mq"] < 0] + [
@@ -97,9 +97,9 @@ def test_packed_bwd_refusals(kw, code):
 
 
 def decode(q=P, qr=512, kp=P, vp=P, pages=9, page=16, table=P, width=4, lens=P, S=2, o=P, orow=512, lse=P, splits=1, ws=None, Hq=8,
-           Hk=4, D=64, dt=HALF):
+           Hk=4, D=64, dt=HALF, scale=0.125):
     return _lib().melgpt_paged_attn_decode(q, qr, 64, kp, vp, pages, page, table, width, width, lens, S, o, orow, 64, lse, splits, ws, Hq,
-                                           Hk, D, 0.125, dt, None)
+                                           Hk, D, scale, dt, None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -110,6 +110,11 @@ def decode(q=P, qr=512, kp=P, vp=P, pages=9, page=16, table=P, width=4, lens=P, 
     (dict(q=P + 8), ALIGN), (dict(orow=4), ALIGN), (dict(vp=P + 8), ALIGN)])
 def test_decode_refusals(kw, code):
     assert decode(**kw) == code
+
+
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan])
+def test_scales_that_are_not_finite_are_refused(scale):
+    assert packed(scale=scale) == packed_bwd(scale=scale) == decode(scale=scale) == BAD
 
 
 def test_splits():
