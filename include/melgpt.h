@@ -585,7 +585,8 @@ int melgpt_kv_append(const void* q, long long q_row, long long q_head, const voi
  * write_gaps: rows of the outputs that no sequence owns are zeroed (lse -inf), otherwise left as they were.
  * splits: workgroups that share a row tile's keys (16-bit lane without out_low; 1: one), joined in a fixed order by a second
  * kernel; melgpt_packed_attn_splits proposes it from the sizes.  With splits > 1 `workspace` holds splits * Hq * Mq * (D + 2)
- * f32, 16-byte aligned.
+ * f32, 16-byte aligned.  The backward's splits (melgpt_packed_attn_bwd_splits) share a key tile's query heads in the same
+ * way, with 2 * splits * Mk * Hk * D f32.
  * D 64 or 128; scale multiplies the scores; at most 4 M rows (65535 tiles of 64 with one more per sequence). */
 int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int Hq, int D, int dtype);
 int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
@@ -597,8 +598,9 @@ int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, con
                            const void* out, long long o_row, long long o_head, const void* out_low, const void* dout, long long do_row,
                            long long do_head, const float* lse, float* delta, void* dq, long long dq_row, long long dq_head,
                            void* dk, long long dk_row, long long dk_head, void* dv, long long dv_row, long long dv_head,
-                           int write_gaps, long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype,
-                           void* stream);
+                           int write_gaps, int splits, float* workspace, long long Mq, long long Mk, int Hq, int Hk, int D,
+                           float scale, int dtype, void* stream);
+int melgpt_packed_attn_bwd_splits(long long Mk, int S, int Hq, int Hk, int dtype);
 
 /* Attention of one query token per sequence over the cache that melgpt_kv_append fills: q, out (S, Hq, D) with row and head
  * strides, keys 0 .. lengths[s] - 1 of sequence s through page_table[s * table_ld + j / page_size] (columns beyond `width`

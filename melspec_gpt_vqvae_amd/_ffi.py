@@ -137,8 +137,9 @@ _PROTOS = {
                          _l, _i, _l, _i, _i, _i, _i, _p],
     "melgpt_packed_attn_splits": [_l, _l, _i, _i, _i, _i],
     "melgpt_packed_attn_fwd": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _i, _p, _l, _l, _p, _p, _i, _i, _p, _l, _l, _i, _i, _i, _f, _i, _p],
-    "melgpt_packed_attn_bwd": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _i, _p, _l, _l, _p, _p, _l, _l, _p, _p, _p, _l, _l, _p, _l, _l,
-                               _p, _l, _l, _i, _l, _l, _i, _i, _i, _f, _i, _p],
+    "melgpt_packed_attn_bwd": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _i, _p, _l, _l, _p, _p, _l, _l, _p, _p, _p, _l, _l, _p,
+                               _l, _l, _p, _l, _l, _i, _i, _p, _l, _l, _i, _i, _i, _f, _i, _p],
+    "melgpt_packed_attn_bwd_splits": [_l, _i, _i, _i, _i],
     "melgpt_paged_attn_splits": [_i, _i, _i, _l],
     "melgpt_paged_attn_decode": [_p, _l, _l, _p, _p, _l, _i, _p, _l, _i, _p, _i, _p, _l, _l, _p, _i, _p, _i, _i, _i, _f, _i, _p],
     "melgpt_groupnorm_swish_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p],

@@ -35,8 +35,9 @@ struct PackedParams {
   long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
   float *lse, *delta;            // (Hq, Mq)
   const int *cu_q, *cu_k;        // (S + 1)
-  int splits;                    // forward, 16-bit: workgroups that share a row tile's keys
-  float* part;                   // splits > 1: (splits, Hq, Mq, D) sums of e^(s - m) v, then (splits, Hq, Mq, 2): m (base 2), sums
+  int splits;                    // 16-bit: workgroups that share a row tile's keys (forward) or a key tile's query heads (backward)
+  float* part;                   // splits > 1: (splits, Hq, Mq, D) sums of e^(s - m) v, then (splits, Hq, Mq, 2): m (base 2), sums;
+                                 // backward: (splits, [dk, dv], Mk, Hk, D)
   int S, Hq, Hk, G, write_gaps;  // write_gaps: zero the rows no sequence owns
   long long Mq, Mk;
   float scale;
@@ -1025,16 +1026,18 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   f32x16 grad[L::DB];                                              // A: dv, B: dk
 #pragma unroll
   for (int d = 0; d < L::DB; ++d) grad[d] = zero16();
-  const int blocks = first < nq ? (nq - first + 63) / 64 : 0, total = blocks * p.G;
+  // this workgroup's share of the key head's query heads
+  const int heads = (p.G + p.splits - 1) / p.splits, h0 = hk * p.G + heads * (int)blockIdx.z;
+  const int blocks = first < nq ? (nq - first + 63) / 64 : 0, total = blocks * min(heads, p.G - heads * (int)blockIdx.z);
   if (total > 0) {
     // Tiles in order: head by head, the queries from the last down.  Addresses and sizes of the tile to load next are kept as
     // running scalars.  Wave parity picks the row of statistics (lse, delta) a wave fetches; waves of a parity store the same.
     const Fetch64<D, true, 8> fetch_q(p.q_row, wave, lane), fetch_g(p.do_row, wave, lane);
     const int top = first + 64 * (blocks - 1), st_row = wave & 1;
-    const long long q_at = (long long)(q_lo + top) * p.q_row + (long long)hk * p.G * p.q_head;
-    const long long g_at = (long long)(q_lo + top) * p.do_row + (long long)hk * p.G * p.do_head;
+    const long long q_at = (long long)(q_lo + top) * p.q_row + (long long)h0 * p.q_head;
+    const long long g_at = (long long)(q_lo + top) * p.do_row + (long long)h0 * p.do_head;
     const T *qa = (const T*)p.q + q_at, *ga = (const T*)p.dout + g_at;
-    const float* sa = (st_row ? p.delta : p.lse) + (long long)hk * p.G * p.Mq + q_lo + top;
+    const float* sa = (st_row ? p.delta : p.lse) + (long long)h0 * p.Mq + q_lo + top;
     const long long q_down = 64 * p.q_row, g_down = 64 * p.do_row, q_next = (long long)(top - first) * p.q_row + p.q_head,
                     g_next = (long long)(top - first) * p.do_row + p.do_head, s_next = top - first + p.Mq;
     const unsigned rest = (unsigned)min(nq - top, 64);             // rows of a head's last tile
@@ -1180,6 +1183,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   __syncthreads();
   if (qh == 1 || k_in >= nk) return;
   T* out = second ? (T*)p.dk + row * p.dk_row + hk * p.dk_head : (T*)p.dv + row * p.dv_row + hk * p.dv_head;
+  float* part = p.splits > 1 ? p.part + ((((long long)blockIdx.z * 2 + !second) * p.Mk + row) * p.Hk + hk) * D : nullptr;
   const float f = second ? p.scale : 1.f;
 #pragma unroll
   for (int d = 0; d < L::DB; ++d)
@@ -1188,8 +1192,27 @@ __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
       f32x4 x;
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = (grad[d][4 * j + r] + room[(16 * d + 4 * j + r) * 64 + lane]) * f;
-      store4<T>(out + 32 * d + 8 * j + 4 * hh, x);
+      if (part) *(f32x4*)(part + 32 * d + 8 * j + 4 * hh) = x;
+      else store4<T>(out + 32 * d + 8 * j + 4 * hh, x);
     }
+}
+
+// adds the shares of a key's gradients in their order: D / 4 lanes, four values each
+template <int D>
+__global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedParams p) {
+  using T = bf16_t;
+  constexpr int TPK = D / 4;
+  const long long all = p.Mk * p.Hk, n = (long long)blockIdx.x * (256 / TPK) + threadIdx.x / TPK;
+  if (n >= 2 * all) return;
+  const bool v = n >= all;
+  const long long at = v ? n - all : n, row = at / p.Hk;
+  const int d = 4 * (threadIdx.x % TPK), hk = (int)(at % p.Hk);
+  const bool gap = row < bound_at(p.cu_k, p.S, p.Mk, 1) || row >= bound_at(p.cu_k, p.S, p.Mk, p.S + 1);
+  if (gap && !p.write_gaps) return;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < p.splits; ++i) a += *(const f32x4*)(p.part + (2 * i * all + n) * D + d);
+  store4<T>((v ? (T*)p.dv + row * p.dv_row + hk * p.dv_head : (T*)p.dk + row * p.dk_row + hk * p.dk_head) + d, a);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1239,7 +1262,12 @@ int launch_bwd(const PackedParams& p, hipStream_t s) {
   const dim3 gq(p.Hq, (unsigned)tq), gk(p.Hk, (unsigned)tk);
   if constexpr (sizeof(T) == 2) {
     if (p.Mq > 0) hipLaunchKernelGGL((packed_dq32_kernel<D>), gq, dim3(256), 0, s, p);
-    if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv32_kernel<D>), gk, dim3(512), 0, s, p);
+    if (p.Mk > 0) {
+      hipLaunchKernelGGL((packed_dkv32_kernel<D>), dim3(p.Hk, (unsigned)tk, (unsigned)p.splits), dim3(512), 0, s, p);
+      const long long per = 256 / (D / 4);
+      if (p.splits > 1)
+        hipLaunchKernelGGL((packed_dkv_join_kernel<D>), dim3((unsigned)((2 * p.Hk * p.Mk + per - 1) / per)), dim3(256), 0, s, p);
+    }
   } else {
     if (p.Mq > 0) hipLaunchKernelGGL((packed_dq_f32_kernel<D>), gq, dim3(256), 0, s, p);
     if (p.Mk > 0) hipLaunchKernelGGL((packed_dkv_f32_kernel<D>), gk, dim3(256), 0, s, p);
@@ -1294,12 +1322,22 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
   return D == 64 ? launch_fwd<bf16_t, 64>(p, s) : launch_fwd<bf16_t, 128>(p, s);
 }
 
+// Workgroups that share a key tile's query heads, where the key tiles alone (one workgroup a CU) would not fill the card twice:
+// one key head of 128 under 8, 4000 tokens, whole backward: 596 us in one piece, 238 in 8; two under 16: 647 / 379 in 4; four
+// under 16, 4096 tokens: 409 / 326 in 2.  Beyond twice the card it loses: eight under 32 heads of 64, 4000 tokens 344 / 360.
+extern "C" int melgpt_packed_attn_bwd_splits(long long Mk, int S, int Hq, int Hk, int dtype) {
+  if (dtype != MELGPT_BF16 || Mk <= 0 || S <= 0 || Hk <= 0 || Hq <= Hk) return 1;
+  const long long base = Hk * ((Mk + 63) / 64 + (S - 1) / 2), n = 512 / base;
+  return (int)(n < 1 ? 1 : n > Hq / Hk ? Hq / Hk : n);
+}
+
 extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
                                       long long k_head, const void* v, long long v_row, long long v_head, const int* cu_q,
                                       const int* cu_k, int S, const void* out, long long o_row, long long o_head, const void* out_low,
                                       const void* dout, long long do_row, long long do_head, const float* lse, float* delta,
                                       void* dq, long long dq_row, long long dq_head, void* dk, long long dk_row,
-                                      long long dk_head, void* dv, long long dv_row, long long dv_head, int write_gaps,
+                                      long long dk_head, void* dv, long long dv_row, long long dv_head, int write_gaps, int splits,
+                                      float* workspace,
                                       long long Mq, long long Mk, int Hq, int Hk, int D, float scale, int dtype, void* stream) {
   PackedParams p = {};
   p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head;
@@ -1313,6 +1351,10 @@ extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long 
   if (e) return e;
   if (Mq > 0 && (!dout || !delta || !dq)) return MELGPT_ERR_BAD_ARG;
   if (Mk > 0 && (!dk || !dv)) return MELGPT_ERR_BAD_ARG;
+  if (splits < 1 || (splits > 1 && !workspace)) return MELGPT_ERR_BAD_ARG;
+  if (splits > 1 && (dtype == MELGPT_F32 || splits > 1024 || Hk * Mk > (1LL << 25))) return MELGPT_ERR_UNSUPPORTED;
+  if (!aligned16(workspace)) return MELGPT_ERR_ALIGN;
+  p.splits = splits; p.part = workspace;
   if ((Mq > 1 && do_row < D) || do_row > (1 << 24)) return MELGPT_ERR_UNSUPPORTED;
   const int vec = dtype == MELGPT_F32 ? 4 : 8;
   if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_row % vec || do_head % vec || dq_row % vec ||

@@ -1240,10 +1240,13 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
         _into(dv, v, q, k, v, out, dout)
         _same_device(i, dq, dk, dv)
     delta = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
+    splits, ws = _ffi.lib().melgpt_packed_attn_bwd_splits(Mk, S, Hq, Hk, dt), None
+    if splits > 1:
+        ws = torch.empty(2 * splits * Mk * Hk * D, dtype=torch.float32, device=q.device)
     call("melgpt_packed_attn_bwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),
          cu_k.data_ptr(), S, out.data_ptr(), our, ouh, _addr(low), dout.data_ptr(), dor, doh, lse.data_ptr(), delta.data_ptr(), dq.data_ptr(),
-         dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0), dv.stride(1), gaps, Mq,
-         Mk, Hq, Hk, D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
+         dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0), dv.stride(1), gaps,
+         splits, _addr(ws), Mq, Mk, Hq, Hk, D, D ** -0.5 if scale is None else scale, dt, _raw_stream(i))
     return dq, dk, dv
 
 

@@ -31,10 +31,12 @@ def main():
     pa.test_few_queries_over_many_keys()
     print("packed attention ok", flush=True)
     pa.test_output_in_two_halves(64)
+    pa.test_backward_with_few_key_heads(7, 1, 64)
     pg.check([300, 0, 128, 129, 1, 1100, 256], 7, 1, 128, 32, H, seed=3, extra_width=100)
     for D in (64, 128):
         pg.check([0, 1, 31, 129, 0, 500], 16, 2, D, 16, H)
         pa.test_output_in_two_halves(64)
+    pa.test_backward_with_few_key_heads(7, 1, 64)
     pg.check([3000], 7, 1, D, 64, H)
     pg.test_prompt_then_tokens("half")
     print("all ok", flush=True)

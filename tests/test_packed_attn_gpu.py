@@ -341,6 +341,26 @@ def test_output_in_two_halves(D):
     assert (out - plain).abs().max() <= 4 * h * v.abs().max()       # (two roundings of probabilities, two of the output)
 
 
+@pytest.mark.parametrize("Hq,Hk,D", [(7, 1, 64), (8, 2, 128), (5, 1, 128)])
+def test_backward_with_few_key_heads(Hq, Hk, D):
+    """query heads of a key head shared out over workgroups; rows no sequence owns; a given buffer with strides"""
+    from melspec_gpt_vqvae_amd import _ffi, ops
+
+    lens_q, lens_k = [130, 1, 64, 0, 20], [150, 3, 64, 70, 10]
+    check(lens_q, lens_k, Hq, Hk, D, _half(), seed=9)
+    assert _ffi.lib().melgpt_packed_attn_bwd_splits(sum(lens_k), len(lens_k), Hq, Hk, 1) > 1
+    q, k, v, do = [x.to(DEV) for x in make(lens_q + [9], lens_k + [33], Hq, Hk, D, _half(), 9)]
+    cu_q, cu_k = _cu(lens_q).to(DEV), _cu(lens_k).to(DEV)            # 9 and 33 rows behind the last sequence
+    for x, n in ((q, 9), (k, 33), (v, 33), (do, 9)):
+        x[-n:] = float("nan")
+    out, lse = ops.packed_attn_fwd(q, k, v, cu_q, cu_k)
+    new = ops.packed_attn_bwd(q, k, v, out, do, lse, cu_q, cu_k)
+    room = torch.full((k.shape[0], 2, Hk, D), 3.0, dtype=q.dtype, device=DEV)
+    given = ops.packed_attn_bwd(q, k, v, out, do, lse, cu_q, cu_k, grads=(torch.empty_like(q), room[:, 0], room[:, 1]))
+    for a, b in zip(new[1:], given[1:]):
+        assert torch.isfinite(a).all() and torch.equal(a[:-33], b[:-33]) and (a[-33:] == 0).all() and (b[-33:] == 3.0).all()
+
+
 def test_rows_far_apart():
     """rows whose offsets pass 2^32 bytes: the same bits as from tensors side by side"""
     from melspec_gpt_vqvae_amd import ops

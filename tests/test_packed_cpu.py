@@ -84,14 +84,16 @@ def test_packed_refusals(kw, code):
 
 
 def packed_bwd(q=P, qr=512, k=P, kr=512, v=P, vr=512, cq=P, ck=P, S=2, o=P, orow=512, lse=P, Mq=100, Mk=100, Hq=8, Hk=4, D=64, dt=HALF,
-               do=P, dor=512, delta=P, dq=P, dqr=512, dk=P, dv=P, low=P, scale=0.125):
+               do=P, dor=512, delta=P, dq=P, dqr=512, dk=P, dv=P, low=P, scale=0.125, splits=1, ws=None):
     return _lib().melgpt_packed_attn_bwd(q, qr, 64, k, kr, 64, v, vr, 64, cq, ck, S, o, orow, 64, low, do, dor, 64, lse, delta, dq, dqr, 64,
-                                         dk, 256, 64, dv, 256, 64, 1, Mq, Mk, Hq, Hk, D, scale, dt, None)
+                                         dk, 256, 64, dv, 256, 64, 1, splits, ws, Mq, Mk, Hq, Hk, D, scale, dt, None)
 
 
 @pytest.mark.parametrize("kw,code", [r for r in PACKED_REFUSALS if "Mq" not in r[0] or r[0]["Mq"] < 0] + [
     (dict(do=None), BAD), (dict(delta=None), BAD), (dict(dq=None), BAD), (dict(dk=None), BAD), (dict(dv=None), BAD),
-    (dict(dor=32), UNSUPPORTED), (dict(Mq=1 << 23), UNSUPPORTED), (dict(dq=P + 8), ALIGN), (dict(dqr=513), ALIGN), (dict(do=P + 4), ALIGN)])
+    (dict(dor=32), UNSUPPORTED), (dict(Mq=1 << 23), UNSUPPORTED), (dict(dq=P + 8), ALIGN), (dict(dqr=513), ALIGN), (dict(do=P + 4), ALIGN),
+    (dict(splits=0), BAD), (dict(splits=2), BAD), (dict(splits=2, ws=P, dt=F32, low=None), UNSUPPORTED), (dict(splits=2000, ws=P), UNSUPPORTED),
+    (dict(splits=2, ws=P + 4), ALIGN)])
 def test_packed_bwd_refusals(kw, code):
     assert packed_bwd(**kw) == code
 
@@ -129,6 +131,12 @@ def test_packed_splits():
     f = _lib().melgpt_packed_attn_splits
     assert f(1500, 16001, 1, 32, 128, F32) == 1 and f(100, 100, 1, 16, 64, HALF) == 1 and f(30000, 30000, 1, 32, 128, HALF) == 1
     assert f(1, 16000, 1, 32, 128, HALF) > 4 and 1 < f(1500, 16001, 1, 32, 128, HALF) <= 16 and f(0, 5, 1, 1, 64, HALF) == 1
+
+
+def test_packed_bwd_splits():
+    f = _lib().melgpt_packed_attn_bwd_splits
+    assert f(4000, 1, 8, 8, HALF) == f(4000, 1, 8, 1, F32) == f(0, 1, 8, 1, HALF) == f(100000, 1, 8, 1, HALF) == 1
+    assert f(4000, 1, 8, 1, HALF) == 8 and f(200, 3, 7, 1, HALF) == 7 and 1 < f(4000, 1, 32, 2, HALF) < 16
 
 
 def test_cpu_tensors_and_wrong_arguments_are_refused():
