@@ -1,0 +1,69 @@
+"""Packed and cached sequence operators at the edges of what their documentation allows."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _dt(name):
+    from melspec_gpt_vqvae_amd import _ffi
+
+    return torch.float32 if name == "f32" else _ffi.HALF_DTYPE
+
+
+def _bits(x):
+    """bits of a tensor, every NaN alike (its payload is the conversion's)"""
+    x = torch.where(torch.isnan(x), torch.full_like(x, float("nan")), x).contiguous()
+    return x.view(torch.int16 if x.element_size() == 2 else torch.int32)
+
+
+# ------------------------------------------------------------------------------- values beyond the rotated part of a head
+def _with_odd_values(M, H, D, rot, dtype, seed):
+    """-> a finite tensor and the same with infinities, NaN and negative zeros scattered over the values beyond `rot`"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, H, D, generator=g)
+    y = x.clone()
+    where = torch.rand(M, H, D, generator=g) < 0.1
+    where[..., :rot] = False
+    where[0, 0, D - 1] = where[M - 1, H - 1, rot] = True
+    odd = torch.tensor([float("inf"), float("-inf"), float("nan"), -0.0])
+    y[where] = odd[torch.randint(0, 4, (int(where.sum()),), generator=g)]
+    return x.to(dtype).to(DEV), y.to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("M,Hq,Hk,D,rot", [(5, 3, 2, 64, 32), (5, 3, 2, 64, 0), (4, 2, 1, 128, 16), (3, 1, 1, 80, 48), (8200, 1, 1, 64, 32)])
+def test_values_beyond_the_rotation_pass_unchanged(M, Hq, Hk, D, rot, interleaved, dtype):
+    """without a norm: the bits of every value beyond `rot`, whatever lies beside it, and the rotated values as if the others
+    were finite; forward, backward and on the way into a cache"""
+    from melspec_gpt_vqvae_amd import ops
+    from melspec_gpt_vqvae_amd.transformer.packed import rotary_freqs
+
+    dt, page = _dt(dtype), 16
+    f = rotary_freqs(rot, device=DEV) if rot else None
+    pos = (3 + torch.arange(M, device=DEV)).to(torch.int32)
+    (q, q_odd), (k, k_odd) = _with_odd_values(M, Hq, D, rot, dt, 1), _with_odd_values(M, Hk, D, rot, dt, 2)
+
+    def right(got, x, finite):
+        assert torch.equal(_bits(got[..., rot:]), _bits(x[..., rot:]))
+        assert torch.equal(_bits(got[..., :rot]), _bits(finite[..., :rot]))
+
+    base = ops.qk_norm_rotary_fwd(q, k, pos, f, interleaved=interleaved)
+    got = ops.qk_norm_rotary_fwd(q_odd, k_odd, pos, f, interleaved=interleaved)
+    for a, b, c in zip(got, (q_odd, k_odd), base):
+        right(a, b, c)
+    base_g = ops.qk_norm_rotary_bwd(q, k, q, k, pos, f, interleaved=interleaved)
+    got_g = ops.qk_norm_rotary_bwd(q_odd, k_odd, q, k, pos, f, interleaved=interleaved)
+    for a, b, c in zip(got_g[:2], (q_odd, k_odd), base_g):
+        right(a, b, c)
+    pages = -(-(M + 3) // page)
+    kp, vp = [torch.zeros(pages, Hk, page, D, dtype=dt, device=DEV) for _ in range(2)]
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    qo = ops.kv_append(k_odd, k_odd, kp, vp, table, torch.zeros(M, dtype=torch.int32, device=DEV), pos, q=q_odd, freqs=f,
+                       interleaved=interleaved)
+    right(qo, q_odd, base[0])
+    p = pos.long()
+    right(kp[p // page, :, p % page], k_odd, base[1])
+    assert torch.equal(_bits(vp[p // page, :, p % page]), _bits(k_odd))
