@@ -582,7 +582,8 @@ int melgpt_kv_append(const void* q, long long q_row, long long q_head, const voi
  * the natural log of the scores' exponential sum; scratch that the backward fills with sum_d dout * out.
  * out_low (16-bit lane, optional, (Mq, Hq, D) contiguous): what the rounding of out took away, written by the forward and,
  * given to the backward, restored in its delta.
- * write_gaps: rows of the outputs that no sequence owns are zeroed (lse -inf), otherwise left as they were.
+ * write_gaps: 1: rows of the outputs that no sequence owns are zeroed (lse -inf); 0: they are left as they were; 2 (forward):
+ * zeroed in lse (-inf) and out_low, left in out.
  * splits: workgroups that share a row tile's keys (16-bit lane without out_low; 1: one), joined in a fixed order by a second
  * kernel; melgpt_packed_attn_splits proposes it from the sizes.  With splits > 1 `workspace` holds splits * Hq * Mq * (D + 2)
  * f32, 16-byte aligned.  The backward's splits (melgpt_packed_attn_bwd_splits) share a key tile's query heads in the same

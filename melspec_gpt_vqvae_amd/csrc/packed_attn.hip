@@ -38,7 +38,7 @@ struct PackedParams {
   int splits;                    // 16-bit: workgroups that share a row tile's keys (forward) or a key tile's query heads (backward)
   float* part;                   // splits > 1: (splits, Hq, Mq, D) sums of e^(s - m) v, then (splits, Hq, Mq, 2): m (base 2), sums;
                                  // backward: (splits, [dk, dv], Mk, Hk, D)
-  int S, Hq, Hk, G, write_gaps;  // write_gaps: zero the rows no sequence owns
+  int S, Hq, Hk, G, write_gaps;  // write_gaps: zero the rows no sequence owns (2: those of lse and low, not of o)
   long long Mq, Mk;
   float scale;
 };
@@ -332,8 +332,10 @@ __global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
   if (!mine) return;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;        // (NaN stays NaN)
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
+  if (p.write_gaps < 2 || (R.seq >= 0 && R.seq < p.S)) {
 #pragma unroll
-  for (int d = 0; d < L::DT; ++d) store4<T>(op + 16 * d + 4 * g, o[d] * inv);
+    for (int d = 0; d < L::DT; ++d) store4<T>(op + 16 * d + 4 * g, o[d] * inv);
+  }
   if (g == 0) p.lse[h * p.Mq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
@@ -629,11 +631,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
+  if (p.write_gaps < 2 || (R.seq >= 0 && R.seq < p.S)) {
 #pragma unroll
-  for (int d = 0; d < L::DB; ++d)
+    for (int d = 0; d < L::DB; ++d)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      store4<T>(op + 32 * d + 8 * j + 4 * hh, f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv);
+      for (int j = 0; j < 4; ++j)
+        store4<T>(op + 32 * d + 8 * j + 4 * hh, f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv);
+  }
   if (p.low) {   // the backward's delta = do . o loses a rounding of o against ds' own size; with both halves it does not
     T* lp = (T*)p.low + (row * p.Hq + h) * D;
 #pragma unroll
@@ -673,7 +677,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
     sum += st[2 * i * all + 1] * f;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  store4<T>((T*)p.o + row * p.o_row + h * p.o_head + d, a * inv);
+  if (!gap || p.write_gaps < 2) store4<T>((T*)p.o + row * p.o_row + h * p.o_head + d, a * inv);
   if (d == 0) p.lse[n] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 

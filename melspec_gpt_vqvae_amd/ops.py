@@ -1177,9 +1177,9 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
     cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
     -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  `out`, where given, is a buffer of its own.  Rows behind the last sequence: left
-    as they were in a given `out`, zero in a new one.  scale: 1 / sqrt(D) unless given.  want_low: -> (out, lse, low), low
-    what rounding out to 16 bits took from it (None for f32), for packed_attn_bwd.  Values that are not finite reach the
-    queries that see them and no others."""
+    as they were in a given `out`, zero in a new one (lse -inf, low 0).  scale: 1 / sqrt(D) unless given.  want_low: -> (out,
+    lse, low), low what rounding out to 16 bits took from it (None for f32), for packed_attn_bwd.  Values that are not finite
+    reach the queries that see them and no others."""
     i = _device_of(q)
     if i != _current_device():
         return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out, want_low=want_low)
@@ -1189,8 +1189,8 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     q, qr, qh = _heads(q, vec)
     k, kr, kh = _heads(k, vec)
     v, vr, vh = _heads(v, vec)
-    gaps = out is None
-    if gaps:
+    gaps = 1 if out is None else 2
+    if out is None:
         out = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)
     else:
         _into(out, q, q, k, v)

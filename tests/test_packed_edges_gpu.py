@@ -67,3 +67,35 @@ def test_values_beyond_the_rotation_pass_unchanged(M, Hq, Hk, D, rot, interleave
     p = pos.long()
     right(kp[p // page, :, p % page], k_odd, base[1])
     assert torch.equal(_bits(vp[p // page, :, p % page]), _bits(k_odd))
+
+
+# --------------------------------------------------------------------------------------- rows that no sequence owns
+def _poisoned(*shapes_and_types):
+    """leaves freed blocks of these sizes, full of sevens, to the allocator"""
+    keep = [torch.full(s, 7.0, dtype=t, device=DEV) for s, t in shapes_and_types for _ in range(3)]
+    del keep
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("lens_q,lens_k", [([10, 50, 131], [10, 50, 131]), ([4, 20], [50, 2080])])   # (the second: keys shared)
+def test_log_sums_of_rows_that_no_sequence_owns(lens_q, lens_k, dtype):
+    """with a buffer for the output its rows of nobody stay as they were; the new tensors beside it are defined there too"""
+    from melspec_gpt_vqvae_amd import ops
+
+    dt, Mq, Mk = _dt(dtype), lens_q[-1] + 69, lens_k[-1] + 20
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(Mq, 4, 64, generator=g).to(dt).to(DEV)
+    k, v = [torch.randn(Mk, 2, 64, generator=g).to(dt).to(DEV) for _ in range(2)]
+    cu_q, cu_k = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lens_q, lens_k)]
+    mine = torch.zeros(Mq, dtype=torch.bool, device=DEV)
+    mine[lens_q[0]:lens_q[-1]] = True
+    for low in (False, True):
+        want = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, want_low=low)
+        out = torch.full_like(q, 5.0)
+        _poisoned((want[1].shape, torch.float32), (q.shape, dt))
+        got = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, out=out, want_low=low)
+        assert got[0] is out and (out[~mine] == 5).all() and torch.equal(out[mine], want[0][mine])
+        assert (got[1][:, ~mine] == -float("inf")).all() and torch.equal(got[1], want[1])
+        if low and dt != torch.float32:
+            assert (got[2][~mine] == 0).all() and torch.equal(got[2], want[2])
