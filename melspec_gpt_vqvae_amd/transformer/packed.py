@@ -1,6 +1,7 @@
 """Differentiable operators for packed sequences of different lengths, over the kernels of ops.py: what a transformer with
 rotary positions, normed queries and keys and shared key heads needs between its projections.  The serving forms
-(ops.kv_append, ops.paged_attn_decode) stand in ops.py; they have no gradient.
+(ops.kv_append, ops.paged_attn_decode) stand in ops.py; they have no gradient.  Gradients are reverse mode, once: second
+derivatives and forward mode raise.
 
 A captured backward pass (HIP graph): call ops.*_fwd / ops.*_bwd directly, or capture forward and backward together with
 torch.autograd.grad on leaves that no live eager graph holds - autograd's leaf nodes remember the stream they were made on."""
@@ -9,6 +10,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import ops
@@ -36,8 +38,14 @@ def rotary_freqs(rot, base=10000.0, *, stretch=1.0, base_stretch=1.0, ramp=None,
     return f.to(device)
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _through_autograd(*tensors):
+    """whether a call goes through its autograd function: for a gradient; with a tangent of forward-mode differentiation,
+    which the function refuses and the bare kernel would drop; and in a trace, which holds the function and not the kernel"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return True
+    return torch._C._get_tracing_state() is not None
 
 
 class _QkNormRotaryFn(torch.autograd.Function):
@@ -60,7 +68,7 @@ class _QkNormRotaryFn(torch.autograd.Function):
 
 def qk_norm_rotary(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
     """ops.qk_norm_rotary_fwd with gradients for q, k and both weights."""
-    if not _wants_grad(q, k, q_weight, k_weight):
+    if not _through_autograd(q, k, q_weight, k_weight):
         return ops.qk_norm_rotary_fwd(q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
                                       amplitude=amplitude)
     return _QkNormRotaryFn.apply(q, k, q_weight, k_weight, positions, freqs, float(eps), bool(interleaved), float(amplitude))
@@ -83,6 +91,6 @@ class _PackedAttentionFn(torch.autograd.Function):
 
 def packed_attention(q, k, v, cu_q, cu_k=None, *, scale=None):
     """ops.packed_attn_fwd's output with gradients for q, k and v (those of a key head summed over its query heads)."""
-    if not _wants_grad(q, k, v):
+    if not _through_autograd(q, k, v):
         return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale)[0]
     return _PackedAttentionFn.apply(q, k, v, cu_q, cu_k, scale)

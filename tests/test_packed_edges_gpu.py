@@ -99,3 +99,27 @@ def test_log_sums_of_rows_that_no_sequence_owns(lens_q, lens_k, dtype):
         assert (got[1][:, ~mine] == -float("inf")).all() and torch.equal(got[1], want[1])
         if low and dt != torch.float32:
             assert (got[2][~mine] == 0).all() and torch.equal(got[2], want[2])
+
+
+# ------------------------------------------------------------------------------------------ forward mode, traces
+def test_forward_mode_is_refused_and_a_trace_replays():
+    import torch.autograd.forward_ad as forward_ad
+    from melspec_gpt_vqvae_amd.transformer import packed as pk
+
+    dt = _dt("half")
+    g = torch.Generator().manual_seed(5)
+    q, q2 = [torch.randn(30, 4, 64, generator=g).to(dt).to(DEV) for _ in range(2)]
+    k, k2 = [torch.randn(30, 2, 64, generator=g).to(dt).to(DEV) for _ in range(2)]
+    cu, pos = torch.tensor([0, 30], dtype=torch.int32, device=DEV), torch.arange(30, dtype=torch.int32, device=DEV)
+    f = pk.rotary_freqs(64, device=DEV)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError):
+            pk.packed_attention(d, k, k, cu)
+        with pytest.raises(NotImplementedError):
+            pk.qk_norm_rotary(d, k, pos, f)
+    layer = lambda a, b: pk.packed_attention(*pk.qk_norm_rotary(a, b, pos, f), b, cu)
+    traced = torch.jit.trace(layer, (q, k), check_trace=False)
+    # (a trace goes through the autograd functions, as a call with gradients does)
+    a, b = q2.clone().requires_grad_(True), k2
+    assert torch.equal(traced(q2, k2), layer(a, b).detach())
