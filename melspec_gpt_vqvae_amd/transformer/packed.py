@@ -38,14 +38,17 @@ def rotary_freqs(rot, base=10000.0, *, stretch=1.0, base_stretch=1.0, ramp=None,
     return f.to(device)
 
 
-def _through_autograd(*tensors):
-    """whether a call goes through its autograd function: for a gradient; with a tangent of forward-mode differentiation,
-    which the function refuses and the bare kernel would drop; and in a trace, which holds the function and not the kernel"""
+def _differentiated(*tensors):
+    """whether one of them wants a gradient or carries a tangent of forward-mode differentiation"""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return True
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        return True
-    return torch._C._get_tracing_state() is not None
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _through_autograd(*tensors):
+    """whether a call goes through its autograd function: for a gradient; with a tangent, which the function refuses and the
+    bare kernel would drop; and in a trace, which holds the function and not the kernel"""
+    return _differentiated(*tensors) or torch._C._get_tracing_state() is not None
 
 
 class _QkNormRotaryFn(torch.autograd.Function):
@@ -67,7 +70,8 @@ class _QkNormRotaryFn(torch.autograd.Function):
 
 
 def qk_norm_rotary(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
-    """ops.qk_norm_rotary_fwd with gradients for q, k and both weights."""
+    """ops.qk_norm_rotary_fwd with gradients for q, k and both weights (not for freqs)."""
+    assert not _differentiated(freqs), "the frequencies have no gradient: give them detached"
     if not _through_autograd(q, k, q_weight, k_weight):
         return ops.qk_norm_rotary_fwd(q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
                                       amplitude=amplitude)

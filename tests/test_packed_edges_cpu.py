@@ -62,3 +62,20 @@ def test_a_trace_holds_the_operator(requires_grad, monkeypatch):
     assert torch.equal(attention(q2, k2, v2), 2 * q2 + v2.numpy().mean())
     a, b = rotary(q2, k2)
     assert torch.equal(a, 2 * q2) and torch.equal(b, 3 * k2)
+
+
+def test_frequencies_that_want_a_gradient_are_refused(monkeypatch):
+    """the rotation has no gradient for its frequencies: they are refused rather than left without one"""
+    from melspec_gpt_vqvae_amd.transformer import packed as pk
+
+    _opaque(monkeypatch)
+    q, k = [torch.randn(5, 2, 64) for _ in range(2)]
+    pos, f = torch.arange(5, dtype=torch.int32), pk.rotary_freqs(64, device="cpu").requires_grad_(True)
+    for a in (q, q.clone().requires_grad_(True)):
+        with pytest.raises(AssertionError):
+            pk.qk_norm_rotary(a, k, pos, f)
+        with torch.no_grad():
+            pk.qk_norm_rotary(a, k, pos, f)
+    pk.qk_norm_rotary(q, k, pos, f.detach())
+    with forward_ad.dual_level(), pytest.raises(AssertionError):
+        pk.qk_norm_rotary(q, k, pos, forward_ad.make_dual(f.detach(), torch.ones(32, dtype=torch.float64)))
