@@ -1012,6 +1012,50 @@ def _into(x, like, *inputs):
     assert p == 0 or all(p != y.data_ptr() for y in inputs), "a result is a buffer of its own"
 
 
+def _span(x):
+    """first byte of a tensor and the one behind its last"""
+    at = x.data_ptr()
+    if x.is_contiguous():
+        return at, at + x.nbytes
+    return at, at + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+
+
+def _runs(x):
+    """-> (first bytes in rising order, length) of the runs of neighbouring values that a tensor consists of"""
+    length, starts = x.element_size(), None
+    dims = [(n, s * x.element_size()) for n, s in zip(x.shape, x.stride()) if n > 1 and s > 0]
+    while dims and dims[-1][1] == length:
+        length *= dims.pop()[0]
+    starts = torch.tensor([x.data_ptr()])
+    for n, s in dims:
+        starts = (starts[:, None] + s * torch.arange(n)).flatten()
+    return starts.sort().values, length
+
+
+def _overlap(x, y):
+    """whether two tensors share memory, exactly (their spans do)"""
+    if x.dim() == y.dim() == 3 and x.stride(0) * x.element_size() == y.stride(0) * y.element_size() > 0:
+        # side by side in rows of one length (a fused buffer): both within a row, one in front of the other
+        row = x.stride(0) * x.element_size()
+        (x0, x1), (y0, y1) = _span(x[0]), _span(y[0])
+        d = (y0 - x0) % row
+        if x1 - x0 <= d and d + y1 - y0 <= row:
+            return False
+    (xs, nx), (ys, ny) = _runs(x), _runs(y)
+    at = torch.searchsorted(xs, ys, right=True)                    # x's first run behind the start of each of y's
+    return bool(((at > 0) & (xs[(at - 1).clamp(min=0)] + nx > ys)).any() or
+                ((at < len(xs)) & (xs[at.clamp(max=len(xs) - 1)] < ys + ny)).any())
+
+
+def _apart(x, *others):
+    """x, a caller's buffer for a result, must not share memory with any of the others: kernels write it while they read those"""
+    lo, hi = _span(x)
+    for y in others:
+        if y is not None and y.data_ptr() < hi:                    # (an empty tensor's address is 0, as is its end)
+            a, b = _span(y)
+            assert b <= lo or not _overlap(x, y), "a result shares memory with an input or another result"
+
+
 def _addr(x):
     return None if x is None else x.data_ptr()
 
@@ -1124,7 +1168,7 @@ def kv_append(k, v, k_pages, v_pages, page_table, sequences, positions, *, q=Non
     dt = dtype_code(k.dtype)
     P, Hkp, page, Dp = _pages_of(i, k_pages, v_pages, page_table, k.dtype)
     assert (Hkp, Dp) == (Hk, D), (k_pages.shape, k.shape)
-    assert k_pages.data_ptr() != v_pages.data_ptr() or k_pages.numel() == 0, "keys and values want pages of their own"
+    assert abs(k_pages.data_ptr() - v_pages.data_ptr()) >= k_pages.numel() * k_pages.element_size(), "keys and values want pages of their own"
     assert sequences.dtype == torch.int32 and sequences.shape == (M,) and sequences.is_contiguous(), "sequences: (rows,) int32"
     vec = 4 if dt == _ffi.F32 else 8
     _same_device(i, v, q, q_out, sequences)
@@ -1141,7 +1185,7 @@ def kv_append(k, v, k_pages, v_pages, page_table, sequences, positions, *, q=Non
             q_out = torch.empty((M, Hq, D), dtype=k.dtype, device=k.device)
         else:
             assert q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous()
-            assert q_out.data_ptr() != q.data_ptr(), "q_out is a buffer of its own"
+            _apart(q_out, q, k, v, k_pages, v_pages, page_table, sequences, positions, freqs, q_weight, k_weight)
         q, qr, qh = _heads(q, vec)
     if M == 0:
         return q_out
@@ -1195,6 +1239,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     else:
         _into(out, q, q, k, v)
         _same_device(i, out)
+        _apart(out, q, k, v, cu_q, cu_k)
     lse = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
     low = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device) if want_low and dt != _ffi.F32 else None
     splits, ws = 1, None
@@ -1239,6 +1284,8 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
         _into(dk, k, q, k, v, out, dout, dv)
         _into(dv, v, q, k, v, out, dout)
         _same_device(i, dq, dk, dv)
+        for j, x in enumerate(grads):
+            _apart(x, q, k, v, out, dout, lse, low, cu_q, cu_k, *grads[:j])
     delta = torch.empty((Hq, Mq), dtype=torch.float32, device=q.device)
     splits, ws = _ffi.lib().melgpt_packed_attn_bwd_splits(Mk, S, Hq, Hk, dt), None
     if splits > 1:
@@ -1271,6 +1318,7 @@ def paged_attn_decode(q, k_pages, v_pages, page_table, lengths, *, scale=None, m
         out = torch.empty((S, Hq, D), dtype=q.dtype, device=q.device)
     else:
         _into(out, q, q)
+        _apart(out, q, k_pages, v_pages, page_table, lengths)
     lse = torch.empty((S, Hq), dtype=torch.float32, device=q.device)
     if S == 0:
         return out, lse

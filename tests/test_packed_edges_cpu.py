@@ -79,3 +79,59 @@ def test_frequencies_that_want_a_gradient_are_refused(monkeypatch):
     pk.qk_norm_rotary(q, k, pos, f.detach())
     with forward_ad.dual_level(), pytest.raises(AssertionError):
         pk.qk_norm_rotary(q, k, pos, forward_ad.make_dual(f.detach(), torch.ones(32, dtype=torch.float64)))
+
+
+# ------------------------------------------------------------------------------------------------------ results apart
+def _elements(x):
+    """byte addresses of a tensor's elements, one by one"""
+    at = torch.zeros((), dtype=torch.int64)
+    for n, s in zip(x.shape, x.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return set((x.data_ptr() + x.element_size() * at.flatten()).tolist())
+
+
+def test_results_that_overlap_inputs_at_any_offset_are_refused():
+    from melspec_gpt_vqvae_amd.ops import _apart
+
+    room = torch.zeros(40000)
+    rows = lambda at, M, H, D=64: room[at:at + M * H * D].view(M, H, D)
+    fused = room[:6 * 12 * 64].view(6, 12, 64)                     # q | k | v of 4 heads each, row by row
+    heads = room[:12 * 6 * 64].view(12, 6, 64).transpose(0, 1)     # the same heads outermost
+    good = [(rows(0, 6, 4), rows(6 * 256, 6, 4)), (fused[:, :4], fused[:, 4:8]), (fused[:, 8:], fused[:, :4]), (fused[:, 4:8], fused[:, 8:]),
+            (heads[:, :4], heads[:, 4:]), (heads[:, 1::2], heads[:, ::2]), (fused[:, ::2], fused[:, 1::2]), (fused[:3], fused[3:]),
+            (rows(0, 0, 4), rows(0, 6, 4)), (fused[:1, :4], fused[1:, :4]), (fused[..., :32], fused[..., 32:]), (rows(0, 6, 4), None)]
+    for x, y in good:
+        _apart(x, y)
+        if y is not None:
+            _apart(y, x)
+    bad = [(rows(0, 6, 4), rows(64, 6, 4)), (rows(64, 6, 4), rows(0, 6, 4)), (fused[:, :4], fused[:, 3:7]), (fused[:, 4:8], fused),
+           (heads[:, :4], heads[:, 3:]), (fused[:, :4], heads[:, :4]), (fused[..., :32], fused[..., 24:56]), (rows(0, 6, 4), rows(5 * 256 + 192, 1, 1)),
+           (fused[:, :4], rows(12 * 64 * 5 + 64, 2, 2)), (fused[1:3, :4], fused[2:4, 2:6]), (rows(0, 6, 4), room[100:108].view(torch.int32))]
+    for x, y in bad:
+        for a, b in ((x, y), (y, x)):
+            with pytest.raises(AssertionError):
+                _apart(a, None, rows(30000, 2, 2), b)
+
+
+def test_results_apart_against_every_element():
+    import random
+
+    from melspec_gpt_vqvae_amd.ops import _apart
+
+    room, rng, seen = torch.zeros(6000), random.Random(1), [0, 0]
+    for _ in range(3000):
+        pair = []
+        for _ in range(2):
+            M, H, D = rng.randint(1, 5), rng.randint(1, 4), 4 * rng.randint(1, 3)
+            h = 4 * rng.choice([0, D // 4, D // 4 + rng.randint(0, 3), rng.randint(1, 40)])
+            r = 4 * rng.choice([0, H * h // 4 + D // 4, 24, rng.randint(1, 60)])
+            pair.append(room.as_strided((M, H, D), (r, h, 1), 4 * rng.randint(0, 120)))
+        x, y = pair
+        apart = _elements(x).isdisjoint(_elements(y))
+        seen[apart] += 1
+        if apart:
+            _apart(x, y)
+        else:
+            with pytest.raises(AssertionError):
+                _apart(x, y)
+    assert min(seen) > 500

@@ -123,3 +123,52 @@ def test_forward_mode_is_refused_and_a_trace_replays():
     # (a trace goes through the autograd functions, as a call with gradients does)
     a, b = q2.clone().requires_grad_(True), k2
     assert torch.equal(traced(q2, k2), layer(a, b).detach())
+
+
+# --------------------------------------------------------------------------------------------------- results apart
+def test_results_that_share_memory_with_inputs_are_refused():
+    from melspec_gpt_vqvae_amd import ops
+
+    dt, M = _dt("half"), 40
+    room = torch.zeros(1 << 20, dtype=dt, device=DEV)
+    rows = lambda at, H: room[at:at + M * H * 64].view(M, H, 64)
+    q, k, v, do = rows(0, 4), rows(20000, 2), rows(30000, 2), rows(40000, 4)
+    cu = torch.tensor([0, M], dtype=torch.int32, device=DEV)
+    fused = torch.zeros(M, 8, 64, dtype=dt, device=DEV)            # (side by side in rows: apart)
+    out, lse = ops.packed_attn_fwd(fused[:, :4], fused[:, 4:6], fused[:, 6:], cu, out=rows(0, 4))
+    for at in (64, 20000 - 64, 30000 + 128):
+        with pytest.raises(AssertionError):
+            ops.packed_attn_fwd(q, k, v, cu, out=rows(at, 4))
+    out, lse = ops.packed_attn_fwd(q, k, v, cu)
+    free = 100000
+    ops.packed_attn_bwd(q, k, v, out, do, lse, cu, grads=(rows(free, 4), rows(free + 20000, 2), rows(free + 30000, 2)))
+    for at in ((64, free, free + 10000), (free, 30000 - 64, free + 20000), (free, free + 20000, 40000 + 64), (free, free + 64, free + 20000),
+               (free, free + 20000, free + 20000 + 64)):
+        with pytest.raises(AssertionError):
+            ops.packed_attn_bwd(q, k, v, out, do, lse, cu, grads=(rows(at[0], 4), rows(at[1], 2), rows(at[2], 2)))
+    # the cache: pages as parts of one buffer
+    page = lambda at: room[at:at + 8 * 2 * 16 * 64].view(8, 2, 16, 64)
+    kp, vp = page(200000), page(300000)
+    seq, pos = torch.zeros(M, dtype=torch.int32, device=DEV), torch.arange(M, dtype=torch.int32, device=DEV)
+    table = torch.arange(8, dtype=torch.int32, device=DEV)[None]
+    ops.kv_append(k, v, kp, vp, table, seq, pos, q=q, q_out=rows(free, 4))
+    for at in (64, 20000 - 64, 30000 + 64, 200000 + 64, 300000 - 64):
+        with pytest.raises(AssertionError):
+            ops.kv_append(k, v, kp, vp, table, seq, pos, q=q, q_out=rows(at, 4))
+    with pytest.raises(AssertionError):
+        ops.kv_append(k, v, kp, page(200000 + 1024), table, seq, pos, q=q)
+    lengths = torch.tensor([M], dtype=torch.int32, device=DEV)
+    ops.paged_attn_decode(q[:1], kp, vp, table, lengths, out=rows(free, 4)[:1])
+    for at in (64, 200000 + 64, 300000 + 16 * 64 * 4):
+        with pytest.raises(AssertionError):
+            ops.paged_attn_decode(q[:1], kp, vp, table, lengths, out=rows(at, 4)[:1])
+
+
+def test_append_of_no_rows_with_a_given_buffer():
+    from melspec_gpt_vqvae_amd import ops
+
+    q = torch.zeros(0, 2, 64, device=DEV)
+    pages = [torch.zeros(1, 2, 16, 64, device=DEV) for _ in range(2)]
+    none, table = torch.zeros(0, dtype=torch.int32, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    room = torch.empty(0, 2, 64, device=DEV)
+    assert ops.kv_append(q, q, *pages, table, none, none, q=q, q_out=room) is room
