@@ -588,7 +588,8 @@ int melgpt_kv_append(const void* q, long long q_row, long long q_head, const voi
  * kernel; melgpt_packed_attn_splits proposes it from the sizes.  With splits > 1 `workspace` holds splits * Hq * Mq * (D + 2)
  * f32, 16-byte aligned.  The backward's splits (melgpt_packed_attn_bwd_splits) share a key tile's query heads in the same
  * way, with 2 * splits * Mk * Hk * D f32.
- * D 64 or 128; scale multiplies the scores; at most 4 M rows (65535 tiles of 64 with one more per sequence). */
+ * D 64 or 128; rows of q, k, v and dout at most 2^24 values apart (64 of them within 4 GB); scale multiplies the scores; at
+ * most 4 M rows (65535 tiles of 64 with one more per sequence). */
 int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int Hq, int D, int dtype);
 int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                            const void* v, long long v_row, long long v_head, const int* cu_q, const int* cu_k, int S, void* out,

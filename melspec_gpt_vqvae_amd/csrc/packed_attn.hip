@@ -1231,16 +1231,21 @@ int check(const PackedParams& p, int D, int dtype) {
   const int vec = dtype == MELGPT_F32 ? 4 : 8;
   if (p.Mq > 0 && (!p.q || !p.o || !p.lse)) return MELGPT_ERR_BAD_ARG;
   if (p.Mk > 0 && (!p.k || !p.v)) return MELGPT_ERR_BAD_ARG;
-  // rows do not overlap, and 64 of them lie within 4 GB of each other (the kernels' buffer loads)
-  if ((p.Mk > 1 && (p.k_row < D || p.v_row < D)) || (p.Mq > 1 && p.q_row < D) || p.k_row > (1 << 24) || p.v_row > (1 << 24) ||
-      p.q_row > (1 << 24))
-    return MELGPT_ERR_UNSUPPORTED;
+  // rows do not overlap, and 64 of them lie within 4 GB of each other (the kernels' buffer loads); one row has no stride
+  if (p.Mk > 1 && (p.k_row < D || p.v_row < D || p.k_row > (1 << 24) || p.v_row > (1 << 24))) return MELGPT_ERR_UNSUPPORTED;
+  if (p.Mq > 1 && (p.q_row < D || p.q_row > (1 << 24))) return MELGPT_ERR_UNSUPPORTED;
   if (p.low && dtype == MELGPT_F32) return MELGPT_ERR_UNSUPPORTED;
   if (!aligned16(p.low) || !aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.o)) return MELGPT_ERR_ALIGN;
   if (p.q_row % vec || p.q_head % vec || p.k_row % vec || p.k_head % vec || p.v_row % vec || p.v_head % vec || p.o_row % vec ||
       p.o_head % vec)
     return MELGPT_ERR_ALIGN;
   return MELGPT_OK;
+}
+
+// a single row's stride is never used, but the rows behind it must lie outside its buffer
+void single_rows(PackedParams& p, int D) {
+  if (p.Mq <= 1) p.q_row = p.do_row = D;
+  if (p.Mk <= 1) p.k_row = p.v_row = D;
 }
 
 template <typename T, int D>
@@ -1321,6 +1326,7 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
   if (!aligned16(workspace)) return MELGPT_ERR_ALIGN;
   if (Mq == 0) return MELGPT_OK;
   p.G = Hq / Hk;
+  single_rows(p, D);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == MELGPT_F32) return D == 64 ? launch_fwd<float, 64>(p, s) : launch_fwd<float, 128>(p, s);
   return D == 64 ? launch_fwd<bf16_t, 64>(p, s) : launch_fwd<bf16_t, 128>(p, s);
@@ -1359,12 +1365,13 @@ extern "C" int melgpt_packed_attn_bwd(const void* q, long long q_row, long long 
   if (splits > 1 && (dtype == MELGPT_F32 || splits > 1024 || Hk * Mk > (1LL << 25))) return MELGPT_ERR_UNSUPPORTED;
   if (!aligned16(workspace)) return MELGPT_ERR_ALIGN;
   p.splits = splits; p.part = workspace;
-  if ((Mq > 1 && do_row < D) || do_row > (1 << 24)) return MELGPT_ERR_UNSUPPORTED;
+  if (Mq > 1 && (do_row < D || do_row > (1 << 24))) return MELGPT_ERR_UNSUPPORTED;
   const int vec = dtype == MELGPT_F32 ? 4 : 8;
   if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || do_row % vec || do_head % vec || dq_row % vec ||
       dq_head % vec || dk_row % vec || dk_head % vec || dv_row % vec || dv_head % vec)
     return MELGPT_ERR_ALIGN;
   p.G = Hq / Hk;
+  single_rows(p, D);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == MELGPT_F32) return D == 64 ? launch_bwd<float, 64>(p, s) : launch_bwd<float, 128>(p, s);
   return D == 64 ? launch_bwd<bf16_t, 64>(p, s) : launch_bwd<bf16_t, 128>(p, s);

@@ -990,11 +990,11 @@ def _same_device(i, *tensors):
         assert t_ is None or t_.get_device() == i, f"a tensor is on {t_.device}, expected cuda:{i}"
 
 
-def _heads(x, vec):
+def _heads(x, vec, farthest=1 << 62):
     """(rows, heads, D) tensor -> the same, or a copy where its rows or heads are not 16-byte aligned, its values not side by
-    side or its rows overlap; -> (tensor, row stride, head stride)"""
+    side, its rows overlap or lie more than `farthest` values apart; -> (tensor, row stride, head stride)"""
     r, h, u = x.stride()
-    if u != 1 or r % vec or h % vec or (r < x.shape[2] and x.shape[0] > 1) or x.data_ptr() & 15:
+    if u != 1 or r % vec or h % vec or ((r < x.shape[2] or r > farthest) and x.shape[0] > 1) or x.data_ptr() & 15:
         x = x.clone(memory_format=torch.contiguous_format)
         r, h, u = x.stride()
     return x, r, h
@@ -1216,6 +1216,9 @@ def _packed_args(i, q, k, v, cu_q, cu_k):
     return Mq, Mk, Hq, Hk, D, S, cu_k
 
 
+_FARTHEST = 1 << 24   # values between two rows of packed attention's inputs: 64 rows lie within 4 GB (melgpt_packed_attn_fwd)
+
+
 def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=False):
     """Causal attention of packed sequences: q (Mq, Hq, D), k, v (Mk, Hk, D), any row and head strides, Hq a multiple of Hk;
     sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
@@ -1230,9 +1233,9 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     dt = dtype_code(q.dtype)
     Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(i, q, k, v, cu_q, cu_k)
     vec = 4 if dt == _ffi.F32 else 8
-    q, qr, qh = _heads(q, vec)
-    k, kr, kh = _heads(k, vec)
-    v, vr, vh = _heads(v, vec)
+    q, qr, qh = _heads(q, vec, _FARTHEST)
+    k, kr, kh = _heads(k, vec, _FARTHEST)
+    v, vr, vh = _heads(v, vec, _FARTHEST)
     gaps = 1 if out is None else 2
     if out is None:
         out = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)
@@ -1268,11 +1271,11 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
     assert low is None or (low.shape == q.shape and low.dtype == q.dtype and low.is_contiguous())
     _same_device(i, out, dout, lse, low)
     vec = 4 if dt == _ffi.F32 else 8
-    q, qr, qh = _heads(q, vec)
-    k, kr, kh = _heads(k, vec)
-    v, vr, vh = _heads(v, vec)
+    q, qr, qh = _heads(q, vec, _FARTHEST)
+    k, kr, kh = _heads(k, vec, _FARTHEST)
+    v, vr, vh = _heads(v, vec, _FARTHEST)
     out, our, ouh = _heads(out, vec)
-    dout, dor, doh = _heads(dout, vec)
+    dout, dor, doh = _heads(dout, vec, _FARTHEST)
     gaps = grads is None
     if gaps:
         dq = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device)

@@ -172,3 +172,41 @@ def test_append_of_no_rows_with_a_given_buffer():
     none, table = torch.zeros(0, dtype=torch.int32, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
     room = torch.empty(0, 2, 64, device=DEV)
     assert ops.kv_append(q, q, *pages, table, none, none, q=q, q_out=room) is room
+
+
+# ------------------------------------------------------------------------------------------------- rows far apart
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("M", [1, 3])
+def test_rows_more_than_2_24_values_apart(M, dtype):
+    """views of one position of a (rows, positions, heads, D) buffer: the same bits as from tensors side by side"""
+    from melspec_gpt_vqvae_amd import ops
+    from melspec_gpt_vqvae_amd.transformer import packed as pk
+
+    dt, D, far = _dt(dtype), 64, (1 << 24) + 64
+    room = torch.zeros((M - 1) * far + 4096, dtype=dt, device=DEV)
+    view = lambda H, at: room.as_strided((M, H, D), (far if M > 1 else 1 << 27, D, 1), at)
+    g = torch.Generator().manual_seed(2)
+    near = [torch.randn(M, H, D, generator=g).to(dt).to(DEV) for H in (4, 2, 2, 4)]
+    q, k, v, do = [view(x.shape[1], 512 * i) for i, x in enumerate(near)]
+    for x, y in zip((q, k, v, do), near):
+        x.copy_(y)
+    cu = torch.tensor([0, M], dtype=torch.int32, device=DEV)
+    out, lse = ops.packed_attn_fwd(*near[:3], cu)
+    got, got_lse = ops.packed_attn_fwd(q, k, v, cu)
+    assert torch.equal(got, out) and torch.equal(got_lse, lse)
+    given = view(4, 512 * 4)
+    ops.packed_attn_fwd(q, k, v, cu, out=given)
+    assert torch.equal(given, out)
+    grads = ops.packed_attn_bwd(*near[:3], out, near[3], lse, cu)
+    places = tuple(view(H, 512 * i) for H, i in ((4, 5), (2, 6), (2, 7)))
+    for a, b, c in zip(ops.packed_attn_bwd(q, k, v, given, do, lse, cu), grads, ops.packed_attn_bwd(q, k, v, given, do, lse, cu, grads=places)):
+        assert torch.equal(a, b) and torch.equal(c, b)
+    # one far tensor among near ones, each in turn, through the differentiable form
+    for i, x in enumerate((q, k, v)):
+        leaves = [(x if j == i else y).detach().requires_grad_(True) for j, y in enumerate(near[:3])]
+        o = pk.packed_attention(*leaves, cu)
+        plain = [y.detach().requires_grad_(True) for y in near[:3]]
+        o2 = pk.packed_attention(*plain, cu)
+        assert torch.equal(o, o2)
+        for a, b in zip(torch.autograd.grad(o, leaves, do), torch.autograd.grad(o2, plain, near[3])):
+            assert torch.equal(a, b)
