@@ -237,6 +237,22 @@ struct Stage {
   }
 };
 
+// a tile of B rows that no sequence owns: the forward's zeros (256 threads)
+template <typename T, int D, int B>
+__device__ __forceinline__ void rows_of_nobody(const PackedParams& p, const Rows& R, int h, int t) {
+  if (!p.write_gaps || blockIdx.z) return;
+  constexpr int VEC = 16 / sizeof(T), C = D / VEC;                 // 16-byte pieces of a row
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  const int first = B * R.tile, n = min(R.n - first, B);
+  for (int i = t; i < n * C; i += 256) {
+    const long long row = R.lo + first + i / C;
+    const int c = i % C;
+    if (p.write_gaps == 1) *(u32x4*)((T*)p.o + row * p.o_row + h * p.o_head + c * VEC) = zero;
+    if (p.low) *(u32x4*)((T*)p.low + (row * p.Hq + h) * D + c * VEC) = zero;
+    if (c == 0) p.lse[h * p.Mq + row] = -__builtin_inff();
+  }
+}
+
 // --------------------------------------------------------------------------------------------- forward, f32 lane
 // 256 threads, 64 queries of one head: a wave owns 16 queries and walks the keys 32 at a time (16 heads of 64 at length 266:
 // 18 us, the time of 80 workgroups' chains of 9 steps; at 4000 rows 75 - 80 TFLOP/s, of 154 in a large product).  S^T = K Q^T puts the query
@@ -253,9 +269,9 @@ __global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
   head_of(blockIdx.x, p, h);
   const Rows R = find_rows<64, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
+  if (R.seq < 0 || R.seq >= p.S) return rows_of_nobody<T, D, 64>(p, R, h, t);
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
-  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
   const int q_in = 64 * R.tile + 16 * wave + (lane & 15);          // this lane's query within its sequence
   const bool mine = q_in < R.n;
   const long long row = R.lo + min(q_in, R.n - 1);
@@ -332,10 +348,8 @@ __global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
   if (!mine) return;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;        // (NaN stays NaN)
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
-  if (p.write_gaps < 2 || (R.seq >= 0 && R.seq < p.S)) {
 #pragma unroll
-    for (int d = 0; d < L::DT; ++d) store4<T>(op + 16 * d + 4 * g, o[d] * inv);
-  }
+  for (int d = 0; d < L::DT; ++d) store4<T>(op + 16 * d + 4 * g, o[d] * inv);
   if (g == 0) p.lse[h * p.Mq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
@@ -459,9 +473,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   head_of(blockIdx.x, p, h);
   const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
+  if (R.seq < 0 || R.seq >= p.S) return rows_of_nobody<T, D, 128>(p, R, h, t);
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
-  if ((R.seq < 0 || R.seq >= p.S) && !p.write_gaps) return;
   const int w0 = 128 * R.tile + 32 * wave;                     // the wave's first query
   const int last = min(128 * R.tile + 127, R.n - 1);
   const int most = min(max(last + nk - R.n + 1, 0), nk);
@@ -631,25 +645,24 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)p.o + row * p.o_row + h * p.o_head;
-  if (p.write_gaps < 2 || (R.seq >= 0 && R.seq < p.S)) {
-#pragma unroll
-    for (int d = 0; d < L::DB; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        store4<T>(op + 32 * d + 8 * j + 4 * hh, f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv);
-  }
-  if (p.low) {   // the backward's delta = do . o loses a rounding of o against ds' own size; with both halves it does not
+  // low: the backward's delta = do . o loses a rounding of o against ds' own size; with both halves it does not.  It is taken
+  // from the bits that are stored: rounded a second time by itself, hipcc fuses the product into the conversion of the half
+  // flavour (one rounding instead of two), and at a tie the two halves would not fit each other.
+  auto put = [&](auto low) __attribute__((always_inline)) {
     T* lp = (T*)p.low + (row * p.Hq + h) * D;
 #pragma unroll
     for (int d = 0; d < L::DB; ++d)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f32x4 x = f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] -= bf16_to_f32(f32_to_bf16(x[r]));
-        store4<T>(lp + 32 * d + 8 * j + 4 * hh, x);
+        const int at = 32 * d + 8 * j + 4 * hh;
+        const f32x4 x = f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv;
+        const u32x2 w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+        *(u32x2*)(op + at) = w;
+        if (decltype(low)::value) store4<T>(lp + at, x - f32x4{half_lo(w[0]), half_hi(w[0]), half_lo(w[1]), half_hi(w[1])});
       }
-  }
+  };
+  if (p.low) put(std::true_type());
+  else put(std::false_type());
   if (hh == 0) p.lse[h * p.Mq + row] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
@@ -663,7 +676,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
   const int d = 4 * (threadIdx.x % TPQ), h = (int)(n / p.Mq);
   const long long row = n % p.Mq;
   const bool gap = row < bound_at(p.cu_q, p.S, p.Mq, 1) || row >= bound_at(p.cu_q, p.S, p.Mq, p.S + 1);
-  if (gap && !p.write_gaps) return;
+  if (gap) return;                                                 // (written by the forward itself)
   const float* st = p.part + (long long)p.splits * all * D + 2 * n;
   float top = -__builtin_inff();
   for (int i = 0; i < p.splits; ++i) top = fmaxf(top, st[2 * i * all]);
@@ -677,7 +690,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
     sum += st[2 * i * all + 1] * f;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (!gap || p.write_gaps < 2) store4<T>((T*)p.o + row * p.o_row + h * p.o_head + d, a * inv);
+  store4<T>((T*)p.o + row * p.o_row + h * p.o_head + d, a * inv);
   if (d == 0) p.lse[n] = sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 

@@ -210,3 +210,26 @@ def test_rows_more_than_2_24_values_apart(M, dtype):
         assert torch.equal(o, o2)
         for a, b in zip(torch.autograd.grad(o, leaves, do), torch.autograd.grad(o2, plain, near[3])):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------- the output's two halves fit
+@pytest.mark.parametrize("D", [64, 128])
+def test_output_and_its_remainder_fit_each_other(D):
+    """enough values (10 sequences of 64, 8 heads) that dozens of them lie on a tie of the 16-bit format"""
+    import packed_ref as R
+    from melspec_gpt_vqvae_amd import ops
+
+    dt, n, H = _dt("half"), 64, 8
+    g = torch.Generator().manual_seed(9)
+    q, k, v = [torch.randn(10 * n, H, D, generator=g).to(dt) for _ in range(3)]
+    cu = torch.arange(0, 10 * n + 1, n, dtype=torch.int32, device=DEV)
+    out, _, low = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), cu, want_low=True)
+    both, h = out.double().cpu() + low.double().cpu(), R.half_step(dt)
+    for s in range(10):
+        a = slice(n * s, n * s + n)
+        for i in range(H):
+            r = R.attention(q[a, i], k[a, i], v[a, i], D ** -0.5)
+            # probabilities and output each in two halves: what the first left out is rounded once more
+            rel = R.attention_relative(D, r["s_score"], n, torch.float32)[:, None] + h * h
+            bound = (h * h + 4 * R.U) * r["o"].abs() + rel * r["s_o"] + R.smallest(dt) * (2 + r["a_o"])
+            R.assert_within(both[a, i], r["o"], bound, f"sequence {s} head {i}")
