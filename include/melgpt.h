@@ -608,7 +608,8 @@ int melgpt_packed_attn_bwd_splits(long long Mk, int S, int Hq, int Hk, int dtype
  * strides, keys 0 .. lengths[s] - 1 of sequence s through page_table[s * table_ld + j / page_size] (columns beyond `width`
  * do not exist, a page outside n_pages leaves its keys out; the kernel checks every index), lse (S, Hq) f32.  A sequence
  * without keys gives 0 (lse -inf).  `splits` workgroups share a (sequence, key head): melgpt_paged_attn_splits proposes it
- * from the longest length the caller knows of (any value gives the same result up to f32 rounding); with splits > 1
+ * from the longest length the caller knows of (any value gives the same result up to f32 rounding; splits beyond 2048 workgroups
+ * serve sequences longer than 4096 keys a usual share); with splits > 1
  * `workspace` holds S * Hq * splits * (D + 2) f32, 16-byte aligned.  D 64 or 128, page_size a power of two. */
 int melgpt_paged_attn_splits(int S, int Hq, int Hk, long long max_length);
 int melgpt_paged_attn_decode(const void* q, long long q_row, long long q_head, const void* k_pages, const void* v_pages,

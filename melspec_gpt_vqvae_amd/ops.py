@@ -1303,9 +1303,11 @@ def packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k=None, *, scale=None, gra
 def paged_attn_decode(q, k_pages, v_pages, page_table, lengths, *, scale=None, max_length=None, out=None):
     """Attention of one query token per sequence over a paged cache: q (S, Hq, D), any row and head strides; k_pages, v_pages
     (pages, Hk, page size, D), Hq a multiple of Hk; page_table (S, width) int32; lengths (S,) int32, the keys each sequence
-    has (those of kv_append's last row among them; what the table's width does not hold is not there) -> (out (S, Hq, D), lse (S, Hq) f32).  A sequence without keys gives 0; a
-    table entry outside the pages leaves its keys out.  max_length: the longest length, where the caller knows one shorter
-    than the table's width (it only decides how far a sequence is split).  scale: 1 / sqrt(D) unless given."""
+    has (those of kv_append's last row among them; what the table's width does not hold is not there) -> (out (S, Hq, D), lse
+    (S, Hq) f32).  A sequence without keys gives 0; a table entry outside the pages leaves its keys out.  max_length: the
+    longest length, where the caller knows one shorter than the table's width: it only decides how far sequences are split (a
+    wide table costs a large batch of short sequences some 10 us and the room for partial results).  scale: 1 / sqrt(D)
+    unless given."""
     i = _device_of(q)
     if i != _current_device():
         return _on(i, paged_attn_decode, q, k_pages, v_pages, page_table, lengths, scale=scale, max_length=max_length, out=out)

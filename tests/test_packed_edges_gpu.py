@@ -233,3 +233,91 @@ def test_output_and_its_remainder_fit_each_other(D):
             rel = R.attention_relative(D, r["s_score"], n, torch.float32)[:, None] + h * h
             bound = (h * h + 4 * R.U) * r["o"].abs() + rel * r["s_o"] + R.smallest(dt) * (2 + r["a_o"])
             R.assert_within(both[a, i], r["o"], bound, f"sequence {s} head {i}")
+
+
+# ------------------------------------------------------------------- a few long sequences in a large batch: decode
+def _cached(lens, Hq, Hk, D, page, dtype, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    kp, vp = [torch.randn(sum(need) + 1, Hk, page, D, generator=g, device=DEV).to(dtype) for _ in range(2)]
+    order = torch.randperm(sum(need), generator=g, device=DEV).to(torch.int32)
+    table, at = torch.full((len(lens), max(need)), -1, dtype=torch.int32, device=DEV), 0
+    for s, n in enumerate(need):
+        table[s, :n] = order[at:at + n]
+        at += n
+    return torch.randn(len(lens), Hq, D, generator=g, device=DEV).to(dtype), kp, vp, table, torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+def _decode_reference(q, kp, vp, table, lens, which):
+    """for the sequences of `which`: (output, log sum, sizes of the output's terms, of the scores) in 64 bits, elementwise products"""
+    Hq, Hk, D, page = q.shape[1], kp.shape[1], q.shape[2], kp.shape[2]
+    for s in which:
+        j = torch.arange(lens[s], device=DEV)
+        at = table[s].long()[j // page], j % page
+        k, v = [x[at[0], :, at[1]].double().repeat_interleave(Hq // Hk, 1) for x in (kp, vp)]      # (keys, Hq, D)
+        w = (k * q[s].double()).sum(-1) * D ** -0.5
+        size = (k * q[s].double()).abs().sum(-1).amax(0) * D ** -0.5 if lens[s] else torch.zeros(Hq, device=DEV).double()
+        lse = torch.logsumexp(w, 0) if lens[s] else torch.full((Hq,), -float("inf"), device=DEV).double()
+        p = torch.exp(w - lse)[..., None]
+        yield s, (p * v).sum(0), lse, (p * v.abs()).sum(0), size
+
+
+def _check_decode(lens, Hq, Hk, D, page, dtype, seed, which=None, max_length=None):
+    import packed_ref as R
+    from melspec_gpt_vqvae_amd import ops
+
+    args = _cached(lens, Hq, Hk, D, page, dtype, seed)
+    out, lse = ops.paged_attn_decode(*args, max_length=max_length)
+    h = R.half_step(dtype)
+    for s, o, l, size, score in _decode_reference(*args[:4], lens, range(len(lens)) if which is None else which):
+        n = lens[s]
+        rel = R.attention_relative(D, score, n + 300, dtype)[:, None]
+        R.assert_within(out[s], o, h * o.abs() + rel * size + R.smallest(dtype) * (1 + n * 5), f"out {s}")
+        R.assert_within(lse[s], l, (D + 4) * R.U * score + (n + 300) * R.U + 4 * R.U * l.abs().nan_to_num(posinf=0), f"lse {s}")
+    return args, out, lse
+
+
+@pytest.mark.parametrize("dtype", ["f32", "half"])
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 8, 64), (8, 8, 128)])
+def test_long_sequences_in_a_large_batch_of_short_ones(Hq, Hk, D, dtype):
+    from melspec_gpt_vqvae_amd import _ffi
+
+    lens = [7 * i % 90 for i in range(300)]
+    for s, n in ((0, 4097), (5, 9000), (64, 4096), (127, 12300), (299, 8193)):      # (first, last, at a wave's end, two in one wave)
+        lens[s] = n
+    assert _ffi.lib().melgpt_paged_attn_splits(300, Hq, Hk, 12304) == 4 and 300 * Hk >= 2048
+    _check_decode(lens, Hq, Hk, D, 16, _dt(dtype), 1)
+    _check_decode(lens, Hq, Hk, D, 16, _dt(dtype), 1, which=[0, 5, 127, 299], max_length=5000)      # (a wrong hint: two shares at most)
+
+
+def test_more_long_shares_than_workgroups_that_look_for_them():
+    lens = [4500 + i for i in range(130)]                          # 130 sequences of 16 heads, a second share each: 2080
+    _check_decode(lens, 16, 16, 64, 64, _dt("half"), 2, which=[0, 1, 63, 64, 65, 100, 128, 129])
+
+
+def test_long_sequences_with_two_groups_of_heads():
+    lens = [50] * 70
+    lens[3] = lens[69] = 5000
+    _check_decode(lens, 17 * 16, 16, 64, 32, _dt("half"), 3, which=[0, 3, 68, 69])
+
+
+def test_captured_decode_of_growing_lengths():
+    """one graph, lengths on either side of a share of 4096 keys from replay to replay"""
+    from melspec_gpt_vqvae_amd import ops
+
+    (q, kp, vp, table, lengths), _, _ = _check_decode([9000] * 3 + [100] * 300, 8, 8, 64, 64, _dt("half"), 4, which=[1, 200])
+    step = lambda: ops.paged_attn_decode(q, kp, vp, table, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for a, b, c in ((4096, 1, 0), (4097, 9000, 8192), (0, 0, 0), (8193, 64, 4160), (9000, 9000, 9000)):
+        lengths[:3] = torch.tensor([a, b, c], dtype=torch.int32, device=DEV)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        for s, o, l, size, score in _decode_reference(q, kp, vp, table, lengths.tolist(), range(3)):
+            # (half a bf16 step of values up to 5, the largest of these; the bits are held to the eager call's above)
+            assert float((got[0][s].double() - o).abs().max()) <= 0.02 and (lengths[s] > 0 or torch.isinf(got[1][s]).all())
