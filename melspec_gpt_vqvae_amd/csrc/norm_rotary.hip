@@ -144,16 +144,18 @@ __device__ __forceinline__ void cos_sin(int pos, const double* turns_per_pos, fl
 }
 
 // (products and sums are fused by hand here and below: left to hipcc, which of them it fuses differs between the kernels, and
-// a key would not have the same bits in a cache as outside.  Lanes whose values do not turn skip this: a turn by nothing would
-// multiply a neighbour by 0, and 0 * NaN is not 0)
+// a key would not have the same bits in a cache as outside.  Values that do not turn are left as they are: a turn by nothing
+// would multiply a neighbour by 0, and 0 * NaN is not 0.  By a choice of every result, except in the forward without a cache,
+// where the lanes that do not turn skip this: 14590 rows of 16 + 4 heads of 64 in bf16 take 22.5 us on the way into a cache,
+// 26.5 behind a branch, and 16385 of 32 + 8 of 128 without one 71 behind a branch, 73 by a choice.)
 template <typename T, bool INTERLEAVED>
-__device__ __forceinline__ void turn(float* x, const float* c, const float* s) {
+__device__ __forceinline__ void turn(float* x, const float* c, const float* s, bool turns) {
   using L = Lane<T, INTERLEAVED>;
 #pragma unroll
   for (int e = 0; e < L::N; ++e) {
     const float lo = x[L::lo(e)], hi = x[L::hi(e)];
-    x[L::lo(e)] = fmaf(lo, c[e], -(hi * s[e]));
-    x[L::hi(e)] = fmaf(hi, c[e], lo * s[e]);
+    x[L::lo(e)] = turns ? fmaf(lo, c[e], -(hi * s[e])) : lo;
+    x[L::hi(e)] = turns ? fmaf(hi, c[e], lo * s[e]) : hi;
   }
 }
 
@@ -267,7 +269,8 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(NormRotaryParams p
 #pragma unroll
             for (int e = 0; e < 2 * N; ++e) x[e] *= r * wt[e];
           }
-          if (at.turns) turn<T, INTERLEAVED>(x, c, s);
+          if constexpr (PAGED) turn<T, INTERLEAVED>(x, c, s, at.turns);
+          else if (at.turns) turn<T, INTERLEAVED>(x, c, s, true);
           if (!at.active || h >= p.t[i].H) return;
           T* o;
           if (PAGED && i == 1) {
