@@ -585,12 +585,14 @@ int melgpt_kv_append(const void* q, long long q_row, long long q_head, const voi
  * write_gaps: 1: rows of the outputs that no sequence owns are zeroed (lse -inf); 0: they are left as they were; 2 (forward):
  * zeroed in lse (-inf) and out_low, left in out.
  * splits: workgroups that share a row tile's keys (16-bit lane without out_low; 1: one), joined in a fixed order by a second
- * kernel; melgpt_packed_attn_splits proposes it from the sizes.  With splits > 1 `workspace` holds splits * Hq * Mq * (D + 2)
+ * kernel; melgpt_packed_attn_splits proposes it from the sizes, by the mean length; _splits_for also where the longest sequence
+ * may have up to `longest` keys (up to 16, more than the mean's: further shares for long sequences only).  With splits > 1 `workspace` holds splits * Hq * Mq * (D + 2)
  * f32, 16-byte aligned.  The backward's splits (melgpt_packed_attn_bwd_splits) share a key tile's query heads in the same
  * way, with 2 * splits * Mk * Hk * D f32.
  * D 64 or 128; rows of q, k, v and dout at most 2^24 values apart (64 of them within 4 GB); scale multiplies the scores; at
  * most 4 M rows (65535 tiles of 64 with one more per sequence). */
 int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int Hq, int D, int dtype);
+int melgpt_packed_attn_splits_for(long long Mq, long long Mk, int S, int Hq, int D, int dtype, long long longest);
 int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                            const void* v, long long v_row, long long v_head, const int* cu_q, const int* cu_k, int S, void* out,
                            long long o_row, long long o_head, void* out_low, float* lse, int write_gaps, int splits, float* workspace,

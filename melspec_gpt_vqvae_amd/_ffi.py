@@ -136,6 +136,7 @@ _PROTOS = {
     "melgpt_kv_append": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _p, _l, _i, _i, _p, _i, _i, _f, _p, _p, _f, _p, _i, _p, _p,
                          _l, _i, _l, _i, _i, _i, _i, _p],
     "melgpt_packed_attn_splits": [_l, _l, _i, _i, _i, _i],
+    "melgpt_packed_attn_splits_for": [_l, _l, _i, _i, _i, _i, _l],
     "melgpt_packed_attn_fwd": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _i, _p, _l, _l, _p, _p, _i, _i, _p, _l, _l, _i, _i, _i, _f, _i, _p],
     "melgpt_packed_attn_bwd": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _p, _i, _p, _l, _l, _p, _p, _l, _l, _p, _p, _p, _l, _l, _p,
                                _l, _l, _p, _l, _l, _i, _i, _p, _l, _l, _i, _i, _i, _f, _i, _p],

@@ -146,8 +146,8 @@ __device__ __forceinline__ void cos_sin(int pos, const double* turns_per_pos, fl
 // (products and sums are fused by hand here and below: left to hipcc, which of them it fuses differs between the kernels, and
 // a key would not have the same bits in a cache as outside.  Values that do not turn are left as they are: a turn by nothing
 // would multiply a neighbour by 0, and 0 * NaN is not 0.  By a choice of every result, except in the forward without a cache,
-// where the lanes that do not turn skip this: 14590 rows of 16 + 4 heads of 64 in bf16 take 22.5 us on the way into a cache,
-// 26.5 behind a branch, and 16385 of 32 + 8 of 128 without one 71 behind a branch, 73 by a choice.)
+// where the lanes that do not turn skip this: 14590 rows of 16 + 4 heads of 64 in bf16 take 23 us a call into a cache, 27
+// behind a branch, and 16385 of 32 + 8 of 128 without one 71 behind a branch, 73 turned by nothing.)
 template <typename T, bool INTERLEAVED>
 __device__ __forceinline__ void turn(float* x, const float* c, const float* s, bool turns) {
   using L = Lane<T, INTERLEAVED>;

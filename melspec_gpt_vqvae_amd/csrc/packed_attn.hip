@@ -36,6 +36,8 @@ struct PackedParams {
   float *lse, *delta;            // (Hq, Mq)
   const int *cu_q, *cu_k;        // (S + 1)
   int splits;                    // 16-bit: workgroups that share a row tile's keys (forward) or a key tile's query heads (backward)
+  int usual, pool_rows;          // a forward with a pool: shares of the sequences that are not long; its rows in the grid
+  unsigned by_usual, by_splits;  // 2^31 over usual and splits, rounded up
   float* part;                   // splits > 1: (splits, Hq, Mq, D) sums of e^(s - m) v, then (splits, Hq, Mq, 2): m (base 2), sums;
                                  // backward: (splits, [dk, dv], Mk, Hk, D)
   int S, Hq, Hk, G, write_gaps;  // write_gaps: zero the rows no sequence owns (2: those of lse and low, not of o)
@@ -239,8 +241,8 @@ struct Stage {
 
 // a tile of B rows that no sequence owns: the forward's zeros (256 threads)
 template <typename T, int D, int B>
-__device__ __forceinline__ void rows_of_nobody(const PackedParams& p, const Rows& R, int h, int t) {
-  if (!p.write_gaps || blockIdx.z) return;
+__device__ __forceinline__ void rows_of_nobody(const PackedParams& p, const Rows& R, int h, int z, int t) {
+  if (!p.write_gaps || z) return;
   constexpr int VEC = 16 / sizeof(T), C = D / VEC;                 // 16-byte pieces of a row
   const u32x4 zero = {0u, 0u, 0u, 0u};
   const int first = B * R.tile, n = min(R.n - first, B);
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
   head_of(blockIdx.x, p, h);
   const Rows R = find_rows<64, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
   if (!R.any) return;
-  if (R.seq < 0 || R.seq >= p.S) return rows_of_nobody<T, D, 64>(p, R, h, t);
+  if (R.seq < 0 || R.seq >= p.S) return rows_of_nobody<T, D, 64>(p, R, h, 0, t);
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
   const int q_in = 64 * R.tile + 16 * wave + (lane & 15);          // this lane's query within its sequence
@@ -462,18 +464,64 @@ __device__ __forceinline__ bool clean_tile(char* tile, int t) {
   return found;
 }
 
-template <int D>
-__global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
+// Shares of a row tile's `every` key tiles: `usual` of them (which a mean length decides), but of 16 tiles at most while there
+// are `splits` for that, so that one long sequence among short ones is not walked alone.
+__device__ __forceinline__ int pool_share(const PackedParams& p, int every) {
+  // (quotients rounded up, exact below 2^27 for divisors up to 16: two integer divisions are a tenth of a short share's time)
+  const int even = (int)__umulhi((unsigned)(every + p.usual - 1) << 1, p.by_usual);
+  const int least = (int)__umulhi((unsigned)(every + p.splits - 1) << 1, p.by_splits);
+  return max(max(min(even, 16), least), 1);
+}
+// (With 16 splits or fewer a tile that sees more keys never has fewer shares, so a sequence's last tile tells how many.)
+// Those beyond the usual ones are taken by the pool, the grid's first rows of workgroups, which find them from the lengths: each
+// in strides of the pool, of all in order of sequence, row tile (the last first), share and query head.  128 queries over 16000
+// keys among 63 single ones over 64, 8 heads of 128: 254 us without, 61 with room by the sizes alone, 48 where the caller names
+// the longest; 32 heads 256 / 79, 16 of 64 199 / 40.  Where there is no long one the pool, the second launch and the arithmetic
+// cost 3 - 9 us (64 sequences of 4 over 1000, 32 heads of 128: 138 / 146; of 1 over 300, 16 of 64: 22 / 31): so the variant is
+// a kernel of its own and only taken where much is to be gained.  All lanes of a wave.
+__device__ __forceinline__ bool find_pooled(const PackedParams& p, unsigned e, int lane, Rows& r, int& h, int& z) {
+  for (int s0 = 0; s0 < p.S; s0 += 64) {
+    const int i = min(s0 + lane, p.S - 1) + 1;
+    const int lo = bound_at(p.cu_q, p.S, p.Mq, i), nq = max(bound_at(p.cu_q, p.S, p.Mq, i + 1) - lo, 0);
+    const int every = (bound_at(p.cu_k, p.S, p.Mk, i + 1) - bound_at(p.cu_k, p.S, p.Mk, i) + 63) >> 6;
+    const int some = s0 + lane < p.S && every > 0 ? (nq + 127) >> 7 : 0;
+    if (!__any(some > 0 && every > 16 * p.usual)) continue;
+    const int per = pool_share(p, every), more = max((every + per - 1) / per - p.usual, 0);
+    const unsigned mine = (unsigned)(some * more) * p.Hq;
+    unsigned upto = mine;                                          // of this and the lanes before
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const unsigned before = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += before;
+    }
+    const unsigned all = __builtin_amdgcn_readlane(upto, 63);
+    if (e < all) {
+      const int at = __builtin_ctzll(__ballot(upto > e));
+      const unsigned k = e - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
+      const unsigned shares = __builtin_amdgcn_readlane(more, at), j = k / (unsigned)p.Hq;
+      head_of((int)(k % (unsigned)p.Hq), p, h);
+      r.seq = s0 + at;
+      r.lo = __builtin_amdgcn_readlane(lo, at);
+      r.n = __builtin_amdgcn_readlane(nq, at);
+      r.tiles = (r.n + 127) >> 7;
+      r.tile = r.tiles - 1 - (int)(j / shares);
+      r.any = true;
+      z = p.usual + (int)(j % shares);
+      return true;
+    }
+    e -= all;
+  }
+  return false;
+}
+
+// one row tile's share z of its keys
+template <int D, bool POOL>
+__device__ __forceinline__ void fwd32_rows(const PackedParams& p, const Rows& R, int h, int z, char (&lds)[2][2][64 * Tile32<D>::RB],
+                                           int& odd) {
   using L = Tile32<D>;
   using T = bf16_t;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * L::RB];
-  __shared__ int odd;                                              // a value that is not finite in a tile the causal border cuts
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5;
-  int h;
-  head_of(blockIdx.x, p, h);
-  const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, blockIdx.y, lane);
-  if (!R.any) return;
-  if (R.seq < 0 || R.seq >= p.S) return rows_of_nobody<T, D, 128>(p, R, h, t);
+  if (R.seq < 0 || R.seq >= p.S) return rows_of_nobody<T, D, 128>(p, R, h, z, t);
   int k_lo, nk;
   other_rows(p.cu_k, p.S, p.Mk, R.seq, k_lo, nk);
   const int w0 = 128 * R.tile + 32 * wave;                     // the wave's first query
@@ -504,8 +552,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   for (int d = 0; d < L::DB; ++d) o[d] = zero16();
   float m = -__builtin_inff(), l[2] = {0.f, 0.f};                  // two partial sums: independent chains
   // this workgroup's share of the key tiles
-  const int every = (most + 63) >> 6, per = (every + p.splits - 1) / p.splits;
-  const int i0 = per * (int)blockIdx.z, tiles = min(every - i0, per), k_first = 64 * i0;   // (with out_low there is one share)
+  const int every = (most + 63) >> 6, per = POOL ? pool_share(p, every) : (every + p.splits - 1) / p.splits;
+  const int i0 = per * z, tiles = min(every - i0, per), k_first = 64 * i0;   // (with out_low there is one share)
+  if (POOL && z > 0 && tiles <= 0) return;                         // (the join knows as much)
   if (tiles > 0) {
     const Fetch64<D, false> fetch_k(p.k_row, wave, lane);
     const Fetch64<D, true> fetch_v(p.v_row, wave, lane);
@@ -633,8 +682,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   float sum = l[0] + l[1];
   sum += __shfl_xor(sum, 32, 64);
   if (q_in >= R.n) return;
-  if (p.splits > 1) {
-    const long long at = ((long long)blockIdx.z * p.Hq + h) * p.Mq + row;
+  if (POOL ? per < every : p.splits > 1) {
+    const long long at = ((long long)z * p.Hq + h) * p.Mq + row;
 #pragma unroll
     for (int d = 0; d < L::DB; ++d)
 #pragma unroll
@@ -666,25 +715,80 @@ __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   if (hh == 0) p.lse[h * p.Mq + row] = sum == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// joins the splits of a query in their order: D / 4 lanes, four values each
+template <int D, bool POOL>
+__global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * Tile32<D>::RB];
+  __shared__ int odd;                                              // a value that is not finite in a tile the causal border cuts
+  const int lane = threadIdx.x & 63;
+  int h, row_tile = blockIdx.y;
+  if constexpr (POOL) {
+    if (row_tile < p.pool_rows) {
+      if (blockIdx.z) return;
+      auto at = __builtin_amdgcn_kernarg_segment_ptr();
+      for (unsigned e = row_tile * p.Hq + blockIdx.x;;) {
+        asm volatile("" : "+s"(at));   // (arguments are read anew each time: kept over the loop they spill)
+        PackedParams a;
+        __builtin_memcpy(&a, (const void*)at, sizeof(a));
+        Rows R;
+        int z;
+        if (!find_pooled(a, e, lane, R, h, z)) return;
+        fwd32_rows<D, true>(a, R, h, z, lds, odd);
+        __syncthreads();                                           // (all waves are done with the tiles)
+        e += a.pool_rows * a.Hq;
+      }
+    }
+    row_tile -= p.pool_rows;
+  }
+  head_of(blockIdx.x, p, h);
+  const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, row_tile, lane);
+  if (R.any) fwd32_rows<D, POOL>(p, R, h, blockIdx.z, lds, odd);
+}
+
+// shares that the row tile of a query has behind a pool: a wave looks for its 64 / (D / 4) queries' sequences one after another
 template <int D>
+__device__ __forceinline__ int pooled_shares(const PackedParams& p, long long row, int lane) {
+  constexpr int TPQ = D / 4;
+  int shares = 0;
+#pragma unroll
+  for (int i = 0; i < 64 / TPQ; ++i) {
+    const int r = __builtin_amdgcn_readlane((int)row, i * TPQ);
+    int lo = 0, n = p.S + 2;                                       // the last range that begins at or before the row
+    while (n > 1) {
+      const int step = (n + 63) / 64;
+      const unsigned long long m = __ballot(lane * step < n && bound_at(p.cu_q, p.S, p.Mq, lo + lane * step) <= r);
+      const int c = m ? 63 - __builtin_clzll(m) : 0;
+      lo += c * step;
+      n = min(step, n - c * step);
+    }
+    const int first = bound_at(p.cu_q, p.S, p.Mq, lo), nq = bound_at(p.cu_q, p.S, p.Mq, lo + 1) - first;
+    int k_lo, nk;
+    other_rows(p.cu_k, p.S, p.Mk, lo - 1, k_lo, nk);
+    const int last = min((r - first) | 127, nq - 1), every = (min(max(last + nk - nq + 1, 0), nk) + 63) >> 6;
+    const int per = pool_share(p, every), mine = (every + per - 1) / per;
+    if (lane / TPQ == i) shares = mine;
+  }
+  return shares;
+}
+
+// joins the splits of a query in their order: D / 4 lanes, four values each
+template <int D, bool POOL>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
   using T = bf16_t;
   constexpr int TPQ = D / 4;
-  const long long n = (long long)blockIdx.x * (256 / TPQ) + threadIdx.x / TPQ, all = (long long)p.Hq * p.Mq;
-  if (n >= all) return;
+  const long long all = (long long)p.Hq * p.Mq, mine = (long long)blockIdx.x * (256 / TPQ) + threadIdx.x / TPQ, n = min(mine, all - 1);
   const int d = 4 * (threadIdx.x % TPQ), h = (int)(n / p.Mq);
   const long long row = n % p.Mq;
   const bool gap = row < bound_at(p.cu_q, p.S, p.Mq, 1) || row >= bound_at(p.cu_q, p.S, p.Mq, p.S + 1);
-  if (gap) return;                                                 // (written by the forward itself)
+  const int shares = POOL ? pooled_shares<D>(p, row, threadIdx.x & 63) : p.splits;
+  if (mine >= all || gap || (POOL && shares <= 1)) return;         // (written by the forward itself)
   const float* st = p.part + (long long)p.splits * all * D + 2 * n;
   float top = -__builtin_inff();
-  for (int i = 0; i < p.splits; ++i) top = fmaxf(top, st[2 * i * all]);
+  for (int i = 0; i < shares; ++i) top = fmaxf(top, st[2 * i * all]);
   const float base = top == -__builtin_inff() ? 0.f : top;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < p.splits; ++i) {
+  for (int i = 0; i < shares; ++i) {
     const float f = __builtin_amdgcn_exp2f(st[2 * i * all] - base);
     a += *(const f32x4*)(p.part + (i * all + n) * D + d) * f;
     sum += st[2 * i * all + 1] * f;
@@ -1267,10 +1371,14 @@ int launch_fwd(const PackedParams& p, hipStream_t s) {
   const long long tiles = tiles_for(p.Mq, p.S, bm);
   if (tiles > 65535) return MELGPT_ERR_UNSUPPORTED;
   if constexpr (sizeof(T) == 2) {
-    hipLaunchKernelGGL((packed_fwd32_kernel<D>), dim3(p.Hq, (unsigned)tiles, (unsigned)p.splits), dim3(256), 0, s, p);
-    if (p.splits > 1) {
-      const long long per = 256 / (D / 4);
-      hipLaunchKernelGGL((packed_join_kernel<D>), dim3((unsigned)((p.Hq * p.Mq + per - 1) / per)), dim3(256), 0, s, p);
+    const long long per = 256 / (D / 4);
+    const dim3 joins((unsigned)((p.Hq * p.Mq + per - 1) / per));
+    if (p.usual) {
+      hipLaunchKernelGGL((packed_fwd32_kernel<D, true>), dim3(p.Hq, (unsigned)(p.pool_rows + tiles), p.usual), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((packed_join_kernel<D, true>), joins, dim3(256), 0, s, p);
+    } else {
+      hipLaunchKernelGGL((packed_fwd32_kernel<D, false>), dim3(p.Hq, (unsigned)tiles, (unsigned)p.splits), dim3(256), 0, s, p);
+      if (p.splits > 1) hipLaunchKernelGGL((packed_join_kernel<D, false>), joins, dim3(256), 0, s, p);
     }
   } else
     hipLaunchKernelGGL((packed_fwd_f32_kernel<D>), dim3(p.Hq, (unsigned)tiles), dim3(256), 0, s, p);
@@ -1297,29 +1405,51 @@ int launch_bwd(const PackedParams& p, hipStream_t s) {
   return melgpt_launch_status();
 }
 
+// what the launch rules know of a forward: row tiles' workgroups, how many run at once, key tiles of a mean sequence
+struct SplitModel {
+  double slots, tile_us, base, keys;
+  SplitModel(long long Mq, long long Mk, int S, int Hq, int D)
+      : slots(D == 64 ? 768 : 512), tile_us(D == 64 ? 0.9 : 1.7), base((double)Hq * (double)((Mq + 127) / 128 + (S - 1) / 2)),
+        keys((double)((Mk / S + 63) / 64)) {}
+};
+
 }  // namespace
 
 // Workgroups that share the keys of a row tile, where the row tiles alone would not fill the card (a prompt's continuation
-// over a long past).  By a model of the launch in microseconds: rounds of the 512 (D 128) or 768 (D 64) workgroups that run
-// at once, times a workgroup's 64-key tiles (1.7 / 0.9 us each with full CUs), plus the join (4 us, and 8 bytes a value and
-// split at 4 TB/s).  Measured in one piece / in the n it takes, 32 heads of 128 over 16000 keys: 1500 queries 516 / 416 us
-// (4), 512: 317 / 151 (4), 256: 312 / 91 (8), 128: 311 / 63 (16); 16 heads of 64, 1000 over 8000: 118 / 57 (6).
+// over a long past), by the mean length.  By a model of the launch in microseconds: rounds of the 512 (D 128) or 768 (D 64)
+// workgroups that run at once, times a workgroup's 64-key tiles (1.7 / 0.9 us each with full CUs), plus the join (4 us, and 8
+// bytes a value and split at 4 TB/s).  Measured in one piece / in the n it takes, 32 heads of 128 over 16000 keys: 1500 queries
+// 516 / 416 us (4), 512: 317 / 151 (4), 256: 312 / 91 (8), 128: 311 / 63 (16); 16 heads of 64, 1000 over 8000: 118 / 57 (6).
 extern "C" int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int Hq, int D, int dtype) {
   if (dtype != MELGPT_BF16 || Mq <= 0 || Mk <= 0 || S <= 0 || Hq <= 0 || (D != 64 && D != 128)) return 1;
-  const double slots = D == 64 ? 768 : 512, tile_us = D == 64 ? 0.9 : 1.7;
-  const double base = (double)Hq * (double)((Mq + 127) / 128 + (S - 1) / 2), keys = (double)((Mk / S + 63) / 64);
-  if (base > slots) return 1;
+  const SplitModel m(Mq, Mk, S, Hq, D);
+  if (m.base > m.slots) return 1;
   int best = 1;
   double least = 0;
-  for (int n = 1; n <= 16 && n * 4 <= keys + 3; ++n) {
-    const double rounds = (double)(long long)((base * n + slots - 1) / slots), each = (double)(long long)((keys + n - 1) / n);
-    const double us = rounds * each * tile_us + (n > 1 ? 4 + (double)Mq * Hq * n * D * 8 / 4e6 : 0);
+  for (int n = 1; n <= 16 && n * 4 <= m.keys + 3; ++n) {
+    const double rounds = (double)(long long)((m.base * n + m.slots - 1) / m.slots), each = (double)(long long)((m.keys + n - 1) / n);
+    const double us = rounds * each * m.tile_us + (n > 1 ? 4 + (double)Mq * Hq * n * D * 8 / 4e6 : 0);
     if (n == 1 || us < least) {
       least = us;
       best = n;
     }
   }
   return best;
+}
+
+// The same for a batch whose longest sequence has up to `longest` keys (the rule above goes by the mean): more where that one
+// would take over 100 us alone and twice the time that sequences of the mean length take together, within half a million
+// partial results.
+extern "C" int melgpt_packed_attn_splits_for(long long Mq, long long Mk, int S, int Hq, int D, int dtype, long long longest) {
+  const int usual = melgpt_packed_attn_splits(Mq, Mk, S, Hq, D, dtype);
+  if (dtype != MELGPT_BF16 || Mq <= 0 || Mk <= 0 || S <= 1 || Hq <= 0 || (D != 64 && D != 128)) return usual;
+  const SplitModel m(Mq, Mk, S, Hq, D);
+  const long long tiles = ((longest < Mk ? longest : Mk) + 63) / 64, room = (1 << 19) / (Hq * Mq);
+  const double alone = tiles * m.tile_us / usual, even = (m.base > m.slots ? m.base / m.slots : 1.) * m.keys * m.tile_us / usual;
+  long long n = (tiles + 15) / 16;
+  if (n > 16) n = 16;
+  if (n > room) n = room;
+  return n > usual && alone > 100 && alone > 2 * even ? (int)n : usual;
 }
 
 extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row,
@@ -1339,6 +1469,15 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
   if (!aligned16(workspace)) return MELGPT_ERR_ALIGN;
   if (Mq == 0) return MELGPT_OK;
   p.G = Hq / Hk;
+  const int usual = melgpt_packed_attn_splits(Mq, Mk, S, Hq, D, dtype);
+  // a pool of 512 workgroups or a row of heads (its numbers are 32-bit; 16 shares of 16 tiles or more: see find_pooled)
+  const int rows = (511 + Hq) / Hq;
+  if (splits > usual && splits <= 16 && Mk < (1 << 30) && rows + tiles_for(Mq, S, 128) <= 65535) {
+    p.usual = usual;
+    p.pool_rows = rows;
+    p.by_usual = ((1u << 31) + usual - 1) / usual;
+    p.by_splits = ((1u << 31) + splits - 1) / splits;
+  }
   single_rows(p, D);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == MELGPT_F32) return D == 64 ? launch_fwd<float, 64>(p, s) : launch_fwd<float, 128>(p, s);

@@ -1219,17 +1219,19 @@ def _packed_args(i, q, k, v, cu_q, cu_k):
 _FARTHEST = 1 << 24   # values between two rows of packed attention's inputs: 64 rows lie within 4 GB (melgpt_packed_attn_fwd)
 
 
-def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=False):
+def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=False, max_length=None):
     """Causal attention of packed sequences: q (Mq, Hq, D), k, v (Mk, Hk, D), any row and head strides, Hq a multiple of Hk;
     sequence s is rows cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1] of k and v (int32 on the device, rising from 0;
     cu_k None: the same).  Its last query sees all its keys, each one before it one key less; a query that sees none gives 0.
     -> (out (Mq, Hq, D), lse (Hq, Mq) f32).  `out`, where given, is a buffer of its own.  Rows behind the last sequence: left
     as they were in a given `out`, zero in a new one (lse -inf, low 0).  scale: 1 / sqrt(D) unless given.  want_low: -> (out,
     lse, low), low what rounding out to 16 bits took from it (None for f32), for packed_attn_bwd.  Values that are not finite
-    reach the queries that see them and no others."""
+    reach the queries that see them and no others.  max_length: the keys of the longest sequence, where the caller knows them;
+    it only decides how far the keys of a row are shared out (without it one sequence of a batch with a past may have half of
+    all keys; giving it spares a batch of like lengths up to 10 us)."""
     i = _device_of(q)
     if i != _current_device():
-        return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out, want_low=want_low)
+        return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out, want_low=want_low, max_length=max_length)
     dt = dtype_code(q.dtype)
     Mq, Mk, Hq, Hk, D, S, cu_k = _packed_args(i, q, k, v, cu_q, cu_k)
     vec = 4 if dt == _ffi.F32 else 8
@@ -1247,7 +1249,8 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     low = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device) if want_low and dt != _ffi.F32 else None
     splits, ws = 1, None
     if low is None and dt != _ffi.F32:
-        splits = _ffi.lib().melgpt_packed_attn_splits(Mq, Mk, S, Hq, D, dt)
+        longest = int(max_length) if max_length is not None else Mk // 2 if Mk > Mq else 0
+        splits = _ffi.lib().melgpt_packed_attn_splits_for(Mq, Mk, S, Hq, D, dt, longest)
         if splits > 1:   # (a buffer of the call's own: two captured graphs never share it)
             ws = torch.empty(splits * Hq * Mq * (D + 2), dtype=torch.float32, device=q.device)
     call("melgpt_packed_attn_fwd", q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, cu_q.data_ptr(),

@@ -38,17 +38,23 @@ def rotary_freqs(rot, base=10000.0, *, stretch=1.0, base_stretch=1.0, ramp=None,
     return f.to(device)
 
 
+_tracing = torch._C._get_tracing_state
+
+
 def _differentiated(*tensors):
     """whether one of them wants a gradient or carries a tangent of forward-mode differentiation"""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if grad or dual:
+        for t in tensors:
+            if t is not None and ((grad and t.requires_grad) or (dual and forward_ad.unpack_dual(t).tangent is not None)):
+                return True
+    return False
 
 
 def _through_autograd(*tensors):
     """whether a call goes through its autograd function: for a gradient; with a tangent, which the function refuses and the
     bare kernel would drop; and in a trace, which holds the function and not the kernel"""
-    return _differentiated(*tensors) or torch._C._get_tracing_state() is not None
+    return _differentiated(*tensors) or _tracing() is not None
 
 
 class _QkNormRotaryFn(torch.autograd.Function):
@@ -71,7 +77,8 @@ class _QkNormRotaryFn(torch.autograd.Function):
 
 def qk_norm_rotary(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
     """ops.qk_norm_rotary_fwd with gradients for q, k and both weights (not for freqs)."""
-    assert not _differentiated(freqs), "the frequencies have no gradient: give them detached"
+    if freqs is not None and (freqs.requires_grad or forward_ad._current_level >= 0):
+        assert not _differentiated(freqs), "the frequencies have no gradient: give them detached"
     if not _through_autograd(q, k, q_weight, k_weight):
         return ops.qk_norm_rotary_fwd(q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
                                       amplitude=amplitude)
@@ -93,8 +100,9 @@ class _PackedAttentionFn(torch.autograd.Function):
         return ops.packed_attn_bwd(q, k, v, out, dout, lse, cu_q, cu_k, scale=ctx.scale, low=low) + (None, None, None)
 
 
-def packed_attention(q, k, v, cu_q, cu_k=None, *, scale=None):
-    """ops.packed_attn_fwd's output with gradients for q, k and v (those of a key head summed over its query heads)."""
+def packed_attention(q, k, v, cu_q, cu_k=None, *, scale=None, max_length=None):
+    """ops.packed_attn_fwd's output with gradients for q, k and v (those of a key head summed over its query heads).
+    max_length: as there (a call with gradients does not share keys out)."""
     if not _through_autograd(q, k, v):
-        return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale)[0]
+        return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, scale=scale, max_length=max_length)[0]
     return _PackedAttentionFn.apply(q, k, v, cu_q, cu_k, scale)

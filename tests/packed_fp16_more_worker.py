@@ -34,6 +34,9 @@ def main():
     for il in (False, True):
         pe.test_values_beyond_the_rotation_pass_unchanged(5, 3, 2, 64, 32, il, "half")
     pe.test_log_sums_of_rows_that_no_sequence_owns([4, 20], [50, 2080], "half")
+    for D in (64, 128):
+        pe.test_one_long_sequence_in_a_packed_batch(D, 31)
+    pe.test_long_sequences_in_a_large_batch_of_short_ones(16, 8, 64, "half")
     print("all ok", flush=True)
 
 

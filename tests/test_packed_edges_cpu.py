@@ -13,7 +13,7 @@ def _opaque(monkeypatch):
     def host(x, f):
         return torch.from_numpy(f(x.detach().numpy()).copy())
 
-    def attention(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=False):
+    def attention(q, k, v, cu_q, cu_k=None, *, want_low=False, **kw):
         o = host(q, lambda a: 2 * a + v.detach().numpy().mean())
         return (o, o[..., 0].t().contiguous(), None) if want_low else (o, o[..., 0])
 
@@ -148,3 +148,18 @@ def test_shares_of_a_long_sequence_in_a_large_batch():
         for Hq, Hk in ((32, 8), (16, 16), (1, 1)):
             n, usual = f(S, Hq, Hk, 1 << 30), -(-2048 // (S * Hk))
             assert 1 <= n <= 128 and S * Hq * n <= max(1 << 19, S * Hq * usual)                           # room for partial results
+
+
+def test_shares_of_a_long_sequence_in_a_packed_batch():
+    from melspec_gpt_vqvae_amd import _ffi
+
+    lib, H = _ffi.lib(), _ffi.BF16
+    f, g = lib.melgpt_packed_attn_splits, lib.melgpt_packed_attn_splits_for
+    for n in (63, 255):                                            # 128 queries over 16000 keys among tokens over 64
+        a = (128 + n, 16000 + 64 * n, n + 1, 8, 128, H)
+        assert f(*a) == 1 and g(*a, 16000) == 16 and g(*a, 64) == g(*a, 0) == 1
+    assert g(2000, 2000, 8, 16, 64, H, 2000) == f(2000, 2000, 8, 16, 64, H) == 1                          # nothing to gain
+    for a in ((1500, 16001, 1, 32, 128, H), (100, 100, 1, 16, 64, H), (1, 16000, 1, 32, 128, H), (200, 16000, 9, 8, 128, _ffi.F32), (0, 5, 3, 1, 64, H)):
+        assert g(*a, a[1]) == f(*a)                                # one sequence, the f32 lane, no rows: as before
+    for rows in (64, 4000, 100000):                                # room for partial results
+        assert g(rows, 10 ** 6, 60, 32, 128, H, 500000) * rows * 32 <= max(1 << 19, rows * 32)

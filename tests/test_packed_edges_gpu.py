@@ -321,3 +321,121 @@ def test_captured_decode_of_growing_lengths():
         for s, o, l, size, score in _decode_reference(q, kp, vp, table, lengths.tolist(), range(3)):
             # (half a bf16 step of values up to 5, the largest of these; the bits are held to the eager call's above)
             assert float((got[0][s].double() - o).abs().max()) <= 0.02 and (lengths[s] > 0 or torch.isinf(got[1][s]).all())
+
+
+# ------------------------------------------------------ a few long sequences in a batch of short ones: packed forward
+def _shares(lens_q, lens_k, Hq, D, max_length=None):
+    """(usual, with room for long ones) as ops.packed_attn_fwd asks for them"""
+    from melspec_gpt_vqvae_amd import _ffi
+
+    a = (sum(lens_q), sum(lens_k), len(lens_q), Hq, D, _ffi.BF16)
+    longest = max_length if max_length is not None else a[1] // 2 if a[1] > a[0] else 0
+    return _ffi.lib().melgpt_packed_attn_splits(*a), _ffi.lib().melgpt_packed_attn_splits_for(*a, longest)
+
+
+def _packed_check(lens_q, lens_k, Hq, Hk, D, seed, max_length=None, ahead=0, behind=0):
+    """against 64 bits, with rows of nobody in front and behind; a new and a given output"""
+    import packed_ref as R
+    import test_packed_attn_gpu as pa
+    from melspec_gpt_vqvae_amd import ops
+
+    dt = _dt("half")
+    q, k, v, _ = pa.make([ahead] + lens_q + [behind], [ahead] + lens_k + [behind], Hq, Hk, D, dt, seed)
+    for x in (q, k, v):
+        x[:ahead] = float("nan")
+        x[len(x) - behind:] = float("nan")
+    cu_q, cu_k = [(torch.tensor([0] + l).cumsum(0) + ahead).to(torch.int32).to(DEV) for l in (lens_q, lens_k)]
+    out, lse = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), cu_q, cu_k, max_length=max_length)
+    end = ahead + sum(lens_q)
+    mine = slice(ahead, end)
+    h, own = R.half_step(dt), [x[ahead:len(x) - behind] for x in (q, k, v)]
+    o, l = out[mine].cpu(), lse[:, mine].cpu()
+    for a, b, head, _, r in pa.reference(*own, lens_q, lens_k, D ** -0.5):
+        n = b.stop - b.start
+        rel = R.attention_relative(D, r["s_score"], n + 40, dt)[:, None]         # (the joins add up to 16 shares)
+        R.assert_within(o[a, head], r["o"], h * r["o"].abs() + rel * r["s_o"] + R.smallest(dt) * (1 + r["a_o"]), f"out {a} head {head}")
+        bound = (D + 4) * R.U * r["s_score"] + (n + 40) * R.U + 4 * R.U * r["lse"].abs().nan_to_num(posinf=0)
+        R.assert_within(l[head, a], r["lse"], bound, f"lse {a} head {head}")
+    for part in (slice(0, ahead), slice(end, end + behind)):
+        assert (out[part] == 0).all() and (lse[:, part] == -float("inf")).all()
+    given = torch.full_like(out, 5.0)
+    _poisoned((lse.shape, torch.float32))
+    _, lse2 = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), cu_q, cu_k, max_length=max_length, out=given)
+    assert torch.equal(given[mine], out[mine]) and torch.equal(lse2, lse) and (given[:ahead] == 5).all() and (given[end:] == 5).all()
+
+
+@pytest.mark.parametrize("where", [0, 31, 69])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_long_sequence_in_a_packed_batch(D, where):
+    lens_q, lens_k = [1 + i % 3 for i in range(70)], [1 + 7 * i % 90 for i in range(70)]
+    lens_q[5], lens_k[6], lens_q[7] = 0, 0, 100                     # no queries; no keys; queries that see none
+    lens_q[where], lens_k[where] = 128, 16001
+    usual, room = _shares(lens_q, lens_k, 4, D)
+    assert room > usual
+    _packed_check(lens_q, lens_k, 4, 2, D, 5, ahead=3, behind=40)
+
+
+def test_long_sequences_of_several_row_tiles_and_more_shares_than_workgroups_that_look_for_them():
+    lens_q, lens_k = [3] * 66, [40] * 66
+    for s, n, m in ((2, 300, 4000), (63, 1, 9000), (64, 140, 2300), (65, 129, 6001)):
+        lens_q[s], lens_k[s] = n, m
+    usual, room = _shares(lens_q, lens_k, 32, 64, 9000)
+    assert room > usual
+    _packed_check(lens_q, lens_k, 32, 8, 64, 6, max_length=9000)    # 32 heads x (3 + 1 + 2 + 2 row tiles) x up to 7 shares
+
+
+def test_one_long_prompt_among_tokens():
+    lens = [4001] + [1] * 63
+    usual, room = _shares(lens, lens, 2, 128, 4001)
+    assert usual == 1 < room and _shares(lens, lens, 2, 128) == (1, 1)
+    _packed_check(lens, lens, 2, 1, 128, 7, max_length=4001, behind=5)
+    _packed_check(lens, lens, 2, 1, 128, 7, max_length=100000)      # (a wrong hint decides the shares alone)
+
+
+def test_captured_packed_batch_whose_long_sequence_changes():
+    from melspec_gpt_vqvae_amd import ops
+    import test_packed_attn_gpu as pa
+
+    lens_q, lens_k = [2] * 70, [200] * 70
+    q, k, v, _ = [x.to(DEV) for x in pa.make(lens_q, lens_k, 8, 2, 64, _dt("half"), 8)]
+    cu_q, cu_k = pa._cu(lens_q).to(DEV), pa._cu(lens_k).to(DEV)
+    usual, room = _shares(lens_q, lens_k, 8, 64, 14000)
+    assert room > usual
+    step = lambda: ops.packed_attn_fwd(q, k, v, cu_q, cu_k, max_length=14000)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    even = cu_k.clone()
+    for first, last in ((0, 0), (13000, 0), (0, 13000), (5000, 8000)):
+        cu_k.copy_(even)                                            # keys moved to the first or the last sequence
+        cu_k[1:70] = torch.maximum(cu_k[1:70], torch.full_like(cu_k[1:70], first)).clamp(max=14000 - last)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        plain = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, max_length=0)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        # both round probabilities and output: two half steps each of the sizes (values up to 5 in few keys, weights that add to 1)
+        assert float((got[0].float() - plain[0].float()).abs().max()) <= 4 * 5 * 2.0 ** -8
+        assert torch.allclose(got[1], plain[1], rtol=0, atol=1e-4)
+
+
+def test_values_that_are_not_finite_in_a_long_sequence_of_a_batch():
+    from melspec_gpt_vqvae_amd import ops
+    import test_packed_attn_gpu as pa
+
+    lens_q, lens_k = [2] * 40 + [100], [20] * 40 + [16000]
+    q, k, v, _ = pa.make(lens_q, lens_k, 4, 2, 128, _dt("half"), 9)
+    cu_q, cu_k = pa._cu(lens_q).to(DEV), pa._cu(lens_k).to(DEV)
+    usual, room = _shares(lens_q, lens_k, 4, 128)
+    assert room > usual
+    base, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), v.to(DEV), cu_q, cu_k)
+    bad = v.clone()
+    bad[800 + 15900 + 60, 0, 3] = float("nan")                      # key 15960 of the long one: its queries 60 and on see it
+    bad[800 + 15999, 1, 7] = float("inf")                           # its last query alone
+    out, _ = ops.packed_attn_fwd(q.to(DEV), k.to(DEV), bad.to(DEV), cu_q, cu_k)
+    want = base.clone()
+    want[80 + 60:, :2, 3] = float("nan")
+    want[80 + 99, 2:, 7] = float("inf")
+    assert ((out == want) | (torch.isnan(out) & torch.isnan(want))).all()
