@@ -567,7 +567,7 @@ int melgpt_qk_norm_rotary_bwd(const void* dq_out, long long dq_row, long long dq
  * Row r belongs to sequence sequences[r] and is stored at positions[r]: page page_table[seq * table_ld + pos / page_size],
  * slot pos % page_size.  A row of negative position or sequence is padding: nothing is stored and its q_out row is left as
  * it was (zero_pad: zeroed).  A row whose sequence, table column or page lies outside S, width or n_pages is not stored
- * (the kernel checks every index); two rows of one slot leave one of them. */
+ * (the kernel checks every index); of two rows in one slot each head keeps one or the other. */
 int melgpt_kv_append(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                      const void* v, long long v_row, long long v_head, const int* sequences, const int* positions,
                      const int* page_table, long long table_ld, int S, int width, const double* freqs, int rot,

@@ -7,7 +7,7 @@
 //   pairs: halves (i, i + rot / 2), or interleaved (2 i, 2 i + 1)
 //   backward, u = R(-t) dy:   dw = sum x^ u,  dx = r (u w - x^ mean_d(u w x^)),  x^ = x r,  r = rsqrt(...)
 //
-// Bound by HBM: every value is read and written once (bf16, 16385 rows of 32 + 8 heads of 128: 336 MB in 74 us, 4.5 TB/s where
+// Bound by HBM: every value is read and written once (bf16, 16385 rows of 32 + 8 heads of 128: 336 MB in 73 us, 4.6 TB/s where
 // a large copy reaches 4.9; forward and backward of 33920 rows of 16 + 16 heads of 64: 695 MB in 170 us; appended to a cache,
 // 14590 rows of 16 + 4 + 4 heads of 64: 90 MB in 24 us).  A lane holds two 16-byte vectors of one head, chosen so that both
 // members of its pairs are its own (halves: the vectors at V j and rot / 2 + V j; interleaved: neighbours), so the rotation

@@ -358,7 +358,7 @@ __global__ __launch_bounds__(256) void packed_fwd_f32_kernel(PackedParams p) {
 // ------------------------------------------------------------------------------------- forward, 16-bit operands
 // 256 threads, 128 queries of one head: a wave owns 32 queries (v_mfma_f32_32x32x16: twice the queries per fragment read from
 // LDS, which 16-row tiles are bound by) and walks the keys 64 at a time.  bf16, 32 heads over 8 of 128: eight prompts of up to
-// 4097 in 304 us (855 TFLOP/s, of 1361 in a large matrix product), 1500 queries over 16001 keys in 381 us (984 TFLOP/s).  It is
+// 4097 in 295 us (879 TFLOP/s, of 1361 in a large matrix product), 1500 queries over 16001 keys in 383 us (978 TFLOP/s).  It is
 // bound by matrix and vector instructions together: a step's 32 exponentials and 100 others need nearly the time of its 16
 // products, and the clock sinks under both (on zeros the same instructions run 1.4 times as fast).
 template <int D>
@@ -400,7 +400,10 @@ __device__ __forceinline__ float halves_max(float v) {
   const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
   return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// accumulators 8 st .. 8 st + 7 of a 32-row block as the operand of a 16-row contraction
+// accumulators 8 st .. 8 st + 7 of a 32-row block as the operand of a 16-row contraction.  Probabilities and score gradients are
+// rounded to 16 bits here, and only here: the second products want 16-bit operands (in f32 they would run at 154 TFLOP/s, not
+// 1361), and a product of independent roundings adds no more than the result's own: of its norm, in bf16, the output is 0.0020
+// off (0.0017 with f32 probabilities), the gradients 0.0024.  Statistics and sums are taken before it.
 __device__ __forceinline__ u32x4 operand16(const f32x16& s, int st) {
   return u32x4{pack_bf16x2(s[8 * st], s[8 * st + 1]), pack_bf16x2(s[8 * st + 2], s[8 * st + 3]),
                pack_bf16x2(s[8 * st + 4], s[8 * st + 5]), pack_bf16x2(s[8 * st + 6], s[8 * st + 7])};
@@ -976,7 +979,8 @@ __global__ __launch_bounds__(256) void packed_dkv_f32_kernel(PackedParams p) {
 
 // ------------------------------------------------------------------------------------ backward, 16-bit operands
 // dq and delta: a wave owns 32 queries, 64 keys a step; K lies in LDS in the order its transposed reads want (its row reads
-// meet no bank twice in that order either).  Three products, 16 heads over 4 of 128 as below: 205 us, 770 TFLOP/s.
+// meet no bank twice in that order either).  Three products, 16 heads over 4 of 128 as below: 204 us, 770 TFLOP/s (uneven work here too:
+// 67 key tiles on the longest of the 512 places, 53 evenly).
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
   using L = Tile32<D>;
@@ -1107,8 +1111,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq32_kernel(PackedParams p) {
 // one barrier a block.  Three tiles of queries and output gradients lie in LDS (the last, this one, the one being stored).
 // The halves qh are added at the end, in LDS.  (One wave for both gradients, one to a SIMD, was as fast while tiles came through
 // registers, but it issues every instruction of a block itself, and 400 of them take longer than its 32 products.)
-// 16 heads over 4 of 128 in bf16, sequences of 4096, 265, 1999, 1, 800, 2050: 350 us for its four products (210 GFLOP), 600
-// TFLOP/s; what bounds it is LDS (fragments of four tiles and the probabilities' way from A to B) beside one block in flight.
+// 16 heads over 4 of 128 in bf16, sequences of 4096, 265, 1999, 1, 800, 2050: 324 us for its four products (210 GFLOP), 650
+// TFLOP/s; what bounds it is LDS (fragments of four tiles and the probabilities' way from A to B) beside one block in flight, and
+// uneven work: a key tile has the query blocks behind it to do, one workgroup runs on a CU, and the longest of the 256 CUs'
+// turns are 264 blocks there where an even share is 205.
 template <int D>
 __global__ __launch_bounds__(512, 2) void packed_dkv32_kernel(PackedParams p) {
   using L = Tile32<D>;
@@ -1484,9 +1490,12 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
   return D == 64 ? launch_fwd<bf16_t, 64>(p, s) : launch_fwd<bf16_t, 128>(p, s);
 }
 
-// Workgroups that share a key tile's query heads, where the key tiles alone (one workgroup a CU) would not fill the card twice:
-// one key head of 128 under 8, 4000 tokens, whole backward: 596 us in one piece, 238 in 8; two under 16: 647 / 379 in 4; four
-// under 16, 4096 tokens: 409 / 326 in 2.  Beyond twice the card it loses: eight under 32 heads of 64, 4000 tokens 344 / 360.
+// Workgroups that share a key tile's query heads, as many as keep a launch within 512 workgroups (two rounds of one to a CU): two
+// or more while there are up to 256 key tiles.  One key head of 128 under 8, 4000 tokens, whole backward: 596 us in one piece,
+// 238 in 8; two under 16: 647 / 379 in 4; four under 16, 4096 tokens: 409 / 326 in 2.  It counts tiles, not their work: from 257
+// to some 400 of them two shares would still help long sequences (four heads under 16, 4700 tokens, 296 tiles: 474 / 404; 6400:
+// 682 / 664; two under 14, lengths 4096 to 1: 635 / 450) but cost short ones more (17 of 265, 316 tiles: 96 / 109), and beyond
+// they lose (eight under 32 heads of 64, 4000 tokens: 339 / 359).
 extern "C" int melgpt_packed_attn_bwd_splits(long long Mk, int S, int Hq, int Hk, int dtype) {
   if (dtype != MELGPT_BF16 || Mk <= 0 || S <= 0 || Hk <= 0 || Hq <= Hk) return 1;
   const long long base = Hk * ((Mk + 63) / 64 + (S - 1) / 2), n = 512 / base;

@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
       for (int d = 0; d < L::DT; ++d) o[d] *= keep;
 #pragma unroll
       for (int e = 0; e < L::STEPS; ++e) {
-        u32x4 pf;
+        u32x4 pf;   // (16-bit lane: probabilities rounded for the second product, as in packed_attn.hip; summed in f32 above)
         if constexpr (L::ES == 2)
           pf = u32x4{pack_bf16x2(sc[0][0], sc[0][1]), pack_bf16x2(sc[0][2], sc[0][3]), pack_bf16x2(sc[1][0], sc[1][1]),
                      pack_bf16x2(sc[1][2], sc[1][3])};
