@@ -36,7 +36,7 @@ struct PackedParams {
   float *lse, *delta;            // (Hq, Mq)
   const int *cu_q, *cu_k;        // (S + 1)
   int splits;                    // 16-bit: workgroups that share a row tile's keys (forward) or a key tile's query heads (backward)
-  int usual, pool_rows;          // a forward with a pool: shares of the sequences that are not long; its rows in the grid
+  int usual;                     // a forward with a pool: shares of the sequences that are not long
   unsigned by_usual, by_splits;  // 2^31 over usual and splits, rounded up
   float* part;                   // splits > 1: (splits, Hq, Mq, D) sums of e^(s - m) v, then (splits, Hq, Mq, 2): m (base 2), sums;
                                  // backward: (splits, [dk, dv], Mk, Hk, D)
@@ -469,6 +469,7 @@ __device__ __forceinline__ bool clean_tile(char* tile, int t) {
 
 // Shares of a row tile's `every` key tiles: `usual` of them (which a mean length decides), but of 16 tiles at most while there
 // are `splits` for that, so that one long sequence among short ones is not walked alone.
+constexpr unsigned POOLED = 512;
 __device__ __forceinline__ int pool_share(const PackedParams& p, int every) {
   // (quotients rounded up, exact below 2^27 for divisors up to 16: two integer divisions are a tenth of a short share's time)
   const int even = (int)__umulhi((unsigned)(every + p.usual - 1) << 1, p.by_usual);
@@ -476,14 +477,20 @@ __device__ __forceinline__ int pool_share(const PackedParams& p, int every) {
   return max(max(min(even, 16), least), 1);
 }
 // (With 16 splits or fewer a tile that sees more keys never has fewer shares, so a sequence's last tile tells how many.)
-// Those beyond the usual ones are taken by the pool, the grid's first rows of workgroups, which find them from the lengths: each
-// in strides of the pool, of all in order of sequence, row tile (the last first), share and query head.  128 queries over 16000
-// keys among 63 single ones over 64, 8 heads of 128: 254 us without, 61 with room by the sizes alone, 48 where the caller names
-// the longest; 32 heads 256 / 79, 16 of 64 199 / 40.  Where there is no long one the pool, the second launch and the arithmetic
-// cost 3 - 9 us (64 sequences of 4 over 1000, 32 heads of 128: 138 / 146; of 1 over 300, 16 of 64: 22 / 31): so the variant is
-// a kernel of its own and only taken where much is to be gained.  All lanes of a wave.
-__device__ __forceinline__ bool find_pooled(const PackedParams& p, unsigned e, int lane, Rows& r, int& h, int& z) {
-  for (int s0 = 0; s0 < p.S; s0 += 64) {
+// Those beyond the usual ones are taken by a pool of workgroups, which find them from the lengths: number e, e + POOLED, .. of
+// all in order of sequence, row tile (the last first), share and query head.  128 queries over 16000 keys among 63 single ones
+// over 64, 8 heads of 128: 252 us without, 94 with; 32 heads 255 / 105, 16 of 64 201 / 65.  Where there is no long one the two
+// launches more cost some 6 us (100 sequences of 2 queries over 300 keys, 8 heads of 64: 21 / 28; of 1 over 1000, 16: 93 / 96).
+// All lanes of a wave.
+// s0, e: where the search stands (number e of those from sequence s0 on); it goes on there for the next.
+__device__ __forceinline__ bool any_pooled(const PackedParams& p, int lane) {
+  bool any = false;                                                // (loads side by side; the search waits for each)
+#pragma unroll 4
+  for (int i = lane + 1; i <= p.S; i += 64) any = any || bound_at(p.cu_k, p.S, p.Mk, i + 1) - bound_at(p.cu_k, p.S, p.Mk, i) > 1024 * p.usual;
+  return __any(any);
+}
+__device__ __forceinline__ bool find_pooled(const PackedParams& p, int& s0, unsigned& e, int lane, Rows& r, int& h, int& z) {
+  for (; s0 < p.S; s0 += 64) {
     const int i = min(s0 + lane, p.S - 1) + 1;
     const int lo = bound_at(p.cu_q, p.S, p.Mq, i), nq = max(bound_at(p.cu_q, p.S, p.Mq, i + 1) - lo, 0);
     const int every = (bound_at(p.cu_k, p.S, p.Mk, i + 1) - bound_at(p.cu_k, p.S, p.Mk, i) + 63) >> 6;
@@ -722,29 +729,31 @@ template <int D, bool POOL>
 __global__ __launch_bounds__(256, 2) void packed_fwd32_kernel(PackedParams p) {
   __shared__ __attribute__((aligned(16))) char lds[2][2][64 * Tile32<D>::RB];
   __shared__ int odd;                                              // a value that is not finite in a tile the causal border cuts
-  const int lane = threadIdx.x & 63;
-  int h, row_tile = blockIdx.y;
-  if constexpr (POOL) {
-    if (row_tile < p.pool_rows) {
-      if (blockIdx.z) return;
-      auto at = __builtin_amdgcn_kernarg_segment_ptr();
-      for (unsigned e = row_tile * p.Hq + blockIdx.x;;) {
-        asm volatile("" : "+s"(at));   // (arguments are read anew each time: kept over the loop they spill)
-        PackedParams a;
-        __builtin_memcpy(&a, (const void*)at, sizeof(a));
-        Rows R;
-        int z;
-        if (!find_pooled(a, e, lane, R, h, z)) return;
-        fwd32_rows<D, true>(a, R, h, z, lds, odd);
-        __syncthreads();                                           // (all waves are done with the tiles)
-        e += a.pool_rows * a.Hq;
-      }
-    }
-    row_tile -= p.pool_rows;
-  }
+  int h;
   head_of(blockIdx.x, p, h);
-  const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, row_tile, lane);
+  const Rows R = find_rows<128, true>(p.cu_q, p.S, p.Mq, blockIdx.y, threadIdx.x & 63);
   if (R.any) fwd32_rows<D, POOL>(p, R, h, blockIdx.z, lds, odd);
+}
+
+// the pool (a launch in front: among the others it would take registers from them, and a wave of three at head size 64)
+template <int D>
+__global__ __launch_bounds__(256, 2) void packed_fwd32_pool_kernel(PackedParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[2][2][64 * Tile32<D>::RB];
+  __shared__ int odd;
+  const int lane = threadIdx.x & 63;
+  if (!any_pooled(p, lane)) return;
+  auto at = __builtin_amdgcn_kernarg_segment_ptr();
+  int s0 = 0;
+  for (unsigned e = blockIdx.x;; e += POOLED) {
+    asm volatile("" : "+s"(at));   // (arguments are read anew each time: kept over the loop they spill)
+    PackedParams a;
+    __builtin_memcpy(&a, (const void*)at, sizeof(a));
+    Rows R;
+    int h, z;
+    if (!find_pooled(a, s0, e, lane, R, h, z)) return;
+    fwd32_rows<D, true>(a, R, h, z, lds, odd);
+    __syncthreads();                                               // (all waves are done with the tiles)
+  }
 }
 
 // shares that the row tile of a query has behind a pool: a wave looks for its 64 / (D / 4) queries' sequences one after another
@@ -1380,7 +1389,8 @@ int launch_fwd(const PackedParams& p, hipStream_t s) {
     const long long per = 256 / (D / 4);
     const dim3 joins((unsigned)((p.Hq * p.Mq + per - 1) / per));
     if (p.usual) {
-      hipLaunchKernelGGL((packed_fwd32_kernel<D, true>), dim3(p.Hq, (unsigned)(p.pool_rows + tiles), p.usual), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((packed_fwd32_pool_kernel<D>), dim3(POOLED), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((packed_fwd32_kernel<D, true>), dim3(p.Hq, (unsigned)tiles, p.usual), dim3(256), 0, s, p);
       hipLaunchKernelGGL((packed_join_kernel<D, true>), joins, dim3(256), 0, s, p);
     } else {
       hipLaunchKernelGGL((packed_fwd32_kernel<D, false>), dim3(p.Hq, (unsigned)tiles, (unsigned)p.splits), dim3(256), 0, s, p);
@@ -1445,10 +1455,11 @@ extern "C" int melgpt_packed_attn_splits(long long Mq, long long Mk, int S, int 
 
 // The same for a batch whose longest sequence has up to `longest` keys (the rule above goes by the mean): more where that one
 // would take over 100 us alone and twice the time that sequences of the mean length take together, within half a million
-// partial results.
+// partial results and for up to 512 sequences: with thousands of short ones, looking for a long one costs as much as they do.
+static const int MOST_POOLED = 512;
 extern "C" int melgpt_packed_attn_splits_for(long long Mq, long long Mk, int S, int Hq, int D, int dtype, long long longest) {
   const int usual = melgpt_packed_attn_splits(Mq, Mk, S, Hq, D, dtype);
-  if (dtype != MELGPT_BF16 || Mq <= 0 || Mk <= 0 || S <= 1 || Hq <= 0 || (D != 64 && D != 128)) return usual;
+  if (dtype != MELGPT_BF16 || Mq <= 0 || Mk <= 0 || S <= 1 || S > MOST_POOLED || Hq <= 0 || (D != 64 && D != 128)) return usual;
   const SplitModel m(Mq, Mk, S, Hq, D);
   const long long tiles = ((longest < Mk ? longest : Mk) + 63) / 64, room = (1 << 19) / (Hq * Mq);
   const double alone = tiles * m.tile_us / usual, even = (m.base > m.slots ? m.base / m.slots : 1.) * m.keys * m.tile_us / usual;
@@ -1476,11 +1487,9 @@ extern "C" int melgpt_packed_attn_fwd(const void* q, long long q_row, long long 
   if (Mq == 0) return MELGPT_OK;
   p.G = Hq / Hk;
   const int usual = melgpt_packed_attn_splits(Mq, Mk, S, Hq, D, dtype);
-  // a pool of 512 workgroups or a row of heads (its numbers are 32-bit; 16 shares of 16 tiles or more: see find_pooled)
-  const int rows = (511 + Hq) / Hq;
-  if (splits > usual && splits <= 16 && Mk < (1 << 30) && rows + tiles_for(Mq, S, 128) <= 65535) {
+  // (a pool's numbers are 32-bit; 16 shares of 16 tiles or more: see find_pooled)
+  if (splits > usual && splits <= 16 && S <= MOST_POOLED && Mk < (1 << 30)) {
     p.usual = usual;
-    p.pool_rows = rows;
     p.by_usual = ((1u << 31) + usual - 1) / usual;
     p.by_splits = ((1u << 31) + splits - 1) / splits;
   }

@@ -86,18 +86,22 @@ __device__ __forceinline__ int share_of(const PagedParams& p, int tiles) {
   return POOL ? max(min(even, 128), (tiles + p.shares - 1) / p.shares) : even;
 }
 // The shares beyond the usual ones, of sequences longer than 4096 keys a usual share, so that they do not finish alone: the
-// first POOLED workgroups take them, and start first: number e, e + POOLED, .. of all in order of sequence, share and key
-// head.  256 sequences of 8 key heads of 128, one of 100000 keys among 255 of 500: 1401 us without, 184 with (512: 1445 / 277).
-// Where there are none but the table has room for them, looking for them and a second launch cost 7 us (256 of 500 keys: 104 /
-// 111); a grid with room for every sequence's shares cost 1 ns for each workgroup that had nothing to do, 2 us for each
-// further split there.  All lanes of a wave.
+// POOLED workgroups of a launch in front take them, number e, e + POOLED, .. of all in order of sequence, share and key head.
+// 8 key heads of 128, one sequence of 100000 keys among short ones of 500: 64 in all 371 us without, 160 with, 256 1403 / 207,
+// 512 1445 / 291.  Where there are none but the table has room for them, the two launches more cost 2 - 9 us (256 of 500 keys:
+// 105 / 110).  Among the others' workgroups the pool was no slower to help (256: 184), but its registers cost those a wave of
+// four at head size 64; a grid with room for every sequence's shares cost 1 ns for each workgroup that had nothing to do.
+// All lanes of a wave.
 constexpr unsigned POOLED = 1024;
-__device__ __forceinline__ bool find_pooled(const PagedParams& p, unsigned e, int lane, int& s, int& hk, int& split) {
-  bool any = false;                                                // (loads side by side; the search below waits for each)
+// s0, e: where the search stands (number e of those from sequence s0 on); it goes on there for the next.
+__device__ __forceinline__ bool any_pooled(const PagedParams& p, int lane) {
+  bool any = false;                                                // (loads side by side; the search waits for each)
 #pragma unroll 8
   for (int i = lane; i < p.S; i += 64) any = any || p.lengths[i] > 4096LL * p.usual;
-  if (!__any(any)) return false;
-  for (int s0 = 0; s0 < p.S; s0 += 64) {
+  return __any(any);
+}
+__device__ __forceinline__ bool find_pooled(const PagedParams& p, int& s0, unsigned& e, int lane, int& s, int& hk, int& split) {
+  for (; s0 < p.S; s0 += 64) {
     const int tiles = s0 + lane < p.S ? (length_of(p, s0 + lane) + 31) >> 5 : 0;
     const int per = share_of<true>(p, tiles);
     const unsigned mine = (unsigned)max((tiles + per - 1) / per - p.usual, 0) * p.Hk;
@@ -121,20 +125,23 @@ __device__ __forceinline__ bool find_pooled(const PagedParams& p, unsigned e, in
   return false;
 }
 
-template <typename T, int D, bool POOL>
+// which workgroups a launch has: all (no pool), those of the usual shares, the pool
+enum { ALL_SHARES, USUAL_SHARES, POOLED_SHARES };
+template <typename T, int D, int WHICH>
 __global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
   using L = Geo<T, D>;
   __shared__ __attribute__((aligned(16))) char lds[4][32 * L::RB];
   __shared__ float stat[4][2][16];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = lane >> 4, i16 = lane & 15;
   const int nh = min(p.G - 16 * (int)blockIdx.z, 16);             // query heads of this workgroup
-  const bool pooled = POOL && blockIdx.x < POOLED;
+  constexpr bool POOL = WHICH == POOLED_SHARES;
+  if (POOL && !any_pooled(p, lane)) return;
+  int s0 = 0;
   for (unsigned e = blockIdx.x;; e += POOLED) {
-    const int pairs = p.S * p.Hk, w = POOL ? (int)(blockIdx.x - POOLED) : (int)blockIdx.x;
-    int split = POOL ? w / pairs : (int)blockIdx.y, s = (POOL ? w % pairs : w) / p.Hk, hk = (POOL ? w % pairs : w) % p.Hk;
-    if (pooled && !find_pooled(p, e, lane, s, hk, split)) return;
+    int hk = blockIdx.x % p.Hk, s = blockIdx.x / p.Hk, split = blockIdx.y;
+    if (POOL && !find_pooled(p, s0, e, lane, s, hk, split)) return;
     const int h0 = hk * p.G + 16 * blockIdx.z;
-    const int len = length_of(p, s), tiles = (len + 31) >> 5, per = share_of<POOL>(p, tiles);
+    const int len = length_of(p, s), tiles = (len + 31) >> 5, per = share_of<WHICH != ALL_SHARES>(p, tiles);
     if (split > 0 && (long long)split * per >= tiles) return;        // (the join knows as much)
     const int t0 = split * per, t1 = min(t0 + per, tiles);
     const int* table = p.table + (long long)s * p.table_ld;
@@ -279,7 +286,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(PagedParams p) {
         }
       }
     }
-    if (!POOL || !pooled) return;
+    if (!POOL) return;
     __syncthreads();                                                 // (the waves' results are read before the next share's rows)
   }
 }
@@ -346,8 +353,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <typename T, int D, bool POOL>
 int launch_as(const PagedParams& p, hipStream_t s) {
   const unsigned pairs = (unsigned)(p.S * p.Hk), z = (p.G + 15) / 16;
-  const dim3 grid = POOL ? dim3(POOLED + pairs * p.usual, 1, z) : dim3(pairs, p.usual, z);
-  hipLaunchKernelGGL((paged_decode_kernel<T, D, POOL>), grid, dim3(256), 0, s, p);
+  if (POOL) hipLaunchKernelGGL((paged_decode_kernel<T, D, POOLED_SHARES>), dim3(POOLED, 1, z), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((paged_decode_kernel<T, D, POOL ? USUAL_SHARES : ALL_SHARES>), dim3(pairs, p.usual, z), dim3(256), 0, s, p);
   if (p.splits > 1) {
     const int each = p.S < 4096 ? 4096 / p.S : 1;                  // workgroups to a sequence
     const dim3 joins = POOL ? dim3((unsigned)p.S, each < p.Hq ? each : p.Hq) : dim3((unsigned)(p.S * p.Hq));
@@ -368,14 +375,16 @@ int launch(const PagedParams& p, hipStream_t s) {
 // heads 243 / 211 in 4 / 204 in 8, but all of 4096 191 / 205 in 4 / 224 in 8.
 static long long usual_splits(long long base) { return (2048 + base - 1) / base; }
 
-// Beyond these, room for a split to each 4096 keys of a sequence as long as the longest may be (find_pooled), within half a
-// million partial results.
+// Beyond these, room for a split to each 4096 keys of a sequence as long as the longest may be (find_pooled), where that is over
+// four usual shares of 4096 (256 sequences of lengths up to 8192: 812 us without, 860 with a pool), within half a million
+// partial results and for up to 512 sequences (thousands of short ones: looking for a long one costs as much as they do).
+static const int MOST_POOLED = 512;
 extern "C" int melgpt_paged_attn_splits(int S, int Hq, int Hk, long long max_length) {
   if (S <= 0 || Hk <= 0 || Hq < Hk || max_length <= 512) return 1;
   const long long base = (long long)S * Hk * ((Hq / Hk + 15) / 16), most = (max_length + 127) / 128, room = (1 << 19) / ((long long)S * Hq);
   long long n = usual_splits(base), more = (max_length + 4095) / 4096;
   if (more > room) more = room;
-  if (n < more) n = more;
+  if (S <= MOST_POOLED && max_length > 16384 * n && n < more) n = more;
   if (n > most) n = most;
   if (n > 128) n = 128;
   return (int)(n < 1 ? 1 : n);
@@ -408,7 +417,8 @@ extern "C" int melgpt_paged_attn_decode(const void* q, long long q_row, long lon
   p.least = base < 256 ? 4 : 16;
   p.shares = splits;
   p.usual = splits;
-  if (splits > usual && pairs <= (1 << 20) && pairs * splits < (1LL << 31)) p.usual = (int)usual;   // (the pool's numbers are 32-bit)
+  // (the pool's numbers are 32-bit)
+  if (splits > usual && S <= MOST_POOLED && pairs <= (1 << 20) && pairs * splits < (1LL << 31)) p.usual = (int)usual;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == MELGPT_F32) return D == 64 ? launch<float, 64>(p, st) : launch<float, 128>(p, st);

@@ -1227,8 +1227,8 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     as they were in a given `out`, zero in a new one (lse -inf, low 0).  scale: 1 / sqrt(D) unless given.  want_low: -> (out,
     lse, low), low what rounding out to 16 bits took from it (None for f32), for packed_attn_bwd.  Values that are not finite
     reach the queries that see them and no others.  max_length: the keys of the longest sequence, where the caller knows them;
-    it only decides how far the keys of a row are shared out (without it one sequence of a batch with a past may have half of
-    all keys; giving it spares a batch of like lengths up to 10 us)."""
+    it only decides how far the keys of a row are shared out (without it one of 32 or more sequences with a past may have half
+    of all keys; giving it spares a batch of like lengths some 6 us)."""
     i = _device_of(q)
     if i != _current_device():
         return _on(i, packed_attn_fwd, q, k, v, cu_q, cu_k, scale=scale, out=out, want_low=want_low, max_length=max_length)
@@ -1249,7 +1249,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, scale=None, out=None, want_low=
     low = torch.empty((Mq, Hq, D), dtype=q.dtype, device=q.device) if want_low and dt != _ffi.F32 else None
     splits, ws = 1, None
     if low is None and dt != _ffi.F32:
-        longest = int(max_length) if max_length is not None else Mk // 2 if Mk > Mq else 0
+        longest = int(max_length) if max_length is not None else Mk // 2 if Mk > Mq and S >= 32 else 0
         splits = _ffi.lib().melgpt_packed_attn_splits_for(Mq, Mk, S, Hq, D, dt, longest)
         if splits > 1:   # (a buffer of the call's own: two captured graphs never share it)
             ws = torch.empty(splits * Hq * Mq * (D + 2), dtype=torch.float32, device=q.device)

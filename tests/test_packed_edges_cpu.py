@@ -143,7 +143,8 @@ def test_shares_of_a_long_sequence_in_a_large_batch():
 
     f = _ffi.lib().melgpt_paged_attn_splits
     assert f(256, 32, 8, 100000) == 25 and f(512, 32, 8, 100000) == 25 and f(64, 32, 8, 100000) == 25     # 4096 keys each
-    assert f(256, 32, 8, 4096) == 1 and f(64, 32, 8, 8192) == 4 and f(3, 32, 4, 131072) == 128            # as without long ones
+    assert f(256, 32, 8, 4096) == f(256, 32, 8, 16384) == 1 and f(64, 32, 8, 8192) == 4 and f(3, 32, 4, 131072) == 128   # as without
+    assert f(513, 32, 8, 100000) == 1
     for S in (1, 64, 1000, 5000, 100000):
         for Hq, Hk in ((32, 8), (16, 16), (1, 1)):
             n, usual = f(S, Hq, Hk, 1 << 30), -(-2048 // (S * Hk))

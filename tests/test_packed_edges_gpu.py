@@ -236,13 +236,13 @@ def test_output_and_its_remainder_fit_each_other(D):
 
 
 # ------------------------------------------------------------------- a few long sequences in a large batch: decode
-def _cached(lens, Hq, Hk, D, page, dtype, seed):
+def _cached(lens, Hq, Hk, D, page, dtype, seed, width=0):
     g = torch.Generator(device=DEV)
     g.manual_seed(seed)
     need = [-(-n // page) for n in lens]
     kp, vp = [torch.randn(sum(need) + 1, Hk, page, D, generator=g, device=DEV).to(dtype) for _ in range(2)]
     order = torch.randperm(sum(need), generator=g, device=DEV).to(torch.int32)
-    table, at = torch.full((len(lens), max(need)), -1, dtype=torch.int32, device=DEV), 0
+    table, at = torch.full((len(lens), max(max(need), width // page)), -1, dtype=torch.int32, device=DEV), 0
     for s, n in enumerate(need):
         table[s, :n] = order[at:at + n]
         at += n
@@ -263,11 +263,11 @@ def _decode_reference(q, kp, vp, table, lens, which):
         yield s, (p * v).sum(0), lse, (p * v.abs()).sum(0), size
 
 
-def _check_decode(lens, Hq, Hk, D, page, dtype, seed, which=None, max_length=None):
+def _check_decode(lens, Hq, Hk, D, page, dtype, seed, which=None, max_length=None, width=0):
     import packed_ref as R
     from melspec_gpt_vqvae_amd import ops
 
-    args = _cached(lens, Hq, Hk, D, page, dtype, seed)
+    args = _cached(lens, Hq, Hk, D, page, dtype, seed, width)
     out, lse = ops.paged_attn_decode(*args, max_length=max_length)
     h = R.half_step(dtype)
     for s, o, l, size, score in _decode_reference(*args[:4], lens, range(len(lens)) if which is None else which):
@@ -284,29 +284,30 @@ def test_long_sequences_in_a_large_batch_of_short_ones(Hq, Hk, D, dtype):
     from melspec_gpt_vqvae_amd import _ffi
 
     lens = [7 * i % 90 for i in range(300)]
-    for s, n in ((0, 4097), (5, 9000), (64, 4096), (127, 12300), (299, 8193)):      # (first, last, at a wave's end, two in one wave)
+    for s, n in ((0, 4097), (5, 9000), (64, 4096), (127, 18000), (299, 8193)):      # (first, last, at a wave's end, two in one wave)
         lens[s] = n
-    assert _ffi.lib().melgpt_paged_attn_splits(300, Hq, Hk, 12304) == 4 and 300 * Hk >= 2048
+    assert _ffi.lib().melgpt_paged_attn_splits(300, Hq, Hk, 18000) == 5 and 300 * Hk >= 2048
     _check_decode(lens, Hq, Hk, D, 16, _dt(dtype), 1)
-    _check_decode(lens, Hq, Hk, D, 16, _dt(dtype), 1, which=[0, 5, 127, 299], max_length=5000)      # (a wrong hint: two shares at most)
+    _check_decode(lens, Hq, Hk, D, 16, _dt(dtype), 1, which=[0, 5, 127, 299], max_length=5000)      # (wrong hints: one share each,
+    _check_decode(lens[:128] + [60000] + lens[129:], Hq, Hk, D, 16, _dt(dtype), 1, which=[5, 127, 128], max_length=17000)   # larger ones)
 
 
 def test_more_long_shares_than_workgroups_that_look_for_them():
     lens = [4500 + i for i in range(130)]                          # 130 sequences of 16 heads, a second share each: 2080
-    _check_decode(lens, 16, 16, 64, 64, _dt("half"), 2, which=[0, 1, 63, 64, 65, 100, 128, 129])
+    _check_decode(lens, 16, 16, 64, 64, _dt("half"), 2, which=[0, 1, 63, 64, 65, 100, 128, 129], max_length=20000, width=20000)
 
 
 def test_long_sequences_with_two_groups_of_heads():
     lens = [50] * 70
     lens[3] = lens[69] = 5000
-    _check_decode(lens, 17 * 16, 16, 64, 32, _dt("half"), 3, which=[0, 3, 68, 69])
+    _check_decode(lens, 17 * 16, 16, 64, 32, _dt("half"), 3, which=[0, 3, 68, 69], width=20000)
 
 
 def test_captured_decode_of_growing_lengths():
     """one graph, lengths on either side of a share of 4096 keys from replay to replay"""
     from melspec_gpt_vqvae_amd import ops
 
-    (q, kp, vp, table, lengths), _, _ = _check_decode([9000] * 3 + [100] * 300, 8, 8, 64, 64, _dt("half"), 4, which=[1, 200])
+    (q, kp, vp, table, lengths), _, _ = _check_decode([9000] * 3 + [100] * 300, 8, 8, 64, 64, _dt("half"), 4, which=[1, 200], width=20000)
     step = lambda: ops.paged_attn_decode(q, kp, vp, table, lengths)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -329,7 +330,7 @@ def _shares(lens_q, lens_k, Hq, D, max_length=None):
     from melspec_gpt_vqvae_amd import _ffi
 
     a = (sum(lens_q), sum(lens_k), len(lens_q), Hq, D, _ffi.BF16)
-    longest = max_length if max_length is not None else a[1] // 2 if a[1] > a[0] else 0
+    longest = max_length if max_length is not None else a[1] // 2 if a[1] > a[0] and len(lens_q) >= 32 else 0
     return _ffi.lib().melgpt_packed_attn_splits(*a), _ffi.lib().melgpt_packed_attn_splits_for(*a, longest)
 
 
