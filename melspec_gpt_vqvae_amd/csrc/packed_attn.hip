@@ -480,7 +480,7 @@ __device__ __forceinline__ int pool_share(const PackedParams& p, int every) {
 // Those beyond the usual ones are taken by a pool of workgroups, which find them from the lengths: number e, e + POOLED, .. of
 // all in order of sequence, row tile (the last first), share and query head.  128 queries over 16000 keys among 63 single ones
 // over 64, 8 heads of 128: 252 us without, 94 with; 32 heads 255 / 105, 16 of 64 201 / 65.  Where there is no long one the two
-// launches more cost some 6 us (100 sequences of 2 queries over 300 keys, 8 heads of 64: 21 / 28; of 1 over 1000, 16: 93 / 96).
+// launches more cost some 6 us (100 sequences of 2 queries over 300 keys, 8 heads of 64: 21 / 28; of 1 over 1000, 16: 99 / 106).
 // All lanes of a wave.
 // s0, e: where the search stands (number e of those from sequence s0 on); it goes on there for the next.
 __device__ __forceinline__ bool any_pooled(const PackedParams& p, int lane) {
